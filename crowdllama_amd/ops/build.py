@@ -17,6 +17,10 @@ OPS_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(OPS_DIR, "csrc")
 ARCH = os.environ.get("CLA_GFX_ARCH", "gfx950")
 
+# gfx950's packed float32 instructions (which -O3 forms by itself) have given
+# wrong results now and then: no kernel is compiled with them
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 SOURCES = ["gguf.cpp", "engine.cpp", "testutil.cpp", "bindings.cpp",
            "kernels.hip", "mfma_probe.hip", "gemm.hip", "gemm_i8.hip",
            "tokenizer.cpp"]
@@ -31,7 +35,8 @@ def so_path() -> str:
 
 
 def _newest_src_mtime() -> float:
-    return max(os.path.getmtime(os.path.join(CSRC, s)) for s in SOURCES)
+    return max(os.path.getmtime(os.path.join(CSRC, s))
+               for s in os.listdir(CSRC))
 
 
 def needs_build() -> bool:
@@ -57,8 +62,7 @@ def build(verbose: bool = True, force: bool = False) -> str:
                "-I", CSRC, "-I", py_inc, "-I", pybind11.get_include(),
                "-c", os.path.join(CSRC, src), "-o", obj]
         if src.endswith(".hip"):
-            cmd.insert(1, "-x")
-            cmd.insert(2, "hip")
+            cmd[1:1] = ["-x", "hip", *HIP_FLAGS]
         if verbose:
             print("[ops.build]", " ".join(cmd), file=sys.stderr)
         procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE,
