@@ -23,7 +23,7 @@ HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 SOURCES = ["gguf.cpp", "engine.cpp", "testutil.cpp", "bindings.cpp",
            "kernels.hip", "mfma_probe.hip", "gemm.hip", "gemm_i8.hip",
-           "tokenizer.cpp"]
+           "kvcache.hip", "kv_bindings.cpp", "tokenizer.cpp"]
 
 
 def _ext_suffix() -> str:

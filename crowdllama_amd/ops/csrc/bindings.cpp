@@ -32,10 +32,12 @@ std::vector<float> test_rccl_graph_1rank(const std::vector<float>&);
 void launch_gemm_i8_test(const void*, const void*, const float*, float*,
                          int, int, int, int, size_t, size_t, int);
 void launch_mfma_probe_i8_test(const int8_t*, const int8_t*, int32_t*);
+void bind_kv(py::module_& m);
 }
 
 PYBIND11_MODULE(_core, m) {
     m.doc() = "crowdllama-amd MI355X (gfx950) HIP inference engine";
+    bind_kv(m);
 
     m.def("nccl_unique_id", [] {
         ncclUniqueId id;

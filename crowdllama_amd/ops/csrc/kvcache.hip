@@ -1,0 +1,1206 @@
+// The paged KV cache's operators for gfx950 (interface: kvcache.h).
+//
+//   append   rotary positions, new keys and values into the pages
+//   attend   one new token over the cache, split over its length and joined;
+//            each place's weight is added to the cache's mass
+//   observe  the weight that a prompt's rows gave to the places
+//   evict    which places stay once a sequence is too long, by mass
+//
+// Keys and values are 16-bit; queries are of the pool's type or float32 (over
+// a bfloat16 pool). All scores, maxima, sums and masses are float32. Products
+// run on v_mfma_f32_16x16x32: float32 operands go in as sums of 16-bit pieces
+// (a float32 is three bfloat16 exactly), so nothing is lost to the matrix
+// cores' types; the pieces cost matrix instructions only, and attention of
+// one token has far more of those than it has bandwidth.
+#include <algorithm>
+
+#include "common.h"
+#include "kvcache.h"
+
+namespace cla {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <class To, class From>
+__device__ __forceinline__ To bits(const From& x) {
+    static_assert(sizeof(To) == sizeof(From), "same size");
+    return __builtin_bit_cast(To, x);
+}
+
+// ------------------------------------------------------------- 16-bit types
+
+struct Bf16 {
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            bits<bf16x8>(a), bits<bf16x8>(b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const bf16x2 v = {(__bf16)x, (__bf16)y};
+        return bits<uint32_t>(v);
+    }
+    static __device__ __forceinline__ f32x2 unpack(uint32_t w) {
+        return f32x2{bits<float>(w << 16), bits<float>(w & 0xFFFF0000u)};
+    }
+    // The leading 8 bits of x and y as a packed pair; x and y become what
+    // is left, without error. Three calls take all 24 bits.
+    static __device__ __forceinline__ uint32_t piece(float& x, float& y) {
+        const uint32_t ux = bits<uint32_t>(x) & 0xFFFF0000u;
+        const uint32_t uy = bits<uint32_t>(y) & 0xFFFF0000u;
+        x -= bits<float>(ux);
+        y -= bits<float>(uy);
+        return (ux >> 16) | uy;
+    }
+};
+
+struct F16 {
+    static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            bits<f16x8>(a), bits<f16x8>(b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ uint32_t pack(float x, float y) {
+        const f16x2 v = {(_Float16)x, (_Float16)y};
+        return bits<uint32_t>(v);
+    }
+    static __device__ __forceinline__ f32x2 unpack(uint32_t w) {
+        const f16x2 v = bits<f16x2>(w);
+        return f32x2{(float)v.x, (float)v.y};
+    }
+    // As above, 11 bits a call; for values of [0, 1] (attention weights),
+    // whose remainder float16 holds to 2^-25 of the largest.
+    static __device__ __forceinline__ uint32_t piece(float& x, float& y) {
+        const f16x2 v = {(_Float16)x, (_Float16)y};
+        x -= (float)v.x;
+        y -= (float)v.y;
+        return bits<uint32_t>(v);
+    }
+};
+
+struct Pages {
+    uint16_t* pool;
+    int64_t page_stride, table_stride;
+    const int32_t* table;
+    int32_t pages, max_pages, page;
+    uint32_t per16, magic;   // page / 16, and ceil(2^32 / that)
+
+    // Where 16 places from p on (p a multiple of 16) lie: the first one's
+    // row; null where the table or the pool has no such page.
+    __device__ __forceinline__ uint16_t* rows16(int b, int p, int head,
+                                                int dim) const {
+        const uint32_t p16 = (uint32_t)p >> 4;
+        const uint32_t i = per16 == 1 ? p16 : __umulhi(p16, magic);
+        const int32_t pg = kv_page_of(table + (int64_t)b * table_stride, i,
+                                      max_pages, pages);
+        if (pg < 0) return nullptr;
+        return pool + (int64_t)pg * page_stride
+               + (int64_t)head * 2 * page * dim
+               + (int64_t)(p16 - i * per16) * 16 * dim;
+    }
+};
+
+Pages pages_of(const KvPages& kv) {
+    Pages p;
+    p.pool = reinterpret_cast<uint16_t*>(kv.pool);
+    p.page_stride = kv.page_stride;
+    p.table_stride = kv.table_stride;
+    p.table = kv.table;
+    p.pages = kv.pages;
+    p.max_pages = kv.max_pages;
+    p.page = kv.page;
+    p.per16 = (uint32_t)kv.page / 16;
+    // exact for p16 * per16 < 2^32: pages have at most 1024 places and
+    // sequences at most 2^30 (checked by check_pages)
+    p.magic = p.per16 > 1 ? (uint32_t)((0xFFFFFFFFull + p.per16) / p.per16) : 0;
+    return p;
+}
+
+void check_pages(const KvPages& kv, int q_heads, int reach) {
+    if (kv.dim != 64 && kv.dim != 96 && kv.dim != 128)
+        throw std::runtime_error("head_dim must be 64, 96 or 128");
+    if (kv.page < 16 || kv.page > 1024 || kv.page % 16)
+        throw std::runtime_error(
+            "page size must be a multiple of 16, at most 1024");
+    if (kv.type != KVT::BF16 && kv.type != KVT::F16)
+        throw std::runtime_error("the pool must be bfloat16 or float16");
+    if (kv.slots < 1 || kv.kv_heads < 1 || kv.pages < 1 || kv.max_pages < 1)
+        throw std::runtime_error("empty pool or page table");
+    if (reach < 0 || reach > (1 << 30) ||
+        (int64_t)reach > (int64_t)kv.max_pages * kv.page)
+        throw std::runtime_error("a sequence may have at most 2^30 places");
+    if ((int64_t)kv.slots * kv.kv_heads * (reach / 128 + 1) >= (1ll << 31))
+        throw std::runtime_error("too many places in all");
+    if (q_heads && (q_heads % kv.kv_heads || q_heads / kv.kv_heads > 16))
+        throw std::runtime_error(
+            "query heads must be 1 to 16 times the kv heads");
+}
+
+void check_launch() {
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+        throw std::runtime_error(std::string("HIP error: ") +
+                                 hipGetErrorString(e));
+}
+
+// Which sequence row t of packed rows belongs to: the last b whose
+// starts[b] <= t. slots: behind the last sequence. All 64 lanes take part.
+__device__ __forceinline__ int sequence_of(const int32_t* starts, int slots,
+                                           int t) {
+    const int lane = threadIdx.x & 63;
+    int before = 0;
+    for (int base = 0; base <= slots; base += 64) {
+        const int i = base + lane;
+        before += __popcll(__ballot(i <= slots && starts[i] <= t));
+    }
+    return before - 1;
+}
+
+__device__ __forceinline__ float wave_xor_max(float x, int mask) {
+    return fmaxf(x, __shfl_xor(x, mask, 64));
+}
+__device__ __forceinline__ float wave_xor_sum(float x, int mask) {
+    return x + __shfl_xor(x, mask, 64);
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    return __builtin_amdgcn_exp2f(x);
+}
+
+// ------------------------------------------------------------------- append
+
+struct AppendArgs {
+    Pages kv;
+    KvHeads k, v, q, q_out;
+    KvRows mass, pos;
+    const int32_t *starts, *lens, *next_pos;
+    const float* inv_freq;
+    int32_t q_heads, kv_heads, slots, reach;
+};
+
+template <KVT T>
+__device__ __forceinline__ void load8(const void* p, int64_t at, float* x) {
+    if constexpr (T == KVT::F32) {
+        const f32x4* s = reinterpret_cast<const f32x4*>(
+            reinterpret_cast<const float*>(p) + at);
+        const f32x4 a = s[0], b = s[1];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) { x[i] = a[i]; x[4 + i] = b[i]; }
+    } else {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(
+            reinterpret_cast<const uint16_t*>(p) + at);
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const f32x2 f = T == KVT::BF16 ? Bf16::unpack(w[i])
+                                           : F16::unpack(w[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+
+template <KVT T>
+__device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
+    if constexpr (T == KVT::F32) {
+        f32x4* d = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(p) + at);
+        d[0] = f32x4{x[0], x[1], x[2], x[3]};
+        d[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+        u32x4 w;
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] = T == KVT::BF16 ? Bf16::pack(x[2 * i], x[2 * i + 1])
+                                  : F16::pack(x[2 * i], x[2 * i + 1]);
+        *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(p) + at) = w;
+    }
+}
+
+// grid (rows, parts) x 256. A workgroup takes one row's heads (q, k, v side
+// by side), 8 elements a thread and pass; the row's angles are shared by all
+// heads through LDS. position * inv_freq is taken and reduced in 64 bits: in
+// 32 it would be off by 2^-24 of the angle, 0.06 rad at position 10^6.
+template <KVT T, KVT C, int D>
+__global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
+    __shared__ float cs[D / 2], sn[D / 2];
+    const int t = blockIdx.x, tid = threadIdx.x;
+    int b = t, i = 0;
+    if (a.starts) {
+        b = sequence_of(a.starts, a.slots, t);
+        if (b >= 0 && b < a.slots) i = t - a.starts[b];
+    }
+    const bool mine = b >= 0 && b < a.slots;
+    const int64_t place = mine ? (int64_t)a.lens[b] + i : -1;
+    const int position = mine ? a.next_pos[b] + i : 0;
+    if (a.inv_freq && tid < D / 2) {
+        const double turn = (double)position * (double)a.inv_freq[tid];
+        const double whole = rint(turn * 0.15915494309189535);
+        const float rest = (float)fma(whole, -6.283185307179586, turn);
+        // rows behind the last sequence keep their queries as they are
+        sincosf(mine ? rest : 0.f, &sn[tid], &cs[tid]);
+    }
+    __syncthreads();
+
+    const bool stored = place >= 0 && place < a.reach;
+    int32_t page = -1;
+    int row = 0;
+    if (stored) {
+        page = kv_page_of(a.kv.table + (int64_t)b * a.kv.table_stride,
+                          place / a.kv.page, a.kv.max_pages, a.kv.pages);
+        row = (int)(place % a.kv.page);
+    }
+    constexpr int PER = D / 8;
+    const int heads = a.q_heads + 2 * a.kv_heads;
+    for (int it = blockIdx.y * 256 + tid; it < heads * PER;
+         it += gridDim.y * 256) {
+        const int head = it / PER, d = it % PER * 8;
+        const int kvh = head - a.q_heads;
+        if (kvh >= 0 && page < 0) continue;
+        const bool is_v = kvh >= a.kv_heads;
+        const KvHeads& src = kvh < 0 ? a.q : is_v ? a.v : a.k;
+        const int h = kvh < 0 ? head : is_v ? kvh - a.kv_heads : kvh;
+        float x[8];
+        load8<T>(src.data, t * src.row_stride + h * src.head_stride + d, x);
+        if (a.inv_freq && !is_v) {
+            #pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float c = cs[d / 2 + j], s = sn[d / 2 + j];
+                const float x0 = x[2 * j], x1 = x[2 * j + 1];
+                x[2 * j] = x0 * c - x1 * s;
+                x[2 * j + 1] = x0 * s + x1 * c;
+            }
+        }
+        if (kvh < 0)
+            store8<T>(a.q_out.data,
+                      t * a.q_out.row_stride + h * a.q_out.head_stride + d, x);
+        else
+            store8<C>(a.kv.pool,
+                      (int64_t)page * a.kv.page_stride
+                          + ((int64_t)h * 2 + is_v) * a.kv.page * D
+                          + (int64_t)row * D + d, x);
+    }
+    if (blockIdx.y == 0 && stored) {
+        for (int h = tid; h < a.kv_heads; h += 256) {
+            if (a.mass.data)
+                reinterpret_cast<float*>(a.mass.data)[
+                    b * a.mass.slot_stride + h * a.mass.head_stride + place] =
+                    0.f;
+            if (a.pos.data)
+                reinterpret_cast<int32_t*>(a.pos.data)[
+                    b * a.pos.slot_stride + h * a.pos.head_stride + place] =
+                    position;
+        }
+    }
+}
+
+// ------------------------------------------------------------------- attend
+
+constexpr int TILE = 32;          // places a wave takes at a time
+constexpr int WAVES = 4;
+constexpr int UNIT = TILE * WAVES;
+
+// How many workgroups the whole of the batch's places are split into, about.
+constexpr int ATTEND_WGS = 512;
+
+struct AttendArgs {
+    Pages kv;
+    KvHeads q, out;
+    KvRows mass;
+    const int32_t* lens;
+    int32_t add, q_heads, kv_heads, slots, reach, target;
+    float scale2;             // scale * log2(e)
+    float* scores;            // [slots][q heads][ld] in units of log2
+    int64_t ld;
+    float* part_o;            // [workgroup][G][D], relative to part_m
+    float* part_ml;           // [workgroup][G][2]
+};
+
+// The lengths on the device decide how the work is split: every kv head's
+// places are cut into equally many units of 128 for each workgroup, as many
+// as make about `target` workgroups of all of them. A ragged batch's long
+// sequences get more workgroups than its short ones, and the host needs no
+// length. Workgroup `id` takes part j of n of (b, head).
+struct Part {
+    int b, head, j, n, len, first, lo, hi;
+};
+
+__device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
+                                          Part& p) {
+    const int lane = threadIdx.x & 63;
+    int all = 0;
+    for (int base = 0; base < a.slots; base += 64) {
+        const int b = base + lane;
+        const int len = b < a.slots
+            ? kv_clamp_len(a.lens[b] + a.add, a.reach) : 0;
+        all += (len + UNIT - 1) / UNIT;
+    }
+    #pragma unroll
+    for (int m = 32; m; m >>= 1) all += __shfl_xor(all, m, 64);
+    const int per = max(1u, ((uint32_t)all * a.kv_heads + a.target - 1)
+                                / (uint32_t)a.target);
+    int before = 0;
+    for (int base = 0; base < a.slots; base += 64) {
+        const int b = base + lane;
+        const int len = b < a.slots
+            ? kv_clamp_len(a.lens[b] + a.add, a.reach) : 0;
+        const int units = (len + UNIT - 1) / UNIT;
+        const int n = max(1u, (uint32_t)(units + per - 1) / (uint32_t)per);
+        int upto = b < a.slots ? n * a.kv_heads : 0;
+        #pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int x = __shfl_up(upto, m, 64);
+            if (lane >= m) upto += x;
+        }
+        const uint64_t over = __ballot(before + upto > id);
+        if (over) {
+            const int at = __builtin_ctzll(over);
+            p.b = base + at;
+            p.len = __shfl(len, at, 64);
+            p.n = __shfl(n, at, 64);
+            const int units_b = (p.len + UNIT - 1) / UNIT;
+            const int rest = id - before
+                - (__shfl(upto, at, 64) - p.n * a.kv_heads);
+            p.head = rest / p.n;
+            p.j = rest % p.n;
+            p.first = id - p.j;
+            // n = ceil(units / per) parts of ceil(units / n): none is empty
+            const int each = (units_b + p.n - 1) / p.n * UNIT;
+            p.lo = p.j * each;
+            p.hi = min(p.lo + each, p.len);
+            return true;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return false;
+}
+
+// The queries of one kv head as the B operand of 16x16x32 products, in NQ
+// pieces: column n is query head n (zero past the last), k runs over d.
+template <class C, int NQ, int D>
+__device__ __forceinline__ void load_q(const void* q, int64_t at, bool there,
+                                       int g, u32x4 (*f)[D / 32]) {
+    #pragma unroll
+    for (int kk = 0; kk < D / 32; kk++) {
+        const int64_t d = at + kk * 32 + g * 8;
+        if constexpr (NQ == 1) {
+            f[0][kk] = there ? *reinterpret_cast<const u32x4*>(
+                reinterpret_cast<const uint16_t*>(q) + d) : u32x4{0, 0, 0, 0};
+        } else {
+            float x[8];
+            if (there) {
+                load8<KVT::F32>(q, d, x);
+            } else {
+                #pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = 0.f;
+            }
+            #pragma unroll
+            for (int s = 0; s < NQ; s++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++)
+                    f[s][kk][i] = C::piece(x[2 * i], x[2 * i + 1]);
+        }
+    }
+}
+
+// One wave's 32 places: keys as the A operand (two products of 16 places),
+// values as a lane's 8 places of EL elements.
+template <int D>
+struct Tile {
+    static constexpr int EL = D / 16;
+    u32x4 k[2][D / 32];
+    uint32_t v[8][EL / 2];
+};
+
+template <int D>
+__device__ __forceinline__ void load_tile(const uint16_t* r0,
+                                          const uint16_t* r1, int64_t to_v,
+                                          int n, int g, Tile<D>& t) {
+    constexpr int EL = D / 16;
+    #pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const uint16_t* r = u ? r1 : r0;
+        const uint16_t* kp = r + n * D + g * 8;
+        #pragma unroll
+        for (int kk = 0; kk < D / 32; kk++)
+            t.k[u][kk] = *reinterpret_cast<const u32x4*>(kp + kk * 32);
+        const uint16_t* vp = r + to_v + g * 4 * D + n * EL;
+        #pragma unroll
+        for (int j = 0; j < 4; j++) {
+            uint32_t* d = t.v[u * 4 + j];
+            if constexpr (EL == 8) {
+                const u32x4 w = *reinterpret_cast<const u32x4*>(vp + j * D);
+                d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
+            } else if constexpr (EL == 6) {
+                // 12 bytes at a multiple of 4
+                const uint32_t* s =
+                    reinterpret_cast<const uint32_t*>(vp + j * D);
+                d[0] = s[0]; d[1] = s[1]; d[2] = s[2];
+            } else {
+                const u32x2 w = *reinterpret_cast<const u32x2*>(vp + j * D);
+                d[0] = w.x; d[1] = w.y;
+            }
+        }
+    }
+}
+
+// One workgroup takes one part of one kv head's places, its four waves 32 at
+// a time in turn. S = K Q^T and O^T = V^T P^T, so that in both results a
+// lane's column is its query head: maximum, sum and rescaling stay in the
+// lane. S's rows (places) then are just the k index of the second product,
+// and V needs no transposition through LDS: a lane holds 8 places x EL
+// elements, and product e takes element e of each (MFMA row r is d = r*EL+e).
+//
+// Bound by the reads of K and V. Its scores go out as they are where a mass
+// is wanted, since the weights are known only once all parts are.
+template <class C, int NQ, int NP, int D, bool MASS>
+__global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
+    constexpr int EL = D / 16;
+    __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+    __shared__ float s_o[WAVES][16][D];
+    Part p;
+    if (!find_part(a, blockIdx.x, p)) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int G = a.q_heads / a.kv_heads;
+    const int head = p.head * G + n;
+
+    u32x4 q[NQ][D / 32];
+    load_q<C, NQ, D>(a.q.data,
+                     p.b * a.q.row_stride + head * a.q.head_stride, n < G, g,
+                     q);
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[EL];
+    #pragma unroll
+    for (int e = 0; e < EL; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float* scores = MASS && n < G
+        ? a.scores + ((int64_t)p.b * a.q_heads + head) * a.ld : nullptr;
+    const int64_t to_v = (int64_t)a.kv.page * D;
+
+    for (int p0 = p.lo + wave * TILE; p0 < p.hi; p0 += UNIT) {
+        const uint16_t* r0 = a.kv.rows16(p.b, p0, p.head, D);
+        const uint16_t* r1 = p0 + 16 < p.hi
+            ? a.kv.rows16(p.b, p0 + 16, p.head, D) : nullptr;
+        // places that are not there are read from the pool's first page,
+        // and count for nothing
+        Tile<D> t;
+        load_tile<D>(r0 ? r0 : a.kv.pool, r1 ? r1 : a.kv.pool, to_v, n, g, t);
+        const bool whole = r0 && r1 && p0 + TILE <= p.hi;
+        float s[8];
+        #pragma unroll
+        for (int u = 0; u < 2; u++) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int x = NQ - 1; x >= 0; x--)
+                #pragma unroll
+                for (int kk = 0; kk < D / 32; kk++)
+                    acc = C::mfma(t.k[u][kk], q[x][kk], acc);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) s[u * 4 + i] = acc[i] * a.scale2;
+        }
+        if (!whole) {
+            #pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int u = j >> 2;
+                const bool seen = (u ? r1 : r0) &&
+                    p0 + u * 16 + g * 4 + (j & 3) < p.hi;
+                if (!seen) {
+                    s[j] = -INFINITY;
+                    // what lies there may be anything: 0 * inf is NaN
+                    #pragma unroll
+                    for (int e = 0; e < EL / 2; e++) t.v[j][e] = 0;
+                }
+            }
+        }
+        if (MASS && scores) {
+            #pragma unroll
+            for (int u = 0; u < 2; u++)
+                *reinterpret_cast<f32x4*>(scores + p0 + u * 16 + g * 4) =
+                    f32x4{s[u * 4], s[u * 4 + 1], s[u * 4 + 2], s[u * 4 + 3]};
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                          fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        top = wave_xor_max(wave_xor_max(top, 16), 32);
+        if (__any(top > m)) {
+            const float now = fmaxf(m, top);
+            const float f = exp2_fast(m - now);   // 0 from -inf
+            m = now;
+            if (now > -INFINITY) {
+                l *= f;
+                #pragma unroll
+                for (int e = 0; e < EL; e++) o[e] *= f;
+            }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float w[8];
+        #pragma unroll
+        for (int j = 0; j < 8; j++) {
+            w[j] = exp2_fast(s[j] - ref);
+            l += w[j];
+        }
+        u32x4 pf[NP];
+        #pragma unroll
+        for (int x = 0; x < NP; x++)
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+                pf[x][i] = C::piece(w[2 * i], w[2 * i + 1]);
+        #pragma unroll
+        for (int e = 0; e < EL; e++) {
+            u32x4 vf;
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+                vf[i] = __builtin_amdgcn_perm(
+                    t.v[2 * i + 1][e >> 1], t.v[2 * i][e >> 1],
+                    (e & 1) ? 0x07060302u : 0x05040100u);
+            #pragma unroll
+            for (int x = NP - 1; x >= 0; x--) o[e] = C::mfma(vf, pf[x], o[e]);
+        }
+    }
+
+    // join the four waves; a lane's l is of its own places only
+    l = wave_xor_sum(wave_xor_sum(l, 16), 32);
+    if (g == 0) { s_m[wave][n] = m; s_l[wave][n] = l; }
+    #pragma unroll
+    for (int e = 0; e < EL; e++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            s_o[wave][n][(g * 4 + i) * EL + e] = o[e][i];
+    __syncthreads();
+    for (int x = tid; x < G * D; x += 256) {
+        const int h = x / D, d = x % D;
+        float top = s_m[0][h];
+        #pragma unroll
+        for (int w = 1; w < WAVES; w++) top = fmaxf(top, s_m[w][h]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, acc = 0.f;
+        #pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float f = exp2_fast(s_m[w][h] - ref);
+            sum += f * s_l[w][h];
+            acc += f * s_o[w][h][d];
+        }
+        if (p.n == 1) {
+            const float y = sum == 0.f ? 0.f : acc / sum;
+            const int64_t at = p.b * a.out.row_stride
+                + (int64_t)(p.head * G + h) * a.out.head_stride + d;
+            if constexpr (NQ == 1)
+                reinterpret_cast<uint16_t*>(a.out.data)[at] =
+                    (uint16_t)C::pack(y, 0.f);
+            else
+                reinterpret_cast<float*>(a.out.data)[at] = y;
+        } else {
+            a.part_o[((int64_t)blockIdx.x * G + h) * D + d] = acc;
+        }
+        if (d == 0) {
+            a.part_ml[((int64_t)blockIdx.x * G + h) * 2] = top;
+            a.part_ml[((int64_t)blockIdx.x * G + h) * 2 + 1] = sum;
+        }
+    }
+}
+
+// Join the parts: the same workgroups once more. Each makes its share of the
+// head's outputs (the parts' sums, in their order) and, from the scores, the
+// weights of its own places.
+template <class C, bool F32OUT, int D, bool MASS>
+__global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
+    __shared__ float s_m[16], s_r[16];
+    __shared__ float s_acc[256];
+    Part p;
+    if (!find_part(a, blockIdx.x, p)) return;
+    if (!MASS && p.n == 1) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int G = a.q_heads / a.kv_heads;
+    const float* ml = a.part_ml + (int64_t)p.first * G * 2;
+    for (int h = wave; h < G; h += WAVES) {
+        float m = -INFINITY, l = 0.f;
+        for (int j = lane; j < p.n; j += 64) {
+            const float mj = ml[((int64_t)j * G + h) * 2];
+            const float lj = ml[((int64_t)j * G + h) * 2 + 1];
+            const float now = fmaxf(m, mj);
+            const float ref = now == -INFINITY ? 0.f : now;
+            l = l * exp2_fast(m - ref) + lj * exp2_fast(mj - ref);
+            m = now;
+        }
+        float top = m;
+        #pragma unroll
+        for (int x = 32; x; x >>= 1) top = wave_xor_max(top, x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        l *= exp2_fast(m - ref);
+        #pragma unroll
+        for (int x = 32; x; x >>= 1) l = wave_xor_sum(l, x);
+        if (lane == 0) { s_m[h] = ref; s_r[h] = l == 0.f ? 0.f : 1.f / l; }
+    }
+    __syncthreads();
+    if (p.n > 1) {
+        // outputs [j * each, ...) of the head's G * D, `lanes` threads each
+        const int each = (G * D + p.n - 1) / p.n;
+        const int lo = p.j * each, hi = min(lo + each, G * D);
+        const float* po = a.part_o + (int64_t)p.first * G * D;
+        for (int x0 = lo; x0 < hi; x0 += 8) {
+            const int x = x0 + (tid & 7), y = tid >> 3;
+            float acc = 0.f;
+            if (x < hi) {
+                const int h = x / D;
+                const float ref = s_m[h];
+                for (int j = y; j < p.n; j += 32)
+                    acc += po[(int64_t)j * G * D + x]
+                        * exp2_fast(ml[((int64_t)j * G + h) * 2] - ref);
+            }
+            s_acc[tid] = acc;
+            __syncthreads();
+            #pragma unroll
+            for (int m = 128; m >= 8; m >>= 1) {
+                if (tid < m) s_acc[tid] += s_acc[tid + m];
+                __syncthreads();
+            }
+            if (tid < 8 && x < hi) {
+                const int h = x / D;
+                const float v = s_acc[tid] * s_r[h];
+                const int64_t at = p.b * a.out.row_stride
+                    + (int64_t)(p.head * G + h) * a.out.head_stride + x % D;
+                if constexpr (F32OUT)
+                    reinterpret_cast<float*>(a.out.data)[at] = v;
+                else
+                    reinterpret_cast<uint16_t*>(a.out.data)[at] =
+                        (uint16_t)C::pack(v, 0.f);
+            }
+            __syncthreads();
+        }
+    }
+    if constexpr (MASS) {
+        float* mass = reinterpret_cast<float*>(a.mass.data)
+            + p.b * a.mass.slot_stride + p.head * a.mass.head_stride;
+        const float* sc = a.scores
+            + ((int64_t)p.b * a.q_heads + p.head * G) * a.ld;
+        for (int x = p.lo + tid; x < p.hi; x += 256) {
+            float sum = 0.f;
+            for (int h = 0; h < G; h++)
+                sum += exp2_fast(sc[h * a.ld + x] - s_m[h]) * s_r[h];
+            mass[x] += sum;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ observe
+
+struct ObserveArgs {
+    Pages kv;
+    KvHeads q;
+    KvRows mass;
+    const int32_t *starts, *lens;
+    int32_t q_heads, kv_heads, slots, rows, reach;
+    float scale2;
+    float* lse;        // [q heads][rows]: log2 of the sum of 2^scores
+};
+
+// A sequence's rows as the kernels see them: r = i * G + h, query head h of
+// row i, so that one pass over the keys serves the kv head's queries.
+struct Seq {
+    int b, t0, m, len;   // its first packed row, its rows, its places
+};
+
+__device__ __forceinline__ Seq sequence_at(const ObserveArgs& a, int b) {
+    Seq s;
+    s.b = b;
+    s.t0 = max(0, min(a.starts[b], a.rows));
+    s.m = max(0, min(a.starts[b + 1], a.rows) - s.t0);
+    s.len = kv_clamp_len(a.lens[b], a.reach);
+    return s;
+}
+
+// Pass 1, grid (row blocks, kv heads): 16 * RW rows a wave, over all the
+// places that they see. Each lane keeps a maximum and a sum of its own for
+// each of its columns; they meet at the end.
+template <class C, int NQ, int D, int RW>
+__global__ __launch_bounds__(256) void k_kv_observe_sums(ObserveArgs a) {
+    constexpr int ROWS = 16 * RW * WAVES;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
+    const int G = a.q_heads / a.kv_heads;
+    // which sequence's block this is
+    int id = blockIdx.x, b = 0;
+    Seq s;
+    for (;; b++) {
+        if (b == a.slots) return;
+        s = sequence_at(a, b);
+        const int blocks = (s.m * G + ROWS - 1) / ROWS;
+        if (id < blocks) break;
+        id -= blocks;
+    }
+    const int r0 = id * ROWS + wave * 16 * RW;
+    if (r0 >= s.m * G) return;
+
+    u32x4 q[RW][NQ][D / 32];
+    float m[RW], l[RW];
+    int seen[RW];          // places that the lane's column sees
+    #pragma unroll
+    for (int w = 0; w < RW; w++) {
+        const int r = r0 + w * 16 + n, i = r / G, h = r % G;
+        const bool there = r < s.m * G;
+        load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
+                             + (int64_t)(head * G + h) * a.q.head_stride,
+                         there, g, q[w]);
+        m[w] = -INFINITY;
+        l[w] = 0.f;
+        seen[w] = there ? s.len - s.m + i + 1 : 0;
+    }
+    const int r_last = min(r0 + 16 * RW, s.m * G) - 1;
+    const int least = s.len - s.m + r0 / G + 1;
+    const int most = s.len - s.m + r_last / G + 1;
+    for (int p0 = 0; p0 < most; p0 += 16) {
+        const uint16_t* rows = a.kv.rows16(b, p0, head, D);
+        if (!rows) continue;
+        u32x4 k[D / 32];
+        #pragma unroll
+        for (int kk = 0; kk < D / 32; kk++)
+            k[kk] = *reinterpret_cast<const u32x4*>(
+                rows + n * D + kk * 32 + g * 8);
+        #pragma unroll
+        for (int w = 0; w < RW; w++) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int x = NQ - 1; x >= 0; x--)
+                #pragma unroll
+                for (int kk = 0; kk < D / 32; kk++)
+                    acc = C::mfma(k[kk], q[w][x][kk], acc);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                acc[i] *= a.scale2;
+                if (p0 + 16 > least && p0 + g * 4 + i >= seen[w])
+                    acc[i] = -INFINITY;
+            }
+            const float top = fmaxf(fmaxf(acc[0], acc[1]),
+                                    fmaxf(acc[2], acc[3]));
+            const float now = fmaxf(m[w], top);
+            const float ref = now == -INFINITY ? 0.f : now;
+            l[w] *= exp2_fast(m[w] - ref);
+            m[w] = now;
+            #pragma unroll
+            for (int i = 0; i < 4; i++) l[w] += exp2_fast(acc[i] - ref);
+        }
+    }
+    #pragma unroll
+    for (int w = 0; w < RW; w++) {
+        const float top = wave_xor_max(wave_xor_max(m[w], 16), 32);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = l[w] * exp2_fast(m[w] - ref);
+        sum = wave_xor_sum(wave_xor_sum(sum, 16), 32);
+        const int r = r0 + w * 16 + n;
+        if (g == 0 && r < s.m * G)
+            a.lse[(int64_t)(head * G + r % G) * a.rows + s.t0 + r / G] =
+                sum == 0.f ? INFINITY : ref + __log2f(sum);
+    }
+}
+
+// Pass 2, grid (place blocks, kv heads, slots): 16 * PW places a wave, over
+// all rows that see them; a lane sums its columns' weights for its places.
+template <class C, int NQ, int D, int PW>
+__global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
+    const int G = a.q_heads / a.kv_heads;
+    const Seq s = sequence_at(a, blockIdx.z);
+    const int p0 = (blockIdx.x * WAVES + wave) * 16 * PW;
+    if (p0 >= s.len || s.m == 0) return;
+    u32x4 k[PW][D / 32];
+    bool there[PW];
+    #pragma unroll
+    for (int u = 0; u < PW; u++) {
+        const uint16_t* rows = p0 + u * 16 < s.len
+            ? a.kv.rows16(s.b, p0 + u * 16, head, D) : nullptr;
+        there[u] = rows != nullptr;
+        if (!rows) rows = a.kv.pool;
+        #pragma unroll
+        for (int kk = 0; kk < D / 32; kk++)
+            k[u][kk] = *reinterpret_cast<const u32x4*>(
+                rows + n * D + kk * 32 + g * 8);
+    }
+    f32x4 sum[PW];
+    #pragma unroll
+    for (int u = 0; u < PW; u++) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int i0 = max(0, p0 - (s.len - s.m));   // the first row that sees p0
+    const int R = s.m * G;
+    for (int r0 = i0 * G / 16 * 16; r0 < R; r0 += 16) {
+        const int r = r0 + n, i = r / G, h = r % G;
+        u32x4 q[NQ][D / 32];
+        load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
+                             + (int64_t)(head * G + h) * a.q.head_stride,
+                         r < R, g, q);
+        const float lse = r < R
+            ? a.lse[(int64_t)(head * G + h) * a.rows + s.t0 + i] : INFINITY;
+        const int seen = r < R ? s.len - s.m + i + 1 : 0;
+        const bool whole = r0 + 16 <= R &&
+            p0 + 16 * PW <= s.len - s.m + r0 / G + 1;
+        #pragma unroll
+        for (int u = 0; u < PW; u++) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int x = NQ - 1; x >= 0; x--)
+                #pragma unroll
+                for (int kk = 0; kk < D / 32; kk++)
+                    acc = C::mfma(k[u][kk], q[x][kk], acc);
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float w = exp2_fast(fmaf(acc[e], a.scale2, -lse));
+                sum[u][e] += whole || p0 + u * 16 + g * 4 + e < seen ? w : 0.f;
+            }
+        }
+    }
+    float* mass = reinterpret_cast<float*>(a.mass.data)
+        + s.b * a.mass.slot_stride + head * a.mass.head_stride;
+    #pragma unroll
+    for (int u = 0; u < PW; u++)
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float w = sum[u][e];
+            #pragma unroll
+            for (int x = 1; x < 16; x <<= 1) w = wave_xor_sum(w, x);
+            const int p = p0 + u * 16 + g * 4 + e;
+            if (n == 0 && p < s.len && there[u]) mass[p] += w;
+        }
+}
+
+// -------------------------------------------------------------------- evict
+
+struct EvictArgs {
+    Pages kv;
+    int64_t layer_stride;
+    KvLayers mass, pos, mass_out, pos_out;
+    const int32_t *lens, *next_pos;
+    int32_t* lens_out;
+    int32_t layers, slots, kv_heads, keep, recent, limit, reach, most;
+    int32_t *count, *dst, *src;    // [rows], [rows][most] twice
+};
+
+__device__ __forceinline__ int64_t row_at(const KvLayers& t, int layer, int b,
+                                          int h) {
+    return layer * t.layer_stride + b * t.slot_stride + h * t.head_stride;
+}
+
+// Sum over the workgroup; red holds one value a wave.
+__device__ __forceinline__ int block_sum(int x, int* red) {
+    #pragma unroll
+    for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < 16; w++) all += red[w];
+    return all;
+}
+
+// Pass 1, one workgroup of 1024 a row (layer, sequence, kv head): which
+// places stay, and who moves where. The keep-th largest key is found bit by
+// bit, counting the keys at or above each candidate; then one walk in the
+// order of places numbers the free ones and those that come into them.
+__global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
+    __shared__ int red[16];
+    __shared__ int tot[3][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x;
+    const int h = row % a.kv_heads, b = row / a.kv_heads % a.slots,
+              layer = row / a.kv_heads / a.slots;
+    const float* mass = reinterpret_cast<const float*>(a.mass.data)
+        + row_at(a.mass, layer, b, h);
+    const int32_t* pos = reinterpret_cast<const int32_t*>(a.pos.data)
+        + row_at(a.pos, layer, b, h);
+    float* mass_out = reinterpret_cast<float*>(a.mass_out.data)
+        + row_at(a.mass_out, layer, b, h);
+    int32_t* pos_out = reinterpret_cast<int32_t*>(a.pos_out.data)
+        + row_at(a.pos_out, layer, b, h);
+    const int len = kv_clamp_len(a.lens[b], a.reach);
+    if (mass_out != mass)
+        for (int p = tid; p < a.reach; p += 1024) mass_out[p] = mass[p];
+    if (pos_out != pos)
+        for (int p = tid; p < a.reach; p += 1024) pos_out[p] = pos[p];
+    if (len <= a.limit) {
+        if (tid == 0) a.count[row] = -1;
+        return;
+    }
+    const int64_t late = (int64_t)a.next_pos[b] - a.recent;
+    auto key_at = [&](int p) {
+        return kv_rank_key(mass[p], pos[p] >= late);
+    };
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t at = least | (1u << bit);
+        int c = 0;
+        for (int p = tid; p < len; p += 1024) c += key_at(p) >= at;
+        if (block_sum(c, red) >= a.keep) least = at;
+    }
+    int c = 0;
+    for (int p = tid; p < len; p += 1024) c += key_at(p) > least;
+    const int ties = a.keep - block_sum(c, red);   // of these, the first ones
+
+    int32_t* dst = a.dst + (int64_t)row * a.most;
+    int32_t* src = a.src + (int64_t)row * a.most;
+    int equal = 0, free = 0, come = 0;             // so far, in all places
+    const uint64_t below = (1ull << lane) - 1;
+    for (int base = 0; base < len; base += 1024) {
+        const int p = base + tid;
+        const uint32_t k = p < len ? key_at(p) : 0;
+        const bool eq = p < len && k == least;
+        const uint64_t eqs = __ballot(eq);
+        __syncthreads();
+        if (lane == 0) tot[0][wave] = __popcll(eqs);
+        __syncthreads();
+        int rank = equal + __popcll(eqs & below);
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) rank += tot[0][w];
+            equal += tot[0][w];
+        }
+        const bool stays = p < len && (k > least || (eq && rank < ties));
+        const bool is_free = p < len && p < a.keep && !stays;
+        const bool comes = stays && p >= a.keep;
+        const uint64_t fs = __ballot(is_free), cs = __ballot(comes);
+        if (lane == 0) {
+            tot[1][wave] = __popcll(fs);
+            tot[2][wave] = __popcll(cs);
+        }
+        __syncthreads();
+        int fr = free + __popcll(fs & below), cr = come + __popcll(cs & below);
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) { fr += tot[1][w]; cr += tot[2][w]; }
+            free += tot[1][w];
+            come += tot[2][w];
+        }
+        if (is_free) dst[fr] = p;
+        if (comes) src[cr] = p;
+    }
+    if (tid == 0) a.count[row] = come;
+    __syncthreads();
+    for (int i = tid; i < come; i += 1024) {
+        const int d = dst[i], s = src[i];
+        mass_out[d] = mass[s];
+        pos_out[d] = pos[s];
+    }
+}
+
+// Pass 2, grid (blocks of moves, rows): the movers' keys and values, 16
+// lanes a row. Sources are at or above keep and destinations below it, so
+// no order is needed.
+__global__ __launch_bounds__(256) void k_kv_evict_move(EvictArgs a, int dim) {
+    const int row = blockIdx.y;
+    const int h = row % a.kv_heads, b = row / a.kv_heads % a.slots,
+              layer = row / a.kv_heads / a.slots;
+    const int count = a.count[row];
+    if (blockIdx.x == 0 && h == 0 && layer == 0 && threadIdx.x == 0)
+        a.lens_out[b] = count < 0 ? a.lens[b] : a.keep;
+    const int32_t* table = a.kv.table + (int64_t)b * a.kv.table_stride;
+    const int l16 = threadIdx.x & 15;
+    auto where = [&](int p) -> uint16_t* {
+        const int32_t pg = kv_page_of(table, p / a.kv.page, a.kv.max_pages,
+                                      a.kv.pages);
+        if (pg < 0) return nullptr;
+        return a.kv.pool + layer * a.layer_stride
+            + (int64_t)pg * a.kv.page_stride
+            + (int64_t)h * 2 * a.kv.page * dim
+            + (int64_t)(p % a.kv.page) * dim;
+    };
+    const int64_t to_v = (int64_t)a.kv.page * dim;
+    for (int i = blockIdx.x * 16 + (threadIdx.x >> 4); i < count;
+         i += gridDim.x * 16) {
+        const uint16_t* s = where(a.src[(int64_t)row * a.most + i]);
+        uint16_t* d = where(a.dst[(int64_t)row * a.most + i]);
+        if (!s || !d || l16 * 8 >= dim) continue;
+        const u32x4 k = *reinterpret_cast<const u32x4*>(s + l16 * 8);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(s + to_v + l16 * 8);
+        *reinterpret_cast<u32x4*>(d + l16 * 8) = k;
+        *reinterpret_cast<u32x4*>(d + to_v + l16 * 8) = v;
+    }
+}
+
+size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+
+#define KV_DIM(D_, ...)                                                       \
+    do {                                                                      \
+        if ((D_) == 128) { constexpr int D = 128; __VA_ARGS__; }              \
+        else if ((D_) == 96) { constexpr int D = 96; __VA_ARGS__; }           \
+        else { constexpr int D = 64; __VA_ARGS__; }                           \
+    } while (0)
+
+// q's type over the pool's: the pool's own, or float32 over bfloat16
+#define KV_TYPES(Q_, C_, ...)                                                 \
+    do {                                                                      \
+        if ((C_) == KVT::F16) {                                               \
+            if ((Q_) != KVT::F16) bad_types();                                \
+            typedef F16 C; constexpr int NQ = 1, NP = 2; (void)NP;            \
+            __VA_ARGS__;                                                      \
+        } else if ((Q_) == KVT::BF16) {                                       \
+            typedef Bf16 C; constexpr int NQ = 1, NP = 2; (void)NP;           \
+            __VA_ARGS__;                                                      \
+        } else {                                                              \
+            if ((Q_) != KVT::F32) bad_types();                                \
+            typedef Bf16 C; constexpr int NQ = 3, NP = 3; (void)NP;           \
+            __VA_ARGS__;                                                      \
+        }                                                                     \
+    } while (0)
+
+[[noreturn]] void bad_types() {
+    throw std::runtime_error(
+        "queries must have the pool's type, or float32 over bfloat16");
+}
+
+}  // namespace
+
+void launch_kv_append(const KvPages& kv, const KvHeads& k, const KvHeads& v,
+                      const KvHeads& q, const KvHeads& q_out, int q_heads,
+                      KVT type, int rows, const int32_t* starts,
+                      const int32_t* lens, const int32_t* next_pos,
+                      const float* inv_freq, const KvRows& mass,
+                      const KvRows& pos, int reach, hipStream_t stream) {
+    check_pages(kv, 0, reach);
+    if (rows <= 0) return;
+    if (!starts && rows != kv.slots)
+        throw std::runtime_error("append: one row for each sequence");
+    AppendArgs a{pages_of(kv), k, v, q, q_out, mass, pos, starts, lens,
+                 next_pos, inv_freq, q.data ? q_heads : 0, kv.kv_heads,
+                 kv.slots, reach};
+    // few rows: a row's heads over several workgroups
+    const int items = (a.q_heads + 2 * kv.kv_heads) * (kv.dim / 8);
+    const dim3 grid(rows, rows < 256 ? (items + 255) / 256 : 1);
+    #define APPEND(T, C)                                                      \
+        KV_DIM(kv.dim, hipLaunchKernelGGL((k_kv_append<T, C, D>), grid,       \
+                                          dim3(256), 0, stream, a))
+    if (kv.type == KVT::F16) {
+        if (type != KVT::F16) bad_types();
+        APPEND(KVT::F16, KVT::F16);
+    } else if (type == KVT::BF16) {
+        APPEND(KVT::BF16, KVT::BF16);
+    } else {
+        if (type != KVT::F32) bad_types();
+        APPEND(KVT::F32, KVT::BF16);
+    }
+    #undef APPEND
+    check_launch();
+}
+
+namespace {
+int64_t attend_wgs(const KvPages& kv, int reach) {
+    const int64_t rows = (int64_t)kv.slots * kv.kv_heads;
+    return std::min(ATTEND_WGS + rows,
+                    rows * std::max(1, (reach + UNIT - 1) / UNIT));
+}
+int64_t scores_ld(int reach) { return (int64_t)(reach + 31) / 32 * 32; }
+}  // namespace
+
+size_t kv_attend_workspace(const KvPages& kv, int q_heads, int reach,
+                           bool mass) {
+    check_pages(kv, q_heads, reach);
+    const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
+    return aligned(wgs * G * kv.dim * 4) + aligned(wgs * G * 2 * 4)
+        + (mass ? aligned((size_t)kv.slots * q_heads * scores_ld(reach) * 4)
+                : 0);
+}
+
+void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
+                      int q_heads, KVT type, const int32_t* lens, int add,
+                      const KvRows& mass, int reach, float scale, void* ws,
+                      hipStream_t stream) {
+    check_pages(kv, q_heads, reach);
+    const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
+    char* w = reinterpret_cast<char*>(ws);
+    AttendArgs a{pages_of(kv), q, out, mass, lens, add, q_heads, kv.kv_heads,
+                 kv.slots, reach, ATTEND_WGS, scale * LOG2E, nullptr,
+                 scores_ld(reach), nullptr, nullptr};
+    a.part_o = reinterpret_cast<float*>(w);
+    w += aligned(wgs * G * kv.dim * 4);
+    a.part_ml = reinterpret_cast<float*>(w);
+    w += aligned(wgs * G * 2 * 4);
+    a.scores = reinterpret_cast<float*>(w);
+    const dim3 grid((uint32_t)wgs), block(256);
+    #define ATTEND(M)                                                         \
+        KV_TYPES(type, kv.type, KV_DIM(kv.dim, {                              \
+            hipLaunchKernelGGL((k_kv_attend<C, NQ, NP, D, M>), grid, block,   \
+                               0, stream, a);                                 \
+            hipLaunchKernelGGL((k_kv_join<C, (NQ > 1), D, M>), grid, block,   \
+                               0, stream, a);                                 \
+        }))
+    if (mass.data) ATTEND(true); else ATTEND(false);
+    #undef ATTEND
+    check_launch();
+}
+
+size_t kv_observe_workspace(const KvPages& kv, int q_heads, int rows,
+                            int reach) {
+    check_pages(kv, q_heads, reach);
+    return aligned((size_t)q_heads * std::max(rows, 1) * 4);
+}
+
+void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
+                       KVT type, int rows, const int32_t* starts,
+                       const int32_t* lens, const KvRows& mass, int reach,
+                       float scale, void* ws, hipStream_t stream) {
+    check_pages(kv, q_heads, reach);
+    if (rows <= 0 || reach == 0) return;
+    if ((int64_t)rows * (q_heads / kv.kv_heads) >= (1ll << 30))
+        throw std::runtime_error("observe: too many rows");
+    const int G = q_heads / kv.kv_heads;
+    ObserveArgs a{pages_of(kv), q, mass, starts, lens, q_heads, kv.kv_heads,
+                  kv.slots, rows, reach, scale * LOG2E,
+                  reinterpret_cast<float*>(ws)};
+    KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
+        constexpr int RW = NQ > 1 ? 2 : 4, PW = 4;
+        const int64_t per = 16 * RW * WAVES;
+        hipLaunchKernelGGL((k_kv_observe_sums<C, NQ, D, RW>),
+                           dim3((uint32_t)(((int64_t)rows * G + per - 1) / per
+                                           + kv.slots), kv.kv_heads),
+                           dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D, PW>),
+                           dim3((reach + 16 * PW * WAVES - 1)
+                                / (16 * PW * WAVES), kv.kv_heads, kv.slots),
+                           dim3(256), 0, stream, a);
+    }));
+    check_launch();
+}
+
+size_t kv_evict_workspace(const KvPages& kv, int layers, int keep, int reach) {
+    check_pages(kv, 0, reach);
+    const size_t rows = (size_t)layers * kv.slots * kv.kv_heads;
+    const size_t most = std::max(0, std::min(keep, reach - keep));
+    return aligned(rows * 4) + 2 * aligned(rows * most * 4 + 4);
+}
+
+void launch_kv_evict(const KvPages& kv, int layers, int64_t layer_stride,
+                     const int32_t* lens, int32_t* lens_out,
+                     const int32_t* next_pos, const KvLayers& mass,
+                     const KvLayers& pos, const KvLayers& mass_out,
+                     const KvLayers& pos_out, int keep, int recent, int limit,
+                     int reach, void* ws, hipStream_t stream) {
+    check_pages(kv, 0, reach);
+    const int64_t rows = (int64_t)layers * kv.slots * kv.kv_heads;
+    if (layers < 1 || rows > 65535)
+        throw std::runtime_error("evict: 1 to 65535 rows (layers x sequences "
+                                 "x kv heads)");
+    if (keep < 1 || recent < 0 || limit < keep)
+        throw std::runtime_error("evict: keep >= 1, recent >= 0 and "
+                                 "limit >= keep");
+    const int most = std::max(0, std::min(keep, reach - keep));
+    char* w = reinterpret_cast<char*>(ws);
+    EvictArgs a{pages_of(kv), layer_stride, mass, pos, mass_out, pos_out,
+                lens, next_pos, lens_out, layers, kv.slots, kv.kv_heads, keep,
+                recent, limit, reach, most, nullptr, nullptr, nullptr};
+    a.count = reinterpret_cast<int32_t*>(w);
+    w += aligned(rows * 4);
+    a.dst = reinterpret_cast<int32_t*>(w);
+    w += aligned((size_t)rows * most * 4 + 4);
+    a.src = reinterpret_cast<int32_t*>(w);
+    hipLaunchKernelGGL(k_kv_evict_select, dim3((uint32_t)rows), dim3(1024), 0,
+                       stream, a);
+    hipLaunchKernelGGL(k_kv_evict_move,
+                       dim3(std::max(1, (most + 63) / 64), (uint32_t)rows),
+                       dim3(256), 0, stream, a, kv.dim);
+    check_launch();
+}
+
+}  // namespace cla

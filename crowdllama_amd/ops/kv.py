@@ -1,0 +1,403 @@
+"""The paged KV cache's operators on torch tensors.
+
+    append    rotary positions, new keys and values into the pages
+    attend    one new token's attention over the cache
+    observe   the attention weight that a prompt's rows gave to the places
+    evict     keep the places that matter once a sequence is too long
+
+A layer's pool is `[pages, kv_heads, 2, page, head_dim]` (keys, then values;
+bfloat16 or float16), all but the first dimension contiguous, so that one pool
+of all layers, `[pages, layers, kv_heads, 2, page, head_dim]`, serves as
+`pool[:, layer]`. Place p of sequence b is row `p % page` of page
+`table[b, p // page]`; `lens[b]` of its places are in use. `mass` (float32) and
+`pos` (int32) are `[slots, kv_heads, places]`: the attention weight that each
+place has received, summed over tokens and query heads, and the position of
+the token in it. A place is not a position: after `evict`, a sequence's tokens
+keep their positions (keys are stored rotated) and take other places, which
+differ from head to head.
+
+    q = kv.append(k, v, pool[:, l], table, lens, next_pos, q=q,
+                  inv_freq=inv_freq, mass=mass[l], pos=pos[l])
+    out = kv.attend(q, pool[:, l], table, lens + 1, mass=mass[l])
+    ...
+    kv.evict(pool, table, lens, next_pos, mass, pos, keep=2048, recent=512)
+
+`table`, `lens`, `next_pos` and `starts` are int32 on the device and are read
+there: no call waits for the device, and all may be captured into a graph
+(which then goes by the values at replay). Lengths are cut to what the table
+and the mass reach; page numbers outside the pool are not followed: such places
+have no weight, and nothing is stored there. Work goes to the current stream
+of the tensors' device. None of the operators has a gradient.
+"""
+
+from __future__ import annotations
+
+import torch
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_NONE = (0, 0, 0)
+_core = None
+
+
+def _get(dev):
+    """The native module, in a process with one HIP runtime."""
+    global _core
+    if dev.type != "cuda":
+        _fail(f"pool must be on a GPU, not on {dev}")
+    if _core is None:
+        from . import get_core
+        core = get_core()
+        # torch brings its own HIP runtime, which the extension takes too if
+        # it is there first; streams and memory of one are nothing to another
+        with open("/proc/self/maps") as f:
+            found = {line.split(None, 5)[5].strip() for line in f
+                     if "libamdhip64" in line}
+        if len(found) > 1:
+            raise RuntimeError(
+                "two HIP runtimes are loaded (%s): import torch before the "
+                "first use of crowdllama_amd's native module"
+                % ", ".join(sorted(found)))
+        _core = core
+    return _core
+
+
+def _fail(what: str):
+    raise ValueError("kv: " + what)
+
+
+def _on(t, name: str, dtype, dims: int, device):
+    if not isinstance(t, torch.Tensor):
+        _fail(f"{name} must be a tensor, not {type(t).__name__}")
+    if t.dtype is not dtype:
+        _fail(f"{name} must be {dtype}, not {t.dtype}")
+    if t.dim() != dims:
+        _fail(f"{name} must have {dims} dimensions, not {t.dim()}")
+    if t.device != device:
+        _fail(f"{name} is on {t.device}, the pool on {device}")
+
+
+def _dense(t, name: str, n: int):
+    """The last n dimensions are contiguous."""
+    want = 1
+    shape, stride = t.shape, t.stride()
+    for i in range(1, n + 1):
+        if shape[-i] > 1 and stride[-i] != want:
+            _fail(f"{name}'s last {n} dimensions must be contiguous")
+        want *= shape[-i]
+    return want
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail("no operator of the cache has a gradient")
+
+
+def _pages(pool, table, layers: bool):
+    if not isinstance(pool, torch.Tensor):
+        _fail(f"pool must be a tensor, not {type(pool).__name__}")
+    if pool.dtype not in (torch.bfloat16, torch.float16):
+        _fail(f"pool must be bfloat16 or float16, not {pool.dtype}")
+    dims = 6 if layers else 5
+    if pool.dim() != dims or pool.shape[-3] != 2:
+        _fail("pool must be [pages, %skv_heads, 2, page, head_dim]"
+              % ("layers, " if layers else ""))
+    dev = pool.device
+    size = _dense(pool, "pool", 4)
+    shape, stride = pool.shape, pool.stride()
+    p, heads, page, dim = shape[0], shape[-4], shape[-2], shape[-1]
+    steps = ((stride[0], p),) + (((stride[1], shape[1]),) if layers else ())
+    for step, n in steps:
+        if n > 1 and (step < size or step % 8):
+            _fail("pool's pages must be multiples of 16 bytes apart and must "
+                  "not overlap")
+    if layers and p > 1 and shape[1] > 1 and not (
+            stride[0] >= stride[1] * shape[1]
+            or stride[1] >= stride[0] * p):
+        _fail("pool's layers and pages must not overlap")
+    if pool.numel() == 0 or pool.data_ptr() % 16:
+        _fail("pool must not be empty and must be 16-byte aligned")
+    _on(table, "table", torch.int32, 2, dev)
+    _dense(table, "table", 1)
+    slots, reach = table.shape[0], table.shape[1] * page
+    if not slots or not reach:
+        _fail("table must not be empty")
+    return dev, reach, (
+        pool.data_ptr(), stride[0], p, table.data_ptr(), table.stride(0),
+        table.shape[1], page, slots, heads, dim, _TYPES[pool.dtype],
+        dev.index)
+
+
+def _vector(t, name: str, n: int, dev):
+    _on(t, name, torch.int32, 1, dev)
+    if t.shape[0] != n:
+        _fail(f"{name} must have {n} values, not {t.shape[0]}")
+    _dense(t, name, 1)
+    return t.data_ptr()
+
+
+def _heads(t, name: str, rows, heads, dim: int, dtype, dev):
+    _on(t, name, dtype, 3, dev)
+    shape = t.shape
+    if ((rows is not None and shape[0] != rows)
+            or (heads is not None and shape[1] != heads) or shape[2] != dim):
+        _fail(f"{name} must be [{'rows' if rows is None else rows}, "
+              f"{'heads' if heads is None else heads}, {dim}], not "
+              f"{list(shape)}")
+    _dense(t, name, 1)
+    s0, s1, _ = t.stride()
+    unit = 4 if dtype is torch.float32 else 8
+    if t.data_ptr() % 16 or (shape[0] > 1 and s0 % unit) or (
+            shape[1] > 1 and s1 % unit):
+        _fail(f"{name}'s rows must be 16-byte aligned")
+    return t.data_ptr(), s0, s1
+
+
+def _apart(t, name: str):
+    """A tensor that is written must have a place of its own for each value:
+    sorted by stride, each dimension steps over the ones below it."""
+    if t.is_contiguous():
+        return
+    span = 1
+    for step, n in sorted((s, n) for n, s in zip(t.shape, t.stride())
+                          if n > 1):
+        if step < span:
+            _fail(f"{name} is written and must not overlap itself")
+        span = step * n
+
+
+def _meet(a, b) -> bool:
+    """Whether the memory from a's first to its last value meets b's."""
+    ends = [(t.data_ptr(), t.data_ptr() + t.element_size() * (
+        1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+        for t in (a, b)]
+    return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
+
+
+def _same(a, b) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
+    _on(t, name, dtype, len(lead) + 1, dev)
+    if tuple(t.shape[:-1]) != lead:
+        _fail(f"{name} must be {list(lead)} x places, not {list(t.shape)}")
+    if not 0 < t.shape[-1] <= reach:
+        _fail(f"{name} must have 1 to {reach} places (what the table "
+              f"reaches), not {t.shape[-1]}")
+    _dense(t, name, 1)
+    _apart(t, name)
+    return (t.data_ptr(), *t.stride()[:-1])
+
+
+def _queries(q, dtype_of_pool):
+    if not isinstance(q, torch.Tensor):
+        _fail(f"q must be a tensor, not {type(q).__name__}")
+    if q.dtype is not dtype_of_pool and not (
+            q.dtype is torch.float32 and dtype_of_pool is torch.bfloat16):
+        _fail(f"{q.dtype} does not go with a pool of {dtype_of_pool}: it "
+              "must be the pool's type, or float32 over bfloat16")
+
+
+def _group(heads: int, kv_heads: int):
+    if heads % kv_heads or not 1 <= heads // kv_heads <= 16:
+        _fail(f"{heads} query heads over {kv_heads} kv heads: 1 to 16 query "
+              "heads must share each kv head")
+
+
+def _workspace(n: int, dev):
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
+
+
+def _stream(dev) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
+           starts=None, mass=None, pos=None, q_out=None):
+    """Store new tokens' keys and values behind each sequence's last place.
+
+    k, v: `[rows, kv_heads, head_dim]`, of the pool's type or float32 over a
+    bfloat16 pool (rounded once, when stored). Rows `starts[b]` to
+    `starts[b + 1]` are sequence b's next tokens, in order; without `starts`
+    row b is sequence b's. Token i of sequence b goes to place `lens[b] + i`,
+    and is at position `next_pos[b] + i`.
+
+    inv_freq: float32 `[head_dim / 2]`, the radians per position of each
+    adjacent pair; without it nothing is rotated. q `[rows, heads, head_dim]`
+    is rotated as k is, and returned (in `q_out`, which may be q itself).
+    mass, pos: the new places' mass becomes 0 and their pos the position.
+
+    `lens` and `next_pos` are only read (all layers share them). Rows past the
+    last place that a sequence has are not stored; rows past `starts[-1]`
+    belong to no sequence: their queries are returned as they are.
+    """
+    dev, reach, kv = _pages(pool, table, False)
+    slots, heads, dim = kv[7], kv[8], kv[9]
+    _queries(k, pool.dtype)
+    _no_grad(k, v, q)
+    rows = k.shape[0] if k.dim() else 0
+    kh = _heads(k, "k", None, heads, dim, k.dtype, dev)
+    vh = _heads(v, "v", rows, heads, dim, k.dtype, dev)
+    qh = qo = _NONE
+    q_heads = 0
+    if q is not None:
+        qh = _heads(q, "q", rows, None, dim, k.dtype, dev)
+        q_heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((rows, q_heads, dim), dtype=q.dtype,
+                                device=dev)
+        qo = _heads(q_out, "q_out", rows, q_heads, dim, k.dtype, dev)
+        _apart(q_out, "q_out")
+    elif q_out is not None:
+        _fail("q_out without q")
+    if starts is None and rows != slots:
+        _fail(f"without starts there must be one row for each of {slots} "
+              f"sequences, not {rows}")
+    st = 0 if starts is None else _vector(starts, "starts", slots + 1, dev)
+    fr = 0
+    if inv_freq is not None:
+        _on(inv_freq, "inv_freq", torch.float32, 1, dev)
+        _dense(inv_freq, "inv_freq", 1)
+        if inv_freq.shape[0] != dim // 2:
+            _fail(f"inv_freq must have {dim // 2} values")
+        fr = inv_freq.data_ptr()
+    ms = ps = _NONE
+    if mass is not None:
+        ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
+        reach = mass.shape[-1]
+    if pos is not None:
+        ps = _places(pos, "pos", torch.int32, (slots, heads), reach, dev)
+        reach = min(reach, pos.shape[-1])
+    le = _vector(lens, "lens", slots, dev)
+    np = _vector(next_pos, "next_pos", slots, dev)
+    _get(dev).kv_append(kv, kh, vh, qh, qo, q_heads, _TYPES[k.dtype], rows,
+                        st, le, np, fr, ms, ps, reach, _stream(dev))
+    return q_out
+
+
+def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
+    """Attention of one new token of each sequence over its first `lens[b]`
+    places: `[slots, heads, head_dim]`, of q's type.
+
+    q: `[slots, heads, head_dim]`, of the pool's type or float32 over a
+    bfloat16 pool; query heads g * i ... g * i + g - 1 share kv head i.
+    mass: each place's weight is added, summed over the query heads that share
+    the kv head. scale: of the scores, head_dim ** -0.5 by default. A sequence
+    without places gives zeros.
+    """
+    dev, reach, kv = _pages(pool, table, False)
+    slots, heads, dim = kv[7], kv[8], kv[9]
+    _queries(q, pool.dtype)
+    _no_grad(q)
+    qh = _heads(q, "q", slots, None, dim, q.dtype, dev)
+    q_heads = q.shape[1]
+    _group(q_heads, heads)
+    ms = _NONE
+    if mass is not None:
+        ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
+        reach = mass.shape[-1]
+    if out is None:
+        out = torch.empty((slots, q_heads, dim), dtype=q.dtype, device=dev)
+    oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
+    _apart(out, "out")
+    le = _vector(lens, "lens", slots, dev)
+    core = _get(dev)
+    ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
+                                             mass is not None), dev)
+    core.kv_attend(kv, qh, oh, q_heads, _TYPES[q.dtype], le, ms, reach,
+                   dim ** -0.5 if scale is None else float(scale),
+                   ws.data_ptr(), _stream(dev))
+    return out
+
+
+def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
+    """Add to `mass` the attention weights of each sequence's last tokens.
+
+    q: `[rows, heads, head_dim]`, rotated; rows `starts[b]` to `starts[b + 1]`
+    are the queries of sequence b's last tokens (without `starts`, row b is
+    that of sequence b's last), whose keys are in the cache: `lens[b]` counts
+    them. Each sees the places up to its own. What `attend` adds for one token,
+    this adds for a prompt, without making its outputs. Returns mass.
+    """
+    dev, reach, kv = _pages(pool, table, False)
+    slots, heads, dim = kv[7], kv[8], kv[9]
+    _queries(q, pool.dtype)
+    _no_grad(q)
+    qh = _heads(q, "q", None, None, dim, q.dtype, dev)
+    rows, q_heads = q.shape[0], q.shape[1]
+    _group(q_heads, heads)
+    ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
+    reach = mass.shape[-1]
+    if starts is None:
+        if rows != slots:
+            _fail(f"without starts there must be one row for each of {slots} "
+                  f"sequences, not {rows}")
+        starts = torch.arange(slots + 1, dtype=torch.int32, device=dev)
+    st = _vector(starts, "starts", slots + 1, dev)
+    le = _vector(lens, "lens", slots, dev)
+    core = _get(dev)
+    ws = _workspace(core.kv_observe_workspace(kv, q_heads, rows, reach), dev)
+    core.kv_observe(kv, qh, q_heads, _TYPES[q.dtype], rows, st, le,
+                    ms, reach,
+                    dim ** -0.5 if scale is None else float(scale),
+                    ws.data_ptr(), _stream(dev))
+    return mass
+
+
+def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
+          limit=None, out=None):
+    """Keep `keep` places of each sequence with more than `limit` of them
+    (default: `keep`), for each layer and kv head its own; returns
+    `(mass, pos, lens)`.
+
+    pool: `[pages, layers, kv_heads, 2, page, head_dim]`; mass, pos:
+    `[layers, slots, kv_heads, places]`. Places with a pos of at least
+    `next_pos[b] - recent` stay before all others, the others by mass; among
+    equals the lower place stays. Survivors below place `keep` stay where they
+    are; the free places there take the others, both in order. What lies at
+    and above `keep` afterwards is left as it was.
+
+    Keys and values move within the pool. mass, pos and lens are changed in
+    place, or, with `out=(mass, pos, lens)`, written there whole while these
+    stay as they were.
+    """
+    dev, reach, kv = _pages(pool, table, True)
+    slots, heads, layers = kv[7], kv[8], pool.shape[1]
+    keep, recent = int(keep), int(recent)
+    limit = keep if limit is None else int(limit)
+    if keep < 1 or recent < 0 or limit < keep:
+        _fail(f"keep {keep}, recent {recent}, limit {limit}: keep must be at "
+              "least 1, recent not negative and limit not below keep")
+    if max(keep, recent, limit) >= 1 << 31:
+        _fail("keep, recent and limit must be below 2^31")
+    lead = (layers, slots, heads)
+    ms = _places(mass, "mass", torch.float32, lead, reach, dev)
+    ps = _places(pos, "pos", torch.int32, lead, reach, dev)
+    reach = mass.shape[-1]
+    if pos.shape[-1] != reach:
+        _fail("mass and pos must have equally many places")
+    if layers * slots * heads > 65535:
+        _fail("layers x sequences x kv heads must be at most 65535")
+    le = _vector(lens, "lens", slots, dev)
+    np = _vector(next_pos, "next_pos", slots, dev)
+    if out is None:
+        out = (mass, pos, lens)
+    mass_out, pos_out, lens_out = out
+    mo = _places(mass_out, "out's mass", torch.float32, lead, reach, dev)
+    po = _places(pos_out, "out's pos", torch.int32, lead, reach, dev)
+    lo = _vector(lens_out, "out's lens", slots, dev)
+    if mass_out.shape[-1] != reach or pos_out.shape[-1] != reach:
+        _fail("out's mass and pos must have as many places as mass")
+    for new in (mass_out, pos_out, lens_out):
+        for old, same in ((mass, mass_out), (pos, pos_out), (lens, lens_out),
+                          (next_pos, None)):
+            if _meet(new, old) and not (new is same and _same(new, old)):
+                _fail("each of out must be the tensor that it replaces, or "
+                      "apart from all of them")
+    core = _get(dev)
+    ws = _workspace(core.kv_evict_workspace(kv, layers, keep, reach), dev)
+    core.kv_evict(kv, layers, pool.stride(1), le, lo, np,
+                  ms, ps, mo, po, keep, recent, limit, reach, ws.data_ptr(), _stream(dev))
+    return mass_out, pos_out, lens_out

@@ -1,0 +1,199 @@
+"""What the paged cache's operators refuse, and what they decide from values
+on the device, on the CPU."""
+import math
+
+import pytest
+import torch
+
+from crowdllama_amd.ops import get_core, kv
+
+
+def pool(pages=8, heads=2, page=16, dim=64, dtype=torch.bfloat16, layers=None):
+    lead = (pages,) if layers is None else (pages, layers)
+    return torch.zeros(*lead, heads, 2, page, dim, dtype=dtype)
+
+
+def ints(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def attend_args(**kw):
+    a = dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16), pool=pool(),
+             table=torch.zeros(2, 4, dtype=torch.int32), lens=ints(1, 2))
+    a.update(kw)
+    return a
+
+
+def refused(call, args, match):
+    with pytest.raises(ValueError, match=match):
+        call(**args)
+
+
+def test_all_is_checked_before_the_device():
+    refused(kv.attend, attend_args(), "must be on a GPU")
+    refused(kv.attend, attend_args(mass=torch.zeros(2, 2, 64)),
+            "must be on a GPU")
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(q=torch.zeros(2, 4, 64, dtype=torch.float16)), "does not go with"),
+    (dict(q=torch.zeros(2, 4, 64), pool=pool(dtype=torch.float16)),
+     "does not go with"),
+    (dict(pool=pool(dtype=torch.float32)), "bfloat16 or float16"),
+    (dict(q=torch.zeros(2, 3, 64, dtype=torch.bfloat16)), "kv heads"),
+    (dict(q=torch.zeros(2, 34, 64, dtype=torch.bfloat16)), "kv heads"),
+    (dict(q=torch.zeros(2, 0, 64, dtype=torch.bfloat16)), "kv heads"),
+    (dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16)), "q must be"),
+    (dict(q=torch.zeros(2, 4, 96, dtype=torch.bfloat16)), "q must be"),
+    (dict(q=torch.zeros(2, 4, 128, dtype=torch.bfloat16)[..., ::2]),
+     "contiguous"),
+    (dict(q=torch.zeros(2, 4, 68, dtype=torch.bfloat16)[..., 4:]),
+     "16-byte aligned"),
+    (dict(lens=ints(1)), "lens must have 2"),
+    (dict(lens=torch.tensor([1, 2])), "lens must be torch.int32"),
+    (dict(lens=[1, 2]), "lens must be a tensor"),
+    (dict(table=torch.zeros(2, 4)), "table must be torch.int32"),
+    (dict(table=torch.zeros(2, 8, dtype=torch.int32)[:, ::2]), "contiguous"),
+    (dict(table=torch.zeros(2, 0, dtype=torch.int32)), "empty"),
+    (dict(pool=torch.zeros(8, 2, 64, 64, dtype=torch.bfloat16)),
+     "pool must be"),
+    (dict(pool=pool().transpose(2, 3)), "pool must be"),
+    (dict(pool=pool(pages=1).expand(8, -1, -1, -1, -1)), "overlap"),
+    (dict(pool=pool()[..., :32]), "contiguous"),
+    (dict(mass=torch.zeros(2, 2, 65)), "1 to 64 places"),
+    (dict(mass=torch.zeros(2, 4, 64)), "mass must be"),
+    (dict(mass=torch.zeros(2, 2, 64, dtype=torch.float64)), "mass must be"),
+    (dict(mass=torch.zeros(2, 1, 64).expand(2, 2, 64)), "overlap"),
+    (dict(out=torch.zeros(2, 4, 64)), "out must be torch.bfloat16"),
+    (dict(out=torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(2, 4, 64)),
+     "overlap"),
+    (dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16, requires_grad=True)),
+     "gradient"),
+    (dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="meta")),
+     "q is on meta"),
+])
+def test_attend_refuses(kw, match):
+    refused(kv.attend, attend_args(**kw), match)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(), "must be on a GPU"),
+    (dict(v=torch.zeros(3, 2, 64, dtype=torch.bfloat16)), "v must be"),
+    (dict(k=torch.zeros(2, 3, 64, dtype=torch.bfloat16)), "k must be"),
+    (dict(q=torch.zeros(2, 4, 64)), "q must be torch.bfloat16"),
+    (dict(q_out=torch.zeros(2, 4, 64, dtype=torch.bfloat16)), "without q"),
+    (dict(inv_freq=torch.zeros(64)), "32 values"),
+    (dict(inv_freq=torch.zeros(32).double()), "inv_freq must be"),
+    (dict(starts=ints(0, 1)), "starts must have 3"),
+    (dict(k=torch.zeros(3, 2, 64, dtype=torch.bfloat16),
+          v=torch.zeros(3, 2, 64, dtype=torch.bfloat16)), "without starts"),
+    (dict(pos=torch.zeros(2, 2, 64)), "pos must be torch.int32"),
+    (dict(next_pos=ints(1)), "next_pos must have 2"),
+])
+def test_append_refuses(kw, match):
+    a = dict(k=torch.zeros(2, 2, 64, dtype=torch.bfloat16),
+             v=torch.zeros(2, 2, 64, dtype=torch.bfloat16), pool=pool(),
+             table=torch.zeros(2, 4, dtype=torch.int32), lens=ints(0, 0),
+             next_pos=ints(0, 0))
+    a.update(kw)
+    refused(kv.append, a, match)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(), "must be on a GPU"),
+    (dict(mass=None), "mass must be a tensor"),
+    (dict(starts=None), "without starts"),
+    (dict(starts=ints(0, 1, 2, 3)), "starts must have 3"),
+    (dict(q=torch.zeros(5, 64, dtype=torch.bfloat16)), "3 dimensions"),
+])
+def test_observe_refuses(kw, match):
+    a = dict(q=torch.zeros(5, 4, 64, dtype=torch.bfloat16), pool=pool(),
+             table=torch.zeros(2, 4, dtype=torch.int32), lens=ints(3, 2),
+             mass=torch.zeros(2, 2, 64), starts=ints(0, 3, 5))
+    a.update(kw)
+    refused(kv.observe, a, match)
+
+
+def evict_args(**kw):
+    a = dict(pool=pool(layers=3), table=torch.zeros(2, 4, dtype=torch.int32),
+             lens=ints(3, 2), next_pos=ints(3, 2),
+             mass=torch.zeros(3, 2, 2, 64),
+             pos=torch.zeros(3, 2, 2, 64, dtype=torch.int32), keep=5)
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(), "must be on a GPU"),
+    (dict(keep=0), "keep must be"),
+    (dict(recent=-1), "keep must be"),
+    (dict(limit=4), "keep must be"),
+    (dict(limit=1 << 31), "below 2"),
+    (dict(pool=pool()), "pool must be"),
+    (dict(pos=torch.zeros(3, 2, 2, 63, dtype=torch.int32)), "equally many"),
+    (dict(mass=torch.zeros(2, 2, 2, 64)), "mass must be"),
+    (dict(pool=pool(layers=1).expand(8, 3, -1, -1, -1, -1)), "overlap"),
+    (dict(out=(torch.zeros(3, 2, 2, 60),
+               torch.zeros(3, 2, 2, 64, dtype=torch.int32), ints(0, 0))),
+     "as many places"),
+    (dict(table=torch.zeros(22000, 1, dtype=torch.int32),
+          mass=torch.zeros(1).expand(3, 22000, 2, 1)), "overlap"),
+])
+def test_evict_refuses(kw, match):
+    refused(kv.evict, evict_args(**kw), match)
+
+
+def test_evict_refuses_a_mixed_out():
+    a = evict_args()
+    b = torch.zeros(3, 2, 2, 65)
+    a["mass"] = b[..., :64]
+    refused(kv.evict, {**a, "out": (b[..., 1:], a["pos"], a["lens"])}, "apart")
+    refused(kv.evict, {**a, "out": (a["mass"], a["pos"], a["next_pos"])},
+            "apart")
+    refused(kv.evict, {**a, "out": (a["mass"], a["pos"], a["lens"])},
+            "must be on a GPU")
+    refused(kv.evict, {**a, "out": (torch.zeros(3, 2, 2, 64), a["pos"],
+                                    ints(0, 0))}, "must be on a GPU")
+
+
+def pages_arg(page=16, dim=64, slots=1, heads=1, kind=2, max_pages=4):
+    return (0, 0, 1, 0, 0, max_pages, page, slots, heads, dim, kind, 0)
+
+
+@pytest.mark.parametrize("kw,reach,match", [
+    (dict(page=8), 32, "page size"), (dict(page=40), 32, "page size"),
+    (dict(page=2048), 32, "page size"), (dict(dim=80), 32, "head_dim"),
+    (dict(dim=256), 32, "head_dim"), (dict(kind=0), 32, "bfloat16"),
+    (dict(), 65, "2\\^30"), (dict(), -1, "2\\^30"),
+    (dict(max_pages=1 << 27), (1 << 30) + 1, "2\\^30"),
+    (dict(max_pages=1 << 26, slots=4096), 1 << 30, "too many places"),
+])
+def test_sizes_that_the_kernels_do_not_take(kw, reach, match):
+    core = get_core()
+    with pytest.raises(RuntimeError, match=match):
+        core.kv_attend_workspace(pages_arg(**kw), 1, reach, True)
+
+
+def test_pages_outside_the_pool_are_not_followed():
+    find = get_core().test_kv_page_of
+    row = [3, -1, 5, 4, 2 ** 31 - 1, -2 ** 31]
+    assert [find(row, i, 5) for i in range(-1, 8)] == [
+        -1, 3, -1, -1, 4, -1, -1, -1, -1]
+    assert find(row, 2 ** 40, 5) == -1 and find(row, -2 ** 40, 5) == -1
+
+
+def test_lengths_are_cut():
+    cut = get_core().test_kv_clamp_len
+    assert [cut(x, 64) for x in (-2 ** 31, -1, 0, 1, 64, 65, 2 ** 31 - 1)] \
+        == [0, 0, 0, 1, 64, 64, 64]
+
+
+def test_order_of_eviction():
+    key = get_core().test_kv_rank_key
+    masses = [math.nan, -math.inf, -3e38, -1., -1e-45, 0., 1e-45, 1e-3, 1.,
+              3e38, math.inf]
+    keys = [key(m, False) for m in masses]
+    assert keys == sorted(keys) and len(set(keys)) == len(keys)
+    assert key(-0., False) == key(0., False)
+    assert key(math.copysign(math.nan, -1), False) == keys[0]
+    assert all(key(m, True) == 2 ** 32 - 1 > max(keys) for m in masses)
