@@ -85,11 +85,14 @@ async def _run_start(args) -> None:
                     from .engine.batching import BatchingHipEngine
                     engines[m] = BatchingHipEngine(
                         m, path, device=args.device, batch=args.batch,
-                        max_seq=cfg.max_seq)
+                        max_seq=cfg.max_seq, kv_keep=args.kv_keep,
+                        kv_recent=args.kv_recent)
                 else:
                     from .engine.hip_engine import HipEngine
                     engines[m] = HipEngine(m, path, device=args.device,
-                                           max_seq=cfg.max_seq)
+                                           max_seq=cfg.max_seq,
+                                           kv_keep=args.kv_keep,
+                                           kv_recent=args.kv_recent)
 
     peer = Peer(cfg, worker_mode=args.worker_mode, engines=engines)
     await peer.start()
@@ -203,6 +206,13 @@ def main(argv: list[str] | None = None) -> int:
     st.add_argument("--device", type=int, default=0)
     st.add_argument("--batch", type=int, default=1,
                     help="decode slots for continuous batching (worker mode)")
+    st.add_argument("--kv-keep", type=int, default=0,
+                    help="go on past the context length: whenever a slot's "
+                         "KV cache is full, keep this many places by "
+                         "accumulated attention weight (0: off)")
+    st.add_argument("--kv-recent", type=int, default=0,
+                    help="of the --kv-keep places, how many are reserved "
+                         "for the newest tokens")
 
     dh = sub.add_parser("dht", help="start a bootstrap/rendezvous node")
     _add_common(dh)

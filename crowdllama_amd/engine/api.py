@@ -15,6 +15,22 @@ import time
 from dataclasses import dataclass
 
 
+#: An engine that evicts from its KV cache generates at most this many times
+#: max_seq tokens for one request.
+EVICTING_GEN = 16
+
+
+def token_budget(wanted: int, prompt: int, max_seq: int, gen_cap: int,
+                 kv_keep: int = 0) -> int:
+    """How many of the wanted tokens a request gets; below 1 if its prompt
+    does not fit. With eviction (kv_keep) only the prompt is held to
+    max_seq."""
+    room = max_seq - prompt - 1
+    if kv_keep and room >= 1:
+        room = gen_cap
+    return min(wanted, room, gen_cap)
+
+
 @dataclass
 class GenerateResult:
     text: str

@@ -22,7 +22,8 @@ from dataclasses import dataclass, field
 
 from ..quant.gguf import GGUFReader
 from ..tokenizer import NativeTokenizer, Tokenizer
-from .api import EngineBase, GenerateResult, RollingRate
+from .api import EngineBase, GenerateResult, RollingRate, token_budget
+from .api import EVICTING_GEN
 
 DECODE_STRIDE = 8  # graph replays between slot bookkeeping passes
 
@@ -52,7 +53,8 @@ class _Slot:
 
 class BatchingHipEngine(EngineBase):
     def __init__(self, model_name: str, gguf_path: str, device: int = 0,
-                 batch: int = 8, max_seq: int = 4096, max_new: int = 256):
+                 batch: int = 8, max_seq: int = 4096, max_new: int = 256,
+                 kv_keep: int = 0, kv_recent: int = 0):
         from ..ops import get_core
         core = self._core = get_core()
         if core.device_count() == 0:
@@ -64,7 +66,10 @@ class BatchingHipEngine(EngineBase):
         # size the generated-token ring from max_seq so a request's max_new
         # can never exceed it (a request with
         # max_new > gen_cap saturated the ring and decoded forever)
-        cfg.gen_cap = max_seq
+        cfg.gen_cap = max_seq * EVICTING_GEN if kv_keep else max_seq
+        # past max_seq by eviction, as HipEngine
+        cfg.kv_keep, cfg.kv_recent = kv_keep, kv_recent
+        self.kv_keep = kv_keep
         cfg.device = device
         self.eng = core.Engine(gguf_path, cfg)
         self.gen_cap = cfg.gen_cap
@@ -182,8 +187,9 @@ class BatchingHipEngine(EngineBase):
         # clamp to both the sequence budget and the engine's generated-token
         # ring (gen_cap): tokens past gen_cap are never recorded, so a
         # max_new above it would otherwise decode forever
-        max_new = min(max_new_tokens or self.default_max_new,
-                      self.max_seq - len(ids) - 1, self.gen_cap)
+        max_new = token_budget(max_new_tokens or self.default_max_new,
+                               len(ids), self.max_seq, self.gen_cap,
+                               self.kv_keep)
         if max_new < 1:
             raise ValueError("prompt exceeds max_seq")
         return _Req(ids=ids or [self.tok.bos_id], max_new=max_new,

@@ -10,7 +10,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 from ..quant.gguf import GGUFReader
 from ..tokenizer import NativeTokenizer, Tokenizer
-from .api import EngineBase, GenerateResult, RollingRate
+from .api import EngineBase, GenerateResult, RollingRate, token_budget
+from .api import EVICTING_GEN
 
 
 class HipEngine(EngineBase):
@@ -18,7 +19,11 @@ class HipEngine(EngineBase):
     (matching the reference's per-worker request granularity)."""
 
     def __init__(self, model_name: str, gguf_path: str, device: int = 0,
-                 max_seq: int = 4096, use_graph: bool = True):
+                 max_seq: int = 4096, use_graph: bool = True,
+                 kv_keep: int = 0, kv_recent: int = 0):
+        """kv_keep: generate past max_seq by evicting from the KV cache down
+        to this many places (kv_recent of them the newest tokens') whenever
+        it is full; 0 ends a sequence at max_seq."""
         from ..ops import get_core
         core = self._core = get_core()
         if core.device_count() == 0:
@@ -28,7 +33,9 @@ class HipEngine(EngineBase):
         cfg = core.EngineConfig()
         cfg.batch = 1
         cfg.max_seq = max_seq
-        cfg.gen_cap = max_seq  # ring >= any admissible max_new
+        # ring >= any admissible max_new
+        cfg.gen_cap = max_seq * EVICTING_GEN if kv_keep else max_seq
+        cfg.kv_keep, cfg.kv_recent = kv_keep, kv_recent
         cfg.device = device
         cfg.use_graph = use_graph
         self.eng = core.Engine(gguf_path, cfg)
@@ -49,6 +56,7 @@ class HipEngine(EngineBase):
                                         thread_name_prefix="hipengine")
         self._active = 0
         self.max_seq = max_seq
+        self.kv_keep = kv_keep
 
     # ------------------------------------------------------------ generate
 
@@ -57,8 +65,8 @@ class HipEngine(EngineBase):
         BatchingHipEngine); reject only when the PROMPT itself does not fit
         — never truncate it silently."""
         ids = self.tok.encode(prompt)
-        max_new = min(max_new_tokens, self.max_seq - len(ids) - 1,
-                      self.gen_cap)
+        max_new = token_budget(max_new_tokens, len(ids), self.max_seq,
+                               self.gen_cap, self.kv_keep)
         if max_new < 1:
             raise ValueError(
                 f"prompt ({len(ids)} tokens) exceeds max_seq={self.max_seq}")

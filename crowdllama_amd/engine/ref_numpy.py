@@ -38,8 +38,14 @@ def _act_q8(x: np.ndarray) -> np.ndarray:
 
 class RefLlama:
     def __init__(self, gguf_path: str, kv_bf16: bool = True,
-                 act_q8: bool = False):
+                 act_q8: bool = False, max_seq: int = 0, kv_keep: int = 0,
+                 kv_recent: int = 0):
         self.act_q8 = act_q8
+        # eviction: once max_seq places are in use, each layer and kv head
+        # keeps kv_keep of them (EngineConfig.kv_keep)
+        self.max_seq, self.kv_keep, self.kv_recent = (max_seq, kv_keep,
+                                                      kv_recent)
+        self.n_past = 0
         self.r = GGUFReader(gguf_path)
         md = self.r.metadata
         self.n_layers = md["llama.block_count"]
@@ -56,6 +62,32 @@ class RefLlama:
         self._cache: dict[str, np.ndarray] = {}
         # KV cache: [layer][2][t][kv_heads][head_dim]
         self.kv: list[list[np.ndarray]] = [[] for _ in range(self.n_layers)]
+        # kv_keep: [layer][kv head] -> places [K, V, mass, position]
+        self.places: list[list[list[list]]] = self._no_places()
+
+    def _no_places(self):
+        return [[[] for _ in range(self.kv_heads)]
+                for _ in range(self.n_layers)]
+
+    def _evict(self) -> None:
+        """Recent tokens' places stay, then those with the most mass, the
+        lower place among equals. Free places below kv_keep take the
+        survivors from above it, in order."""
+        late = self.n_past - self.kv_recent
+        for layer in self.places:
+            for h, row in enumerate(layer):
+                if len(row) < self.max_seq:
+                    continue
+                order = sorted(
+                    range(len(row)),
+                    key=lambda p: (row[p][3] < late,
+                                   0.0 if row[p][3] >= late else -row[p][2],
+                                   p))
+                stay = set(order[:self.kv_keep])
+                come = iter([row[p] for p in sorted(stay)
+                             if p >= self.kv_keep])
+                layer[h] = [row[p] if p in stay else next(come)
+                            for p in range(self.kv_keep)]
 
     def w(self, name: str) -> np.ndarray:
         if name not in self._cache:
@@ -74,6 +106,8 @@ class RefLlama:
 
     def reset(self):
         self.kv = [[] for _ in range(self.n_layers)]
+        self.places = self._no_places()
+        self.n_past = 0
 
     def _rms(self, x: np.ndarray, g: np.ndarray) -> np.ndarray:
         inv = 1.0 / np.sqrt(np.mean(x * x) + self.eps)
@@ -97,33 +131,47 @@ class RefLlama:
         h, nh, nkv, hd = self.hidden, self.heads, self.kv_heads, self.head_dim
         G = nh // nkv
         x = self.w("token_embd.weight")[token].astype(np.float32)
+        if self.kv_keep:
+            self._evict()
         for li in range(self.n_layers):
             p = f"blk.{li}."
             xn = self._rms(x, self.w(p + "attn_norm.weight"))
             q = self.mm(p + "attn_q.weight", xn)
             k = self.mm(p + "attn_k.weight", xn)
             v = self.mm(p + "attn_v.weight", xn)
-            pos = len(self.kv[li])
+            pos = self.n_past
             q = self._rope(q.reshape(nh, hd), pos)
             k = self._rope(k.reshape(nkv, hd), pos)
             v = v.reshape(nkv, hd)
             if self.kv_bf16:
                 k, v = _bf16_round(k), _bf16_round(v)
-            self.kv[li].append((k, v))
-            ks = np.stack([e[0] for e in self.kv[li]])  # [t, nkv, hd]
-            vs = np.stack([e[1] for e in self.kv[li]])
             attn = np.zeros((nh, hd), dtype=np.float32)
-            for head in range(nh):
-                kvh = head // G
-                scores = ks[:, kvh] @ q[head] / np.sqrt(hd)
-                w = _softmax(scores)
-                attn[head] = w @ vs[:, kvh]
+            if self.kv_keep:
+                for kvh, row in enumerate(self.places[li]):
+                    row.append([k[kvh], v[kvh], 0.0, pos])
+                    ks = np.stack([e[0] for e in row])
+                    vs = np.stack([e[1] for e in row])
+                    for head in range(kvh * G, (kvh + 1) * G):
+                        w = _softmax(ks @ q[head] / np.sqrt(hd))
+                        attn[head] = w @ vs
+                        for e, mass in zip(row, w):
+                            e[2] += float(mass)
+            else:
+                self.kv[li].append((k, v))
+                ks = np.stack([e[0] for e in self.kv[li]])  # [t, nkv, hd]
+                vs = np.stack([e[1] for e in self.kv[li]])
+                for head in range(nh):
+                    kvh = head // G
+                    scores = ks[:, kvh] @ q[head] / np.sqrt(hd)
+                    w = _softmax(scores)
+                    attn[head] = w @ vs[:, kvh]
             x = x + self.mm(p + "attn_output.weight", attn.reshape(-1))
             xn = self._rms(x, self.w(p + "ffn_norm.weight"))
             g = self.mm(p + "ffn_gate.weight", xn)
             u = self.mm(p + "ffn_up.weight", xn)
             act = (g / (1.0 + np.exp(-g))) * u
             x = x + self.mm(p + "ffn_down.weight", act)
+        self.n_past += 1
         xn = self._rms(x, self.w("output_norm.weight"))
         head_name = ("output.weight" if "output.weight" in self.r.tensors
                      else "token_embd.weight")

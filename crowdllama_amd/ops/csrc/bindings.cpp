@@ -103,6 +103,8 @@ PYBIND11_MODULE(_core, m) {
         .def_readwrite("tp_size", &EngineConfig::tp_size)
         .def_readwrite("act_q8", &EngineConfig::act_q8)
         .def_readwrite("gemv_q8", &EngineConfig::gemv_q8)
+        .def_readwrite("kv_keep", &EngineConfig::kv_keep)
+        .def_readwrite("kv_recent", &EngineConfig::kv_recent)
         .def_property("nccl_id",
             [](EngineConfig& c) { return py::bytes(c.nccl_id); },
             [](EngineConfig& c, py::bytes b) { c.nccl_id = std::string(b); });
@@ -140,6 +142,18 @@ PYBIND11_MODULE(_core, m) {
         .def("set_cur_token", &Engine::set_cur_token)
         .def("cur_token", &Engine::cur_token)
         .def("n_past", &Engine::n_past)
+        .def("kv_lens", &Engine::kv_lens)
+        .def("kv_places",
+             [](Engine& e, int layer, int slot) {
+                 std::vector<int32_t> pos;
+                 std::vector<float> mass;
+                 e.kv_places(layer, slot, pos, mass);
+                 const py::ssize_t h = e.meta().kv_heads_l,
+                                   n = (py::ssize_t)pos.size() / h;
+                 return py::make_tuple(
+                     py::array_t<int32_t>({h, n}, pos.data()),
+                     py::array_t<float>({h, n}, mass.data()));
+             }, py::arg("layer"), py::arg("slot"))
         .def("vram_bytes", &Engine::vram_bytes)
         .def("last_decode_ms", &Engine::last_decode_ms)
         .def_property_readonly("meta", [](Engine& e) {

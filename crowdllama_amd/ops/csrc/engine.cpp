@@ -28,6 +28,7 @@ void launch_gemv(const WTensor&, int pre, const float* xin, const float* gw,
 void launch_gemv_q8(const WTensor&, int pre, const float* xin,
                     const float* gw, const float* res, float* y, int B,
                     int ldy, float eps, hipStream_t);
+void launch_zero(float* p, int64_t n, hipStream_t);
 void launch_embed(const WTensor&, const int32_t* ids, float* x, int B,
                   hipStream_t);
 void launch_attn_decode(const float* qkv, const float* inv_freq,
@@ -271,6 +272,17 @@ Engine::Engine(const std::string& gguf_path, const EngineConfig& cfg)
     meta_.kv_heads_l = meta_.kv_heads / tp;
     meta_.ffn_l = meta_.ffn / tp;
     meta_.vocab_l = meta_.vocab / tp;
+    if (cfg_.kv_keep) {
+        if (cfg_.kv_keep < 1 || cfg_.kv_keep >= cfg_.max_seq)
+            throw std::runtime_error("kv_keep must be in [1, max_seq)");
+        if (cfg_.kv_recent < 0 || cfg_.kv_recent > cfg_.kv_keep)
+            throw std::runtime_error("kv_recent must be in [0, kv_keep]");
+        if (cfg_.page_size < 16 || cfg_.page_size > 1024 ||
+            cfg_.page_size % 16)
+            throw std::runtime_error(
+                "kv_keep needs a page_size that is a multiple of 16, "
+                "at most 1024");
+    }
     load_weights(gf);
     alloc_state();
     reset();
@@ -573,6 +585,22 @@ void Engine::alloc_state() {
     slot_active_ = (uint8_t*)dalloc((size_t)B);
     HIP_CHECK(hipMemset(slot_active_, 1, B));  // all-active by default
     kv_pool_ = (uint16_t*)dalloc((size_t)B * max_pages_ * page_stride_ * 2);
+    kv_host_.assign(B, 0);
+    active_host_.assign(B, 1);
+    if (cfg_.kv_keep) {
+        const size_t rows = (size_t)meta_.layers * B * NKV;
+        kv_len_ = (int32_t*)dalloc((size_t)B * 4);
+        kv_step_ = (int32_t*)dalloc((size_t)B * 4);
+        kv_chunk_ = (int32_t*)dalloc(4 * 4);
+        kv_mass_ = (float*)dalloc(rows * cfg_.max_seq * 4);
+        kv_pos_ = (int32_t*)dalloc(rows * cfg_.max_seq * 4);
+        const KvPages all = kv_pages(0), one = kv_pages(0, 0);
+        kv_ws_ = dalloc(std::max(
+            {kv_attend_workspace(all, NH, cfg_.max_seq, true),
+             kv_observe_workspace(one, NH, cfg_.prefill_chunk, cfg_.max_seq),
+             kv_evict_workspace(all, meta_.layers, cfg_.kv_keep,
+                                cfg_.max_seq)}));
+    }
     {   // i8-GEMM activation-quant scratch, sized for the widest input of
         // any projection at the bigger of decode batch / prefill chunk
         const size_t maxK = std::max<size_t>(
@@ -603,7 +631,86 @@ void Engine::reset() {
     HIP_CHECK(hipMemset(gen_count_, 0, B * 4));
     HIP_CHECK(hipMemset(cur_ids_, 0, B * 4));
     HIP_CHECK(hipMemset(slot_active_, 1, B));
+    if (cfg_.kv_keep) HIP_CHECK(hipMemset(kv_len_, 0, B * 4));
+    kv_host_.assign(B, 0);
+    active_host_.assign(B, 1);
     HIP_CHECK(hipDeviceSynchronize());
+}
+
+// One layer's pages, of all slots or of one.
+KvPages Engine::kv_pages(int layer, int slot) {
+    KvPages kv;
+    kv.pool = kv_pool_ + (int64_t)layer * layer_stride_;
+    kv.page_stride = page_stride_;
+    kv.pages = cfg_.batch * max_pages_;
+    kv.table = page_table_ + (slot < 0 ? 0 : (size_t)slot * max_pages_);
+    kv.table_stride = max_pages_;
+    kv.max_pages = max_pages_;
+    kv.page = cfg_.page_size;
+    kv.slots = slot < 0 ? cfg_.batch : 1;
+    kv.kv_heads = meta_.kv_heads_l;
+    kv.dim = meta_.head_dim;
+    kv.type = KVT::BF16;
+    return kv;
+}
+
+KvRows Engine::kv_rows(void* base, int layer, int slot) {
+    const int64_t head = cfg_.max_seq, of = meta_.kv_heads_l * head;
+    return {reinterpret_cast<int32_t*>(base) +
+                ((int64_t)layer * cfg_.batch + std::max(slot, 0)) * of,
+            of, head};
+}
+
+// One layer's attention of a decode step where places are not positions:
+// rotate and store at kv_step_, attend to what the slot holds.
+void Engine::attend_evicting(int layer, hipStream_t s) {
+    const int NH = meta_.heads_l, NKV = meta_.kv_heads_l, D = meta_.head_dim;
+    const int64_t row = (int64_t)(NH + 2 * NKV) * D;
+    const KvHeads q{qkv_, row, D}, k{qkv_ + (int64_t)NH * D, row, D},
+        v{qkv_ + (int64_t)(NH + NKV) * D, row, D},
+        out{attn_out_, (int64_t)NH * D, D};
+    const KvPages kv = kv_pages(layer);
+    const KvRows mass = kv_rows(kv_mass_, layer);
+    launch_kv_append(kv, k, v, q, q, NH, KVT::F32, cfg_.batch, nullptr,
+                     kv_step_, n_past_, inv_freq_, mass,
+                     kv_rows(kv_pos_, layer), cfg_.max_seq, s);
+    launch_kv_attend(kv, q, out, NH, KVT::F32, kv_step_, 1, mass,
+                     cfg_.max_seq, 1.0f / std::sqrt((float)D), kv_ws_, s);
+}
+
+// One layer of a prompt's chunk: as launch_rope_prefill, and the masses.
+void Engine::prefill_evicting(int layer, int slot, int m, hipStream_t s) {
+    const int NH = meta_.heads_l, NKV = meta_.kv_heads_l, D = meta_.head_dim;
+    const int64_t row = (int64_t)(NH + 2 * NKV) * D;
+    const KvHeads q{qkvp_, row, D}, k{qkvp_ + (int64_t)NH * D, row, D},
+        v{qkvp_ + (int64_t)(NH + NKV) * D, row, D};
+    const KvPages kv = kv_pages(layer, slot);
+    const KvRows mass = kv_rows(kv_mass_, layer, slot);
+    // a prompt starts its slot anew, so places are positions still
+    launch_kv_append(kv, k, v, q, q, NH, KVT::F32, m, kv_chunk_,
+                     kv_chunk_ + 2, kv_chunk_ + 2, inv_freq_, mass,
+                     kv_rows(kv_pos_, layer, slot), cfg_.max_seq, s);
+    launch_kv_observe(kv, q, NH, KVT::F32, m, kv_chunk_, kv_chunk_ + 3, mass,
+                      cfg_.max_seq, 1.0f / std::sqrt((float)D), kv_ws_, s);
+}
+
+// Before a step: slots whose cache is full keep kv_keep of its places. The
+// host counts along, so that only such steps launch anything.
+void Engine::evict_full(hipStream_t s) {
+    bool full = false;
+    for (int32_t& n : kv_host_)
+        if (n >= cfg_.max_seq) {
+            full = true;
+            n = cfg_.kv_keep;
+        }
+    if (!full) return;
+    const int64_t head = cfg_.max_seq, slot = meta_.kv_heads_l * head;
+    const KvLayers mass{kv_mass_, cfg_.batch * slot, slot, head},
+        pos{kv_pos_, cfg_.batch * slot, slot, head};
+    launch_kv_evict(kv_pages(0), meta_.layers, layer_stride_, kv_len_,
+                    kv_len_, n_past_, mass, pos, mass, pos, cfg_.kv_keep,
+                    cfg_.kv_recent, cfg_.max_seq - 1, cfg_.max_seq, kv_ws_,
+                    s);
 }
 
 static bool is_quant_dt(DT t) {
@@ -638,7 +745,7 @@ static void gemm_proj(const Proj& p, const float* X, const float* res,
     for (auto& pt : p.parts)
         zero |= gemm_uses_splitk((int)pt.w.n, (int)pt.w.k, M);
     if (zero && !pre_zeroed)
-        HIP_CHECK(hipMemsetAsync(C, 0, (size_t)M * p.n_total * 4, s));
+        launch_zero(C, (int64_t)M * p.n_total, s);
     const int Kq = (int)p.parts[0].w.k;
     bool any_i8 = false;
     if (qb)
@@ -674,15 +781,19 @@ void Engine::reset_slot(int slot) {
     // async on the engine stream: ordered behind any in-flight decode work,
     // no host serialization (per-stride sync memcpys here
     // serialized the batcher thread against the stream).
+    kv_host_.at(slot) = 0;
     HIP_CHECK(hipMemsetAsync(n_past_ + slot, 0, 4, stream_));
     HIP_CHECK(hipMemsetAsync(gen_count_ + slot, 0, 4, stream_));
     HIP_CHECK(hipMemsetAsync(cur_ids_ + slot, 0, 4, stream_));
+    if (cfg_.kv_keep)
+        HIP_CHECK(hipMemsetAsync(kv_len_ + slot, 0, 4, stream_));
 }
 
 // Park / unpark a slot: idle slots do not advance n_past during shared
 // decode steps (k_argmax_final gate), so the attention scan of an idle
 // slot stays at length 1 instead of creeping with every stride.
 void Engine::set_slot_active(int slot, bool active) {
+    active_host_.at(slot) = active;
     HIP_CHECK(hipMemsetAsync(slot_active_ + slot, active ? 1 : 0, 1, stream_));
 }
 
@@ -699,6 +810,8 @@ void Engine::step(hipStream_t s) {
     };
 
     launch_embed(embed_, cur_ids_, x_, B, s);
+    if (cfg_.kv_keep)
+        launch_kv_step(kv_len_, kv_step_, slot_active_, B, s);
     // B=1 always; B=2 when the register-x GEMV covers the projections
     // (quant weights, hidden a single 2048/4096 stripe): its BB=2 form
     // shares one weight stream between both rows, beating the split-K
@@ -733,8 +846,12 @@ void Engine::step(hipStream_t s) {
             gemm_proj(L.qkv, xn_, nullptr, qkv_, B, s, /*pre_zeroed=*/true,
                       nullptr, -1, false, qb, /*pre_quant=*/fq);
         }
-        const bool fqo = !gemv_path && qb && proj_i8_ok(L.o, B);
-        launch_attn_decode(qkv_, inv_freq_, page_table_, kv_layer, n_past_,
+        const bool fqo = !gemv_path && qb && proj_i8_ok(L.o, B) &&
+                         !cfg_.kv_keep;
+        if (cfg_.kv_keep)
+            attend_evicting(li - 1, s);
+        else
+            launch_attn_decode(qkv_, inv_freq_, page_table_, kv_layer, n_past_,
                            part_o_, part_ml_, attn_tickets_, attn_out_,
                            fqo ? xq_ : nullptr, fqo ? xsc_ : nullptr, B, NH,
                            NKV, D, attn_splits_, cfg_.page_size, max_pages_,
@@ -821,7 +938,7 @@ void Engine::step(hipStream_t s) {
                                 eps, s);
         bool zero = gemm_uses_splitk((int)head_.n, (int)head_.k, B);
         if (zero)
-            HIP_CHECK(hipMemsetAsync(lg, 0, (size_t)B * ldl * 4, s));
+            launch_zero(lg, (int64_t)B * ldl, s);
         if (fqh) {
             launch_gemm_i8(head_, xq_, xsc_, (int)head_.k, nullptr,
                            lg, B, ldl, s);
@@ -897,9 +1014,12 @@ void Engine::prefill_chunk_pass(int slot, int pos0, int m) {
         launch_rmsnorm_rows(xp_, L.attn_norm, xnp_, m, meta_.hidden, eps, s);
         gemm_proj(L.qkv, xnp_, nullptr, qkvp_, m, s, false, nullptr, -1,
                   false, qb);
-        launch_rope_prefill(qkvp_, inv_freq_, page_table_, kv_layer, slot,
-                            pos0, m, NH, NKV, D, cfg_.page_size, max_pages_,
-                            page_stride_, s);
+        if (cfg_.kv_keep)
+            prefill_evicting(li - 1, slot, m, s);
+        else
+            launch_rope_prefill(qkvp_, inv_freq_, page_table_, kv_layer, slot,
+                                pos0, m, NH, NKV, D, cfg_.page_size,
+                                max_pages_, page_stride_, s);
         launch_attn_prefill(qkvp_, page_table_, kv_layer, attnp_, slot, pos0,
                             m, NH, NKV, D, cfg_.page_size, max_pages_,
                             page_stride_, scale, s);
@@ -940,6 +1060,10 @@ void Engine::prefill_slot(int slot, const std::vector<int32_t>& ids) {
         const int m = std::min(cfg_.prefill_chunk, len - done);
         HIP_CHECK(hipMemcpyAsync(pids_, ids.data() + done, (size_t)m * 4,
                                  hipMemcpyHostToDevice, stream_));
+        const int32_t chunk[4] = {0, m, pos0, pos0 + m};
+        if (cfg_.kv_keep)
+            HIP_CHECK(hipMemcpyAsync(kv_chunk_, chunk, sizeof(chunk),
+                                     hipMemcpyHostToDevice, stream_));
         prefill_chunk_pass(slot, pos0, m);
         HIP_CHECK(hipStreamSynchronize(stream_));
         pos0 += m;
@@ -961,6 +1085,10 @@ void Engine::prefill_slot(int slot, const std::vector<int32_t>& ids) {
     const int32_t npast = len - 1, zero = 0;
     HIP_CHECK(hipMemcpy(n_past_ + slot, &npast, 4, hipMemcpyHostToDevice));
     HIP_CHECK(hipMemcpy(gen_count_ + slot, &zero, 4, hipMemcpyHostToDevice));
+    if (cfg_.kv_keep)
+        HIP_CHECK(hipMemcpy(kv_len_ + slot, &len, 4, hipMemcpyHostToDevice));
+    kv_host_[slot] = len;
+    active_host_[slot] = 1;
     // prefill implies the slot is (re)activated before its first argmax
     HIP_CHECK(hipMemsetAsync(slot_active_ + slot, 1, 1, stream_));
     launch_argmax(logits_ + (size_t)slot * meta_.vocab,
@@ -988,6 +1116,11 @@ void Engine::decode(int n_steps) {
     HIP_CHECK(hipEventCreate(&e1));
     HIP_CHECK(hipEventRecord(e0, stream_));
     for (int i = 0; i < n_steps; i++) {
+        if (cfg_.kv_keep) {
+            evict_full(stream_);
+            for (int b = 0; b < cfg_.batch; b++)
+                kv_host_[b] += active_host_[b];
+        }
         if (graph_exec_) {
             HIP_CHECK(hipGraphLaunch(graph_exec_, stream_));
         } else {
@@ -1029,6 +1162,36 @@ int32_t Engine::cur_token(int slot) {
     int32_t id = 0;
     HIP_CHECK(hipMemcpy(&id, cur_ids_ + slot, 4, hipMemcpyDeviceToHost));
     return id;
+}
+
+std::vector<int32_t> Engine::kv_lens() {
+    if (!cfg_.kv_keep) return n_past();
+    std::vector<int32_t> out(cfg_.batch);
+    HIP_CHECK(hipMemcpy(out.data(), kv_len_, cfg_.batch * 4,
+                        hipMemcpyDeviceToHost));
+    return out;
+}
+
+void Engine::kv_places(int layer, int slot, std::vector<int32_t>& pos,
+                       std::vector<float>& mass) {
+    if (!cfg_.kv_keep)
+        throw std::runtime_error("kv_places: the engine has no kv_keep");
+    if (layer < 0 || layer >= meta_.layers || slot < 0 ||
+        slot >= cfg_.batch)
+        throw std::runtime_error("kv_places: no such layer or slot");
+    const size_t n = std::min(kv_lens()[slot], cfg_.max_seq);
+    pos.resize(meta_.kv_heads_l * n);
+    mass.resize(meta_.kv_heads_l * n);
+    const KvRows p = kv_rows(kv_pos_, layer, slot),
+                 w = kv_rows(kv_mass_, layer, slot);
+    for (int h = 0; h < meta_.kv_heads_l && n; h++) {
+        HIP_CHECK(hipMemcpy(pos.data() + h * n,
+                            (int32_t*)p.data + h * p.head_stride, n * 4,
+                            hipMemcpyDeviceToHost));
+        HIP_CHECK(hipMemcpy(mass.data() + h * n,
+                            (float*)w.data + h * w.head_stride, n * 4,
+                            hipMemcpyDeviceToHost));
+    }
 }
 
 std::vector<int32_t> Engine::n_past() {

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "common.h"
+#include "kvcache.h"
 
 namespace cla {
 
@@ -39,6 +40,13 @@ struct EngineConfig {
     // lane-parallel staging — B=1 is bandwidth-, not issue-bound.
     bool gemv_q8 = false;
     std::string nccl_id;       // ncclUniqueId bytes (rank 0 creates)
+    // 0: a slot ends at max_seq places. Otherwise decoding goes on past that:
+    // whenever a slot's cache is full, each layer and kv head keeps kv_keep
+    // of its max_seq places, the kv_recent newest tokens' and of the others
+    // those that have received the most attention (kvcache.h). Tokens keep
+    // their positions; prompts still have to fit into max_seq.
+    int kv_keep = 0;
+    int kv_recent = 0;
 };
 
 struct ModelMeta {
@@ -97,6 +105,12 @@ public:
     void set_cur_token(int slot, int32_t id);
     int32_t cur_token(int slot);
     std::vector<int32_t> n_past();
+    // Places in use of each slot: n_past, less what has been evicted.
+    std::vector<int32_t> kv_lens();
+    // kv_keep: position and accumulated attention weight of a slot's places
+    // in one layer, [kv heads of this rank][places in use].
+    void kv_places(int layer, int slot, std::vector<int32_t>& pos,
+                   std::vector<float>& mass);
 
     size_t vram_bytes() const { return vram_bytes_; }
     double last_decode_ms() const { return last_decode_ms_; }
@@ -169,6 +183,20 @@ private:
     float* tmp_hp_ = nullptr;   // [Mchunk][hidden] prefill all-reduce staging
     float* logits_tp_ = nullptr;  // [B][vocab_l] local slice (tp>1)
     float* gather_tp_ = nullptr;  // [tp][B][vocab_l] all-gather recv (tp>1)
+    // kv_keep > 0: places are no longer positions, and have a mass
+    KvPages kv_pages(int layer, int slot = -1);
+    KvRows kv_rows(void* base, int layer, int slot = -1);
+    void attend_evicting(int layer, hipStream_t s);
+    void prefill_evicting(int layer, int slot, int m, hipStream_t s);
+    void evict_full(hipStream_t s);
+    int32_t* kv_len_ = nullptr;      // [B] places in use
+    int32_t* kv_step_ = nullptr;     // [B] the same for a step; -1: parked
+    int32_t* kv_chunk_ = nullptr;    // prefill chunk: {0, m, pos0, pos0 + m}
+    float* kv_mass_ = nullptr;       // [layers][B][kv heads][max_seq]
+    int32_t* kv_pos_ = nullptr;      // likewise
+    void* kv_ws_ = nullptr;
+    std::vector<int32_t> kv_host_;   // kv_len_ as the host counts along
+    std::vector<uint8_t> active_host_;
     int8_t* xq_ = nullptr;        // [maxM][maxK] i8-GEMM activation quant
     float* xsc_ = nullptr;        // [maxK/32][2][M4] scales + dx*sum(qx)
 };

@@ -1675,8 +1675,21 @@ void launch_scatter_logits(const float* src, float* dst, int B, int Vl,
 }
 
 
-// Clear up to 4 device regions in one launch (replaces several
-// hipMemsetAsync nodes ahead of split-K GEMMs: each memset costs a
+// Clear a region (split-K destinations): a kernel, since memset nodes in a
+// captured graph are not reliable on replays after the first.
+__global__ __launch_bounds__(256) void k_zero(float* __restrict__ p,
+                                              int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n;
+         i += (int64_t)gridDim.x * 256)
+        p[i] = 0.f;
+}
+
+void launch_zero(float* p, int64_t n, hipStream_t stream) {
+    if (n <= 0) return;
+    const int64_t blocks = (n + 1023) / 1024;
+    hipLaunchKernelGGL(k_zero, dim3((uint32_t)(blocks < 2048 ? blocks : 2048)),
+                       dim3(256), 0, stream, p, n);
+}
 
 // Layer-start prep: rmsnorm the residual rows AND clear the split-K
 // destinations in one launch (blocks 0..B-1 normalize one row each; the

@@ -85,6 +85,11 @@ void launch_kv_append(const KvPages& kv, const KvHeads& k, const KvHeads& v,
                       const float* inv_freq, const KvRows& mass,
                       const KvRows& pos, int reach, hipStream_t stream);
 
+// A decode step's places: step[b] is where slot b's next token goes, -1 for a
+// slot that takes no part; len counts the tokens of those that do.
+void launch_kv_step(int32_t* len, int32_t* step, const uint8_t* active,
+                    int slots, hipStream_t stream);
+
 // One new token's attention over each sequence's first lens[b] places;
 // mass (may be null) gets each place's weight added, summed over the query
 // heads of the kv head. `add` is added to each length.

@@ -301,6 +301,14 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     }
 }
 
+__global__ __launch_bounds__(64) void k_kv_step(
+    int32_t* len, int32_t* step, const uint8_t* active, int slots) {
+    for (int b = threadIdx.x; b < slots; b += 64) {
+        step[b] = active[b] ? len[b] : -1;
+        if (active[b]) len[b]++;
+    }
+}
+
 // ------------------------------------------------------------------- attend
 
 constexpr int TILE = 32;          // places a wave takes at a time
@@ -1082,6 +1090,13 @@ void launch_kv_append(const KvPages& kv, const KvHeads& k, const KvHeads& v,
         APPEND(KVT::F32, KVT::BF16);
     }
     #undef APPEND
+    check_launch();
+}
+
+void launch_kv_step(int32_t* len, int32_t* step, const uint8_t* active,
+                    int slots, hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv_step, dim3(1), dim3(64), 0, stream, len, step,
+                       active, slots);
     check_launch();
 }
 

@@ -197,3 +197,35 @@ def test_order_of_eviction():
     assert key(-0., False) == key(0., False)
     assert key(math.copysign(math.nan, -1), False) == keys[0]
     assert all(key(m, True) == 2 ** 32 - 1 > max(keys) for m in masses)
+
+
+def test_token_budget():
+    from crowdllama_amd.engine.api import token_budget
+    assert token_budget(100, 20, 64, 64) == 43
+    assert token_budget(10, 20, 64, 64) == 10
+    assert token_budget(100, 63, 64, 64) == 0
+    assert token_budget(100, 20, 64, 1024, kv_keep=40) == 100
+    assert token_budget(5000, 20, 64, 1024, kv_keep=40) == 1024
+    assert token_budget(100, 63, 64, 1024, kv_keep=40) < 1
+
+
+def test_reference_evicts(tmp_path):
+    """The numpy reference past max_seq: every head keeps the newest tokens,
+    and its places' masses add up to what the tokens gave."""
+    from crowdllama_amd.engine.ref_numpy import RefLlama
+    from crowdllama_amd.models import write_synthetic_gguf
+    path = write_synthetic_gguf(str(tmp_path / "t.gguf"), "testllama",
+                                scheme="f32", mode="exact", seed=1)
+    full = RefLlama(path)
+    ref = RefLlama(path, max_seq=12, kv_keep=7, kv_recent=3)
+    for i in range(12):
+        a, b = full.step(i + 3), ref.step(i + 3)
+        assert abs(a - b).max() < 1e-5 * abs(a).max()
+    ref.step(50)
+    for layer in ref.places:
+        for row in layer:
+            pos = [e[3] for e in row]
+            assert len(row) == 8 and len(set(pos)) == 8 and pos[-1] == 12
+            assert {9, 10, 11} <= set(pos)
+    ref.reset()
+    assert ref.n_past == 0 and ref.places[0][0] == []
