@@ -21,6 +21,10 @@ ARCH = os.environ.get("CLA_GFX_ARCH", "gfx950")
 # wrong results now and then: no kernel is compiled with them
 HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
+# kvcache.hip's kernels work on every matrix product's result at once; results
+# in accumulation registers cost a move each
+FILE_FLAGS = {"kvcache.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 SOURCES = ["gguf.cpp", "engine.cpp", "testutil.cpp", "bindings.cpp",
            "kernels.hip", "mfma_probe.hip", "gemm.hip", "gemm_i8.hip",
            "kvcache.hip", "kv_bindings.cpp", "tokenizer.cpp"]
@@ -62,7 +66,7 @@ def build(verbose: bool = True, force: bool = False) -> str:
                "-I", CSRC, "-I", py_inc, "-I", pybind11.get_include(),
                "-c", os.path.join(CSRC, src), "-o", obj]
         if src.endswith(".hip"):
-            cmd[1:1] = ["-x", "hip", *HIP_FLAGS]
+            cmd[1:1] = ["-x", "hip", *HIP_FLAGS, *FILE_FLAGS.get(src, [])]
         if verbose:
             print("[ops.build]", " ".join(cmd), file=sys.stderr)
         procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE,

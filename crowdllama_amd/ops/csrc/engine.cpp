@@ -597,7 +597,8 @@ void Engine::alloc_state() {
         const KvPages all = kv_pages(0), one = kv_pages(0, 0);
         kv_ws_ = dalloc(std::max(
             {kv_attend_workspace(all, NH, cfg_.max_seq, true),
-             kv_observe_workspace(one, NH, cfg_.prefill_chunk, cfg_.max_seq),
+             kv_observe_workspace(one, NH, cfg_.prefill_chunk, cfg_.max_seq,
+                                  KVT::F32),
              kv_evict_workspace(all, meta_.layers, cfg_.kv_keep,
                                 cfg_.max_seq)}));
     }

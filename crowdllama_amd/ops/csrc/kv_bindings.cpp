@@ -102,8 +102,9 @@ void bind_kv(py::module_& m) {
                          rows(mass), reach, scale, at<void>(ws), stream(s));
     });
     m.def("kv_observe_workspace", [](const PagesArg& kv, int q_heads, int n,
-                                     int reach) {
-        return kv_observe_workspace(pages(kv), q_heads, n, reach);
+                                     int reach, int type) {
+        return kv_observe_workspace(pages(kv), q_heads, n, reach,
+                                    static_cast<KVT>(type));
     });
     m.def("kv_observe", [](const PagesArg& kv, const HeadsArg& q, int q_heads,
                            int type, int n, uintptr_t starts, uintptr_t lens,

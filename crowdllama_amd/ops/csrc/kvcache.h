@@ -103,7 +103,7 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
 // The weight that `rows` tokens at the ends of their sequences gave to each
 // place they see, added to mass.
 size_t kv_observe_workspace(const KvPages& kv, int q_heads, int rows,
-                            int reach);
+                            int reach, KVT type);
 void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                        KVT type, int rows, const int32_t* starts,
                        const int32_t* lens, const KvRows& mass, int reach,

@@ -145,6 +145,11 @@ void check_pages(const KvPages& kv, int q_heads, int reach) {
             "query heads must be 1 to 16 times the kv heads");
 }
 
+void check_scale(float scale) {
+    if (!(scale > 0.f && scale < INFINITY))
+        throw std::runtime_error("scale must be positive and finite");
+}
+
 void check_launch() {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess)
@@ -699,6 +704,21 @@ __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
 
 // ------------------------------------------------------------------ observe
 
+// x / d for x * d < 2^32
+struct Div {
+    uint32_t d, magic;
+    __device__ __forceinline__ int of(int x) const {
+        return d == 1 ? x : (int)__umulhi((uint32_t)x, magic);
+    }
+};
+
+Div div_by(int d) {
+    return {(uint32_t)d,
+            d > 1 ? (uint32_t)((0xFFFFFFFFull + (uint32_t)d) / d) : 0u};
+}
+
+constexpr int OBS_PLACES = 256;   // places of a workgroup of the second pass
+
 struct ObserveArgs {
     Pages kv;
     KvHeads q;
@@ -706,7 +726,15 @@ struct ObserveArgs {
     const int32_t *starts, *lens;
     int32_t q_heads, kv_heads, slots, rows, reach;
     float scale2;
-    float* lse;        // [q heads][rows]: log2 of the sum of 2^scores
+    Div group;
+    // first pass: places in parts of `part`, of which there are `parts`
+    int32_t part, parts;
+    // second pass: rows in chunks of `chunk`, of which there are `chunks`
+    int32_t chunk, chunks;
+    float* sums;       // [parts][kv heads][rows][G][2]: maximum, sum
+    float* lse;        // [kv heads][rows][G]: log2 of the sum of 2^scores
+    float* partial;    // [chunks][slots][kv heads][ld]
+    int64_t ld;
 };
 
 // A sequence's rows as the kernels see them: r = i * G + h, query head h of
@@ -724,78 +752,199 @@ __device__ __forceinline__ Seq sequence_at(const ObserveArgs& a, int b) {
     return s;
 }
 
-// Pass 1, grid (row blocks, kv heads): 16 * RW rows a wave, over all the
-// places that they see. Each lane keeps a maximum and a sum of its own for
-// each of its columns; they meet at the end.
+// Rows are staged in LDS with 16 bytes more than they have: an odd number of
+// 16-byte units, so that 16 lanes that read one unit each of 16 rows meet in
+// no bank.
+template <int D> constexpr int LDS_ROW = D + 8;
+
+struct True { constexpr operator bool() const { return true; } };
+struct False { constexpr operator bool() const { return false; } };
+
+template <int D>
+__device__ __forceinline__ u32x4 lds_unit(const uint16_t* rows, int r,
+                                          int unit) {
+    return *reinterpret_cast<const u32x4*>(rows + r * LDS_ROW<D> + unit * 8);
+}
+
+__device__ __forceinline__ float row_lse(float m, float l) {
+    // a row that sees nothing gives nothing: 2^(s - inf)
+    return l == 0.f ? INFINITY : m + __log2f(l);
+}
+
+// Pass 1, grid (row blocks, kv heads, parts): 16 * RW rows a wave, whose
+// queries stay in registers, over the part's places, which the workgroup
+// stages 64 at a time. Each lane keeps a sum (and a maximum, where it needs
+// one) of its own for each of its columns; they meet at the end.
+//
+// Three waves a SIMD for one piece (375 us for 8192 rows of 32 heads, 442 with
+// two), two for three (249 us for 3 x 500 rows over 16000 places, 290 with
+// three waves, which spill).
 template <class C, int NQ, int D, int RW>
-__global__ __launch_bounds__(256) void k_kv_observe_sums(ObserveArgs a) {
-    constexpr int ROWS = 16 * RW * WAVES;
+__global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(ObserveArgs a) {
+    constexpr int ROWS = 16 * RW * WAVES, KT = 64, PER = 16 * D / 8 / 64;
+    __shared__ __align__(16) uint16_t s_k[2][KT * LDS_ROW<D>];
+    __shared__ int s_there[2][4];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
-    const int G = a.q_heads / a.kv_heads;
-    // which sequence's block this is
-    int id = blockIdx.x, b = 0;
-    Seq s;
-    for (;; b++) {
-        if (b == a.slots) return;
-        s = sequence_at(a, b);
-        const int blocks = (s.m * G + ROWS - 1) / ROWS;
-        if (id < blocks) break;
-        id -= blocks;
+    const int G = a.group.d;
+    // which sequence's block this is; a sequence's last rows, which see the
+    // most, go first
+    int id = -1;
+    Seq s{};
+    for (int base = 0, before = 0; base < a.slots; base += 64) {
+        const int b = base + lane;
+        int blocks = 0;
+        if (b < a.slots) {
+            const Seq x = sequence_at(a, b);
+            blocks = (x.m * G + ROWS - 1) / ROWS;
+        }
+        int upto = blocks;
+        #pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int x = __shfl_up(upto, m, 64);
+            if (lane >= m) upto += x;
+        }
+        const uint64_t over = __ballot(before + upto > (int)blockIdx.x);
+        if (over) {
+            const int at = __builtin_ctzll(over);
+            s = sequence_at(a, base + at);
+            id = before + __shfl(upto, at, 64) - 1 - blockIdx.x;
+            break;
+        }
+        before += __shfl(upto, 63, 64);
     }
+    if (id < 0) return;
+    const int R = s.m * G;
     const int r0 = id * ROWS + wave * 16 * RW;
-    if (r0 >= s.m * G) return;
+    // places that the workgroup's last row, and the wave's first, see
+    const int most = s.len - s.m
+        + a.group.of(min(id * ROWS + ROWS, R) - 1) + 1;
+    const int least = s.len - s.m + a.group.of(r0) + 1;
+    const int begin = blockIdx.z * a.part, end = min(begin + a.part, most);
 
     u32x4 q[RW][NQ][D / 32];
     float m[RW], l[RW];
     int seen[RW];          // places that the lane's column sees
     #pragma unroll
     for (int w = 0; w < RW; w++) {
-        const int r = r0 + w * 16 + n, i = r / G, h = r % G;
-        const bool there = r < s.m * G;
+        const int r = r0 + w * 16 + n, i = a.group.of(r), h = r - i * G;
+        const bool there = r < R;
         load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
                              + (int64_t)(head * G + h) * a.q.head_stride,
                          there, g, q[w]);
-        m[w] = -INFINITY;
-        l[w] = 0.f;
         seen[w] = there ? s.len - s.m + i + 1 : 0;
     }
-    const int r_last = min(r0 + 16 * RW, s.m * G) - 1;
-    const int least = s.len - s.m + r0 / G + 1;
-    const int most = s.len - s.m + r_last / G + 1;
-    for (int p0 = 0; p0 < most; p0 += 16) {
-        const uint16_t* rows = a.kv.rows16(b, p0, head, D);
-        if (!rows) continue;
-        u32x4 k[D / 32];
+
+    u32x4 next[PER];
+    bool next_there;
+    auto fetch = [&](int p0) {
+        const int p = p0 + wave * 16;
+        const uint16_t* rows = p < end ? a.kv.rows16(s.b, p, head, D)
+                                       : nullptr;
+        next_there = rows != nullptr;
+        if (!rows) rows = a.kv.pool;
         #pragma unroll
-        for (int kk = 0; kk < D / 32; kk++)
-            k[kk] = *reinterpret_cast<const u32x4*>(
-                rows + n * D + kk * 32 + g * 8);
+        for (int x = 0; x < PER; x++)
+            next[x] = reinterpret_cast<const u32x4*>(rows)[x * 64 + lane];
+    };
+    auto stage = [&](int buf) {
+        #pragma unroll
+        for (int x = 0; x < PER; x++) {
+            const int u = x * 64 + lane;
+            *reinterpret_cast<u32x4*>(
+                &s_k[buf][(wave * 16 + u / (D / 8)) * LDS_ROW<D>
+                          + u % (D / 8) * 8]) = next[x];
+        }
+        if (lane == 0) s_there[buf][wave] = next_there;
+    };
+    // 32 places (the tile's half `half`) against the wave's rows. CUT: some
+    // row does not see them all, or a page is missing. MAX: relative to a
+    // running maximum, else to 0.
+    auto half_tile = [&](int buf, int half, int pu, bool t0, bool t1,
+                         auto CUT, auto MAX) {
+        u32x4 k[2][D / 32];
+        #pragma unroll
+        for (int u = 0; u < 2; u++)
+            #pragma unroll
+            for (int kk = 0; kk < D / 32; kk++)
+                k[u][kk] = lds_unit<D>(s_k[buf], half * 32 + u * 16 + n,
+                                       kk * 4 + g);
         #pragma unroll
         for (int w = 0; w < RW; w++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
             #pragma unroll
             for (int x = NQ - 1; x >= 0; x--)
                 #pragma unroll
                 for (int kk = 0; kk < D / 32; kk++)
-                    acc = C::mfma(k[kk], q[w][x][kk], acc);
+                    #pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        acc[u] = C::mfma(k[u][kk], q[w][x][kk], acc[u]);
+            float e[8];
             #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                acc[i] *= a.scale2;
-                if (p0 + 16 > least && p0 + g * 4 + i >= seen[w])
-                    acc[i] = -INFINITY;
+            for (int j = 0; j < 8; j++) {
+                e[j] = acc[j >> 2][j & 3] * a.scale2;
+                if (CUT && (!(j < 4 ? t0 : t1) ||
+                            pu + (j >> 2) * 16 + g * 4 + (j & 3) >= seen[w]))
+                    e[j] = -INFINITY;
             }
-            const float top = fmaxf(fmaxf(acc[0], acc[1]),
-                                    fmaxf(acc[2], acc[3]));
-            const float now = fmaxf(m[w], top);
-            const float ref = now == -INFINITY ? 0.f : now;
-            l[w] *= exp2_fast(m[w] - ref);
-            m[w] = now;
+            if (MAX) {
+                float top = m[w];
+                #pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, e[j]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                l[w] *= exp2_fast(m[w] - ref);
+                m[w] = top;
+                #pragma unroll
+                for (int j = 0; j < 8; j++) e[j] -= ref;
+            }
             #pragma unroll
-            for (int i = 0; i < 4; i++) l[w] += exp2_fast(acc[i] - ref);
+            for (int j = 0; j < 8; j++) e[j] = exp2_fast(e[j]);
+            l[w] += ((e[0] + e[1]) + (e[2] + e[3]))
+                + ((e[4] + e[5]) + (e[6] + e[7]));
         }
+    };
+    auto pass = [&](auto MAX) {
+        #pragma unroll
+        for (int w = 0; w < RW; w++) {
+            m[w] = MAX ? -INFINITY : 0.f;
+            l[w] = 0.f;
+        }
+        if (begin < end) {
+            fetch(begin);
+            stage(0);
+        }
+        __syncthreads();
+        int buf = 0;
+        for (int p0 = begin; p0 < end; p0 += KT, buf ^= 1) {
+            const bool more = p0 + KT < end;
+            if (more) fetch(p0 + KT);
+            #pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const int pu = p0 + half * 32;
+                const bool t0 = s_there[buf][half * 2];
+                const bool t1 = s_there[buf][half * 2 + 1];
+                if (t0 && t1 && pu + 32 <= least)
+                    half_tile(buf, half, pu, t0, t1, False{}, MAX);
+                else if (t0 || t1)
+                    half_tile(buf, half, pu, t0, t1, True{}, MAX);
+            }
+            if (more) stage(buf ^ 1);
+            __syncthreads();
+        }
+    };
+    // Exponentials relative to 0 need no maximum, and are as exact where
+    // they neither overflow nor vanish; where some row's might have, the
+    // workgroup starts over with one.
+    pass(False{});
+    bool odd = false;
+    #pragma unroll
+    for (int w = 0; w < RW; w++) {
+        const float sum = wave_xor_sum(wave_xor_sum(l[w], 16), 32);
+        odd |= begin < min(end, seen[w]) &&
+            !(sum > 0x1p-60f && sum < 0x1p120f);
     }
+    if (__syncthreads_or(odd)) pass(True{});
     #pragma unroll
     for (int w = 0; w < RW; w++) {
         const float top = wave_xor_max(wave_xor_max(m[w], 16), 32);
@@ -803,23 +952,68 @@ __global__ __launch_bounds__(256) void k_kv_observe_sums(ObserveArgs a) {
         float sum = l[w] * exp2_fast(m[w] - ref);
         sum = wave_xor_sum(wave_xor_sum(sum, 16), 32);
         const int r = r0 + w * 16 + n;
-        if (g == 0 && r < s.m * G)
-            a.lse[(int64_t)(head * G + r % G) * a.rows + s.t0 + r / G] =
-                sum == 0.f ? INFINITY : ref + __log2f(sum);
+        if (g == 0 && r < R) {
+            const int64_t at = ((int64_t)head * a.rows + s.t0) * G + r;
+            if (a.parts == 1) {
+                a.lse[at] = row_lse(top, sum);
+            } else {
+                float* d = a.sums + ((int64_t)blockIdx.z * a.q_heads * a.rows
+                                     + at) * 2;
+                d[0] = top;
+                d[1] = sum;
+            }
+        }
     }
 }
 
-// Pass 2, grid (place blocks, kv heads, slots): 16 * PW places a wave, over
-// all rows that see them; a lane sums its columns' weights for its places.
+// Join the parts of the rows' sums. Which parts there are goes by the row's
+// workgroup in pass 1, but a part that its row does not see gave (-inf, 0).
+__global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t all = (int64_t)a.q_heads * a.rows;
+    if (at >= all) return;
+    float m = -INFINITY, l = 0.f;
+    for (int p = 0; p < a.parts; p++) {
+        const float mp = a.sums[(p * all + at) * 2];
+        const float lp = a.sums[(p * all + at) * 2 + 1];
+        const float now = fmaxf(m, mp);
+        const float ref = now == -INFINITY ? 0.f : now;
+        l = l * exp2_fast(m - ref) + lp * exp2_fast(mp - ref);
+        m = now;
+    }
+    a.lse[at] = row_lse(m, l);
+}
+
+// Pass 2, grid (place blocks x chunks, kv heads, slots): 16 * PW places a
+// wave, whose keys stay in registers, over the chunk's rows, which the
+// workgroup stages QT at a time; a lane sums its columns' weights for its
+// places. Where the rows are one chunk the sums go to the mass, else to
+// `partial`, and the last kernel adds them in order.
 template <class C, int NQ, int D, int PW>
 __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
+    constexpr int QT = NQ == 1 ? 64 : 32, UNITS = QT * D / 8;
+    constexpr int PER = (UNITS + 255) / 256;
+    static_assert(16 * PW * WAVES == OBS_PLACES, "places of a workgroup");
+    __shared__ __align__(16) uint16_t s_q[2][NQ][QT * LDS_ROW<D>];
+    __shared__ float s_lse[2][QT];
+    __shared__ int s_seen[2][QT];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
-    const int G = a.q_heads / a.kv_heads;
+    const int G = a.group.d;
     const Seq s = sequence_at(a, blockIdx.z);
-    const int p0 = (blockIdx.x * WAVES + wave) * 16 * PW;
-    if (p0 >= s.len || s.m == 0) return;
+    // late chunks are seen by more places than early ones: turned from block
+    // to block, so that no XCD (every eighth workgroup) gets the late ones
+    const int block = blockIdx.x / a.chunks;
+    const int chunk = (blockIdx.x + block) % a.chunks;
+    const int first = block * OBS_PLACES, p0 = first + wave * 16 * PW;
+    const int R = s.m * G;
+    // rows from the first that sees the block's first place on
+    const int from = max(0, first - (s.len - s.m)) * G;
+    const int begin = max(chunk * a.chunk, from / QT * QT);
+    const int end = min(chunk * a.chunk + a.chunk, R);
+    if (first >= s.len || begin >= end) return;
+
     u32x4 k[PW][D / 32];
     bool there[PW];
     #pragma unroll
@@ -836,36 +1030,138 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     f32x4 sum[PW];
     #pragma unroll
     for (int u = 0; u < PW; u++) sum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int i0 = max(0, p0 - (s.len - s.m));   // the first row that sees p0
-    const int R = s.m * G;
-    for (int r0 = i0 * G / 16 * 16; r0 < R; r0 += 16) {
-        const int r = r0 + n, i = r / G, h = r % G;
-        u32x4 q[NQ][D / 32];
-        load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
-                             + (int64_t)(head * G + h) * a.q.head_stride,
-                         r < R, g, q);
-        const float lse = r < R
-            ? a.lse[(int64_t)(head * G + h) * a.rows + s.t0 + i] : INFINITY;
-        const int seen = r < R ? s.len - s.m + i + 1 : 0;
-        const bool whole = r0 + 16 <= R &&
-            p0 + 16 * PW <= s.len - s.m + r0 / G + 1;
+
+    // a thread's units of a tile of queries: where they are, and their rows'
+    // heads, both moved on from tile to tile
+    constexpr int FULL = NQ > 1 ? 2 : 1;
+    const char* from_q[PER];
+    int h_of[PER];
+    u32x4 next[PER][FULL];
+    const int64_t size = NQ > 1 ? 4 : 2;
+    const int step_i = a.group.of(QT), step_h = QT - step_i * G;
+    const int64_t step = (step_i * a.q.row_stride
+                          + step_h * a.q.head_stride) * size;
+    const int64_t wrap = (a.q.row_stride - G * a.q.head_stride) * size;
+    #pragma unroll
+    for (int x = 0; x < PER; x++) {
+        const int u = x * 256 + tid, r = begin + u / (D / 8);
+        const int i = a.group.of(r);
+        h_of[x] = r - i * G;
+        from_q[x] = reinterpret_cast<const char*>(a.q.data)
+            + ((int64_t)(s.t0 + i) * a.q.row_stride
+               + (int64_t)(head * G + h_of[x]) * a.q.head_stride
+               + u % (D / 8) * 8) * size;
+    }
+    const float* from_lse = a.lse + ((int64_t)head * a.rows + s.t0) * G;
+    float next_lse = INFINITY;
+    int next_seen = 0;
+    auto fetch = [&](int r0) {
         #pragma unroll
-        for (int u = 0; u < PW; u++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < PER; x++) {
+            const int u = x * 256 + tid;
+            const bool there = (UNITS % 256 == 0 || u < UNITS)
+                && r0 + u / (D / 8) < R;
             #pragma unroll
-            for (int x = NQ - 1; x >= 0; x--)
-                #pragma unroll
-                for (int kk = 0; kk < D / 32; kk++)
-                    acc = C::mfma(k[u][kk], q[x][kk], acc);
-            #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float w = exp2_fast(fmaf(acc[e], a.scale2, -lse));
-                sum[u][e] += whole || p0 + u * 16 + g * 4 + e < seen ? w : 0.f;
+            for (int y = 0; y < FULL; y++)
+                next[x][y] = there
+                    ? reinterpret_cast<const u32x4*>(from_q[x])[y]
+                    : u32x4{0, 0, 0, 0};
+            from_q[x] += step;
+            if (step_h) {
+                h_of[x] += step_h;
+                if (h_of[x] >= G) {
+                    h_of[x] -= G;
+                    from_q[x] += wrap;
+                }
             }
         }
+        if (tid < QT) {
+            const int r = r0 + tid;
+            next_lse = r < R ? from_lse[r] : INFINITY;
+            next_seen = r < R ? s.len - s.m + a.group.of(r) + 1 : 0;
+        }
+    };
+    auto stage = [&](int buf) {
+        #pragma unroll
+        for (int x = 0; x < PER; x++) {
+            const int u = x * 256 + tid;
+            if (UNITS % 256 && u >= UNITS) break;
+            const int at = u / (D / 8) * LDS_ROW<D> + u % (D / 8) * 8;
+            if constexpr (NQ == 1) {
+                *reinterpret_cast<u32x4*>(&s_q[buf][0][at]) = next[x][0];
+            } else {
+                const f32x4 f0 = bits<f32x4>(next[x][0]);
+                const f32x4 f1 = bits<f32x4>(next[x][1]);
+                float f[8] = {f0[0], f0[1], f0[2], f0[3],
+                              f1[0], f1[1], f1[2], f1[3]};
+                #pragma unroll
+                for (int p = 0; p < NQ; p++) {
+                    u32x4 w;
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        w[i] = C::piece(f[2 * i], f[2 * i + 1]);
+                    *reinterpret_cast<u32x4*>(&s_q[buf][p][at]) = w;
+                }
+            }
+        }
+        if (tid < QT) {
+            s_lse[buf][tid] = next_lse;
+            s_seen[buf][tid] = next_seen;
+        }
+    };
+    // 16 rows against the wave's places. CUT: some row does not see them all
+    auto rows16 = [&](const u32x4 (*q)[D / 32], float lse, int seen,
+                      auto CUT) {
+        f32x4 acc[PW];
+        #pragma unroll
+        for (int u = 0; u < PW; u++) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int x = NQ - 1; x >= 0; x--)
+            #pragma unroll
+            for (int kk = 0; kk < D / 32; kk++)
+                #pragma unroll
+                for (int u = 0; u < PW; u++)
+                    acc[u] = C::mfma(k[u][kk], q[x][kk], acc[u]);
+        #pragma unroll
+        for (int u = 0; u < PW; u++)
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float w = exp2_fast(fmaf(acc[u][e], a.scale2, -lse));
+                sum[u][e] += !CUT || p0 + u * 16 + g * 4 + e < seen ? w : 0.f;
+            }
+    };
+    fetch(begin);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int r0 = begin; r0 < end; r0 += QT, buf ^= 1) {
+        const bool more = r0 + QT < end;
+        if (more) fetch(r0 + QT);
+        #pragma unroll
+        for (int t = 0; t < QT / 16; t++) {
+            u32x4 q[NQ][D / 32];
+            #pragma unroll
+            for (int x = 0; x < NQ; x++)
+                #pragma unroll
+                for (int kk = 0; kk < D / 32; kk++)
+                    q[x][kk] = lds_unit<D>(s_q[buf][x], t * 16 + n,
+                                           kk * 4 + g);
+            const float lse = s_lse[buf][t * 16 + n];
+            const int seen = s_seen[buf][t * 16 + n];
+            // rows past the last see 0 places
+            if (__any(p0 + 16 * PW > seen))
+                rows16(q, lse, seen, True{});
+            else
+                rows16(q, lse, seen, False{});
+        }
+        if (more) stage(buf ^ 1);
+        __syncthreads();
     }
-    float* mass = reinterpret_cast<float*>(a.mass.data)
-        + s.b * a.mass.slot_stride + head * a.mass.head_stride;
+    float* to = a.chunks == 1
+        ? reinterpret_cast<float*>(a.mass.data) + s.b * a.mass.slot_stride
+            + head * a.mass.head_stride
+        : a.partial + (((int64_t)chunk * a.slots + s.b) * a.kv_heads + head)
+            * a.ld;
     #pragma unroll
     for (int u = 0; u < PW; u++)
         #pragma unroll
@@ -874,8 +1170,29 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
             #pragma unroll
             for (int x = 1; x < 16; x <<= 1) w = wave_xor_sum(w, x);
             const int p = p0 + u * 16 + g * 4 + e;
-            if (n == 0 && p < s.len && there[u]) mass[p] += w;
+            if (n == 0 && p < s.len) {
+                if (a.chunks > 1) to[p] = there[u] ? w : 0.f;
+                else if (there[u]) to[p] += w;
+            }
         }
+}
+
+// Add the chunks of rows: those that the second pass made, in their order.
+__global__ __launch_bounds__(256) void k_kv_observe_add(ObserveArgs a) {
+    const int p = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
+    const Seq s = sequence_at(a, blockIdx.z);
+    const int G = a.group.d, R = s.m * G;
+    if (p >= s.len || R == 0) return;
+    const int from = max(0, p / OBS_PLACES * OBS_PLACES - (s.len - s.m)) * G;
+    if (from >= R) return;
+    const float* part = a.partial
+        + ((int64_t)s.b * a.kv_heads + head) * a.ld + p;
+    const int64_t step = (int64_t)a.slots * a.kv_heads * a.ld;
+    float w = 0.f;
+    for (int c = from / a.chunk; c <= (R - 1) / a.chunk; c++)
+        w += part[c * step];
+    reinterpret_cast<float*>(a.mass.data)[
+        s.b * a.mass.slot_stride + head * a.mass.head_stride + p] += w;
 }
 
 // -------------------------------------------------------------------- evict
@@ -1123,6 +1440,7 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
                       const KvRows& mass, int reach, float scale, void* ws,
                       hipStream_t stream) {
     check_pages(kv, q_heads, reach);
+    check_scale(scale);
     const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
     char* w = reinterpret_cast<char*>(ws);
     AttendArgs a{pages_of(kv), q, out, mass, lens, add, q_heads, kv.kv_heads,
@@ -1146,10 +1464,52 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
     check_launch();
 }
 
+namespace {
+
+// How the two passes of observe are cut: into at least OBSERVE_WGS
+// workgroups where there is the work for that, since a pass that has fewer
+// waits for its longest ones (causal rows and places are uneven).
+constexpr int OBSERVE_WGS = 4096;
+
+struct ObserveCut {
+    int64_t blocks, parts, part, chunks, chunk, place_blocks;
+    int64_t sums, lse, partial;     // bytes
+};
+
+ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
+                       KVT type) {
+    if ((int64_t)rows * (q_heads / kv.kv_heads) >= (1ll << 28))
+        throw std::runtime_error("observe: too many rows");
+    const int64_t G = q_heads / kv.kv_heads, R = std::max<int64_t>(rows, 1) * G;
+    const int64_t per = 16 * WAVES * (type == KVT::F32 ? 2 : 4);
+    auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    ObserveCut c;
+    c.blocks = up(R, per) + kv.slots - 1;
+    const int64_t places = std::max(reach, 1);
+    c.parts = std::min(up(OBSERVE_WGS, c.blocks * kv.kv_heads),
+                       up(places, 512));
+    c.part = up(up(places, c.parts), 64) * 64;
+    c.parts = up(places, c.part);
+    c.place_blocks = up(places, OBS_PLACES);
+    c.chunks = std::min(
+        up(OBSERVE_WGS, c.place_blocks * kv.kv_heads * kv.slots), up(R, 128));
+    c.chunk = up(up(R, c.chunks), 64) * 64;
+    c.chunks = up(R, c.chunk);
+    c.sums = c.parts > 1 ? aligned((size_t)c.parts * rows * q_heads * 8) : 0;
+    c.lse = aligned((size_t)std::max(rows, 1) * q_heads * 4);
+    c.partial = c.chunks > 1
+        ? aligned((size_t)c.chunks * kv.slots * kv.kv_heads
+                  * c.place_blocks * OBS_PLACES * 4) : 0;
+    return c;
+}
+
+}  // namespace
+
 size_t kv_observe_workspace(const KvPages& kv, int q_heads, int rows,
-                            int reach) {
+                            int reach, KVT type) {
     check_pages(kv, q_heads, reach);
-    return aligned((size_t)q_heads * std::max(rows, 1) * 4);
+    const ObserveCut c = observe_cut(kv, q_heads, rows, reach, type);
+    return c.sums + c.lse + c.partial;
 }
 
 void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
@@ -1157,24 +1517,41 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                        const int32_t* lens, const KvRows& mass, int reach,
                        float scale, void* ws, hipStream_t stream) {
     check_pages(kv, q_heads, reach);
+    check_scale(scale);
     if (rows <= 0 || reach == 0) return;
-    if ((int64_t)rows * (q_heads / kv.kv_heads) >= (1ll << 30))
-        throw std::runtime_error("observe: too many rows");
-    const int G = q_heads / kv.kv_heads;
+    const ObserveCut c = observe_cut(kv, q_heads, rows, reach, type);
+    if (c.parts > 65535 || kv.kv_heads > 65535 || kv.slots > 65535)
+        throw std::runtime_error("observe: too many sequences or kv heads");
+    char* w = reinterpret_cast<char*>(ws);
     ObserveArgs a{pages_of(kv), q, mass, starts, lens, q_heads, kv.kv_heads,
                   kv.slots, rows, reach, scale * LOG2E,
-                  reinterpret_cast<float*>(ws)};
+                  div_by(q_heads / kv.kv_heads), (int32_t)c.part,
+                  (int32_t)c.parts, (int32_t)c.chunk, (int32_t)c.chunks,
+                  reinterpret_cast<float*>(w),
+                  reinterpret_cast<float*>(w + c.sums),
+                  reinterpret_cast<float*>(w + c.sums + c.lse),
+                  c.place_blocks * OBS_PLACES};
     KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
-        constexpr int RW = NQ > 1 ? 2 : 4, PW = 4;
-        const int64_t per = 16 * RW * WAVES;
+        constexpr int RW = NQ > 1 ? 2 : 4;
         hipLaunchKernelGGL((k_kv_observe_sums<C, NQ, D, RW>),
-                           dim3((uint32_t)(((int64_t)rows * G + per - 1) / per
-                                           + kv.slots), kv.kv_heads),
+                           dim3((uint32_t)c.blocks, kv.kv_heads,
+                                (uint32_t)c.parts),
                            dim3(256), 0, stream, a);
-        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D, PW>),
-                           dim3((reach + 16 * PW * WAVES - 1)
-                                / (16 * PW * WAVES), kv.kv_heads, kv.slots),
+        if (c.parts > 1)
+            hipLaunchKernelGGL(k_kv_observe_join,
+                               dim3((uint32_t)(((int64_t)rows * q_heads + 255)
+                                               / 256)),
+                               dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D,
+                                              OBS_PLACES / 16 / WAVES>),
+                           dim3((uint32_t)(c.place_blocks * c.chunks),
+                                kv.kv_heads, kv.slots),
                            dim3(256), 0, stream, a);
+        if (c.chunks > 1)
+            hipLaunchKernelGGL(k_kv_observe_add,
+                               dim3((uint32_t)c.place_blocks, kv.kv_heads,
+                                    kv.slots),
+                               dim3(256), 0, stream, a);
     }));
     check_launch();
 }

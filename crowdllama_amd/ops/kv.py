@@ -206,6 +206,15 @@ def _group(heads: int, kv_heads: int):
               "heads must share each kv head")
 
 
+def _scale(scale, dim: int) -> float:
+    if scale is None:
+        return dim ** -0.5
+    scale = float(scale)
+    if not 0 < scale < 3e38:
+        _fail(f"scale must be positive and finite, not {scale}")
+    return scale
+
+
 def _workspace(n: int, dev):
     return torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
 
@@ -284,7 +293,7 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     q: `[slots, heads, head_dim]`, of the pool's type or float32 over a
     bfloat16 pool; query heads g * i ... g * i + g - 1 share kv head i.
     mass: each place's weight is added, summed over the query heads that share
-    the kv head. scale: of the scores, head_dim ** -0.5 by default. A sequence
+    the kv head. scale: of the scores, positive, head_dim ** -0.5 by default. A sequence
     without places gives zeros.
     """
     dev, reach, kv = _pages(pool, table, False)
@@ -302,13 +311,12 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
         out = torch.empty((slots, q_heads, dim), dtype=q.dtype, device=dev)
     oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
     _apart(out, "out")
-    le = _vector(lens, "lens", slots, dev)
+    le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
                                              mass is not None), dev)
     core.kv_attend(kv, qh, oh, q_heads, _TYPES[q.dtype], le, ms, reach,
-                   dim ** -0.5 if scale is None else float(scale),
-                   ws.data_ptr(), _stream(dev))
+                   scale, ws.data_ptr(), _stream(dev))
     return out
 
 
@@ -336,13 +344,13 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
                   f"sequences, not {rows}")
         starts = torch.arange(slots + 1, dtype=torch.int32, device=dev)
     st = _vector(starts, "starts", slots + 1, dev)
-    le = _vector(lens, "lens", slots, dev)
+    le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
     core = _get(dev)
-    ws = _workspace(core.kv_observe_workspace(kv, q_heads, rows, reach), dev)
+    ws = _workspace(core.kv_observe_workspace(kv, q_heads, rows, reach,
+                                              _TYPES[q.dtype]), dev)
     core.kv_observe(kv, qh, q_heads, _TYPES[q.dtype], rows, st, le,
                     ms, reach,
-                    dim ** -0.5 if scale is None else float(scale),
-                    ws.data_ptr(), _stream(dev))
+                    scale, ws.data_ptr(), _stream(dev))
     return mass
 
 

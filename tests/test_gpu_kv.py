@@ -416,6 +416,56 @@ def test_observe_missing_pages():
     check_observe(q, pool, table, lens, [0, 60, 90], TYPES[1])
 
 
+@pytest.mark.parametrize("types", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("factor,shift", [(20., 0.), (1., -30.), (1., 30.),
+                                          (6., -12.)])
+def test_observe_far_scores(types, factor, shift):
+    """Rows whose scores are all far below or above 0, or far apart: their
+    exponentials would vanish or overflow."""
+    lens, rows = [200, 90], [70, 90]
+    _, pool, table = make(35, lens, 4, 2, 64, 16, types, strange=False)
+    q = torch.randn(160, 4, 64, generator=torch.Generator().manual_seed(2))
+    q, pool = factor * q, pool.float()
+    # one dimension of all keys and queries: adds shift * 8 * scale to each
+    q[..., 0], pool[:, :, 0, :, 0] = shift, 64.
+    check_observe(q.to(types[0]), pool.to(types[1]), table, lens,
+                  [0, 70, 160], types)
+
+
+def test_observe_nan_and_inf():
+    """A row with NaN spoils what it sees, in its kv head; a key with NaN
+    spoils every row that sees it."""
+    from crowdllama_amd.ops import kv
+    lens = [120]
+    _, pool, table = make(36, lens, 4, 2, 64, 16, TYPES[1], strange=False)
+    q = torch.randn(80, 4, 64).bfloat16()
+    args = lambda: (pool.cuda(), table.cuda(), ints(lens))  # noqa: E731
+    cap = table.shape[1] * 16
+    clean = torch.zeros(1, 2, cap, device="cuda")
+    kv.observe(q.cuda(), *args(), clean, starts=ints([0, 80]))
+    bad = q.clone()
+    bad[79, 0, 5] = math.nan                   # the last token
+    got = torch.zeros(1, 2, cap, device="cuda")
+    kv.observe(bad.cuda(), *args(), got, starts=ints([0, 80]))
+    assert got[0, 0, :120].isnan().all() and torch.equal(got[0, 1],
+                                                         clean[0, 1])
+    bad = q.clone()
+    bad[0, 3, 5] = math.inf                    # sees 41 places
+    got.zero_()
+    kv.observe(bad.cuda(), *args(), got, starts=ints([0, 80]))
+    assert got[0, 1, :41].isnan().all() and torch.equal(got[0, 0],
+                                                        clean[0, 0])
+    # rows beside it are summed relative to their maximum instead of to 0:
+    # each way is within weight_error (here below 1e-4) of the exact sum
+    assert torch.allclose(got[0, 1, 41:], clean[0, 1, 41:], rtol=2e-4)
+    at = oracle.place(table, pool.shape[0], 16, 0, 119)
+    pool[at[0], 0, 0, at[1], 3] = math.nan     # seen by the last token only
+    got.zero_()
+    kv.observe(q.cuda(), *args(), got, starts=ints([0, 80]))
+    assert got[0, 0, :120].isnan().all() and torch.equal(got[0, 1],
+                                                         clean[0, 1])
+
+
 # -------------------------------------------------------------------- evict
 
 def make_evict(seed, lens, layers, kv_heads, dim, page, dtype, cap=None):

@@ -69,6 +69,8 @@ def test_all_is_checked_before_the_device():
      "overlap"),
     (dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16, requires_grad=True)),
      "gradient"),
+    (dict(scale=0.), "positive"), (dict(scale=-1.), "positive"),
+    (dict(scale=math.nan), "positive"), (dict(scale=math.inf), "positive"),
     (dict(q=torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="meta")),
      "q is on meta"),
 ])
