@@ -518,7 +518,7 @@ def test_evict(dtype, dim, page, keep, recent):
 
 
 @pytest.mark.parametrize("n,keep", [(1024, 1000), (1025, 512), (5000, 2500),
-                                    (9000, 100)])
+                                    (9000, 100), (40000, 9999)])
 def test_evict_long(n, keep):
     lens = [n, n // 2]
     pool, table, mass, pos = make_evict(41, lens, 1, 2, 64, 64,
