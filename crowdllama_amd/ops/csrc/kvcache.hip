@@ -323,6 +323,15 @@ constexpr int UNIT = TILE * WAVES;
 // How many workgroups the whole of the batch's places are split into, about.
 constexpr int ATTEND_WGS = 512;
 
+// The lengths on the device decide how the work is split: every kv head's
+// places are cut into equally many units of 128 for each workgroup, as many
+// as make about `target` workgroups of all of them. A ragged batch's long
+// sequences get more workgroups than its short ones, and the host needs no
+// length. Workgroup `id` takes part j of n of (b, head).
+struct Part {
+    int b, head, j, n, first, lo, hi, there;
+};
+
 struct AttendArgs {
     Pages kv;
     KvHeads q, out;
@@ -334,27 +343,19 @@ struct AttendArgs {
     int64_t ld;
     float* part_o;            // [workgroup][G][D], relative to part_m
     float* part_ml;           // [workgroup][G][2]
-};
-
-// The lengths on the device decide how the work is split: every kv head's
-// places are cut into equally many units of 128 for each workgroup, as many
-// as make about `target` workgroups of all of them. A ragged batch's long
-// sequences get more workgroups than its short ones, and the host needs no
-// length. Workgroup `id` takes part j of n of (b, head).
-struct Part {
-    int b, head, j, n, len, first, lo, hi;
+    Part* parts;              // [workgroup], for the second kernel
 };
 
 __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
                                           Part& p) {
     const int lane = threadIdx.x & 63;
-    int all = 0;
-    for (int base = 0; base < a.slots; base += 64) {
-        const int b = base + lane;
-        const int len = b < a.slots
-            ? kv_clamp_len(a.lens[b] + a.add, a.reach) : 0;
-        all += (len + UNIT - 1) / UNIT;
-    }
+    auto len_of = [&](int b) {
+        return b < a.slots ? kv_clamp_len(a.lens[b] + a.add, a.reach) : 0;
+    };
+    const int len0 = len_of(lane);
+    int all = (len0 + UNIT - 1) / UNIT;
+    for (int b = 64 + lane; b - lane < a.slots; b += 64)
+        all += (len_of(b) + UNIT - 1) / UNIT;
     #pragma unroll
     for (int m = 32; m; m >>= 1) all += __shfl_xor(all, m, 64);
     const int per = max(1u, ((uint32_t)all * a.kv_heads + a.target - 1)
@@ -362,8 +363,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
     int before = 0;
     for (int base = 0; base < a.slots; base += 64) {
         const int b = base + lane;
-        const int len = b < a.slots
-            ? kv_clamp_len(a.lens[b] + a.add, a.reach) : 0;
+        const int len = base ? len_of(b) : len0;
         const int units = (len + UNIT - 1) / UNIT;
         const int n = max(1u, (uint32_t)(units + per - 1) / (uint32_t)per);
         int upto = b < a.slots ? n * a.kv_heads : 0;
@@ -375,19 +375,20 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
         const uint64_t over = __ballot(before + upto > id);
         if (over) {
             const int at = __builtin_ctzll(over);
+            const int len_b = __shfl(len, at, 64);
             p.b = base + at;
-            p.len = __shfl(len, at, 64);
             p.n = __shfl(n, at, 64);
-            const int units_b = (p.len + UNIT - 1) / UNIT;
             const int rest = id - before
                 - (__shfl(upto, at, 64) - p.n * a.kv_heads);
             p.head = rest / p.n;
-            p.j = rest % p.n;
+            p.j = rest - p.head * p.n;
             p.first = id - p.j;
             // n = ceil(units / per) parts of ceil(units / n): none is empty
-            const int each = (units_b + p.n - 1) / p.n * UNIT;
+            const int each = ((len_b + UNIT - 1) / UNIT + p.n - 1) / p.n
+                * UNIT;
             p.lo = p.j * each;
-            p.hi = min(p.lo + each, p.len);
+            p.hi = min(p.lo + each, len_b);
+            p.there = 1;
             return true;
         }
         before += __shfl(upto, 63, 64);
@@ -479,7 +480,12 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
     __shared__ float s_m[WAVES][16], s_l[WAVES][16];
     __shared__ float s_o[WAVES][16][D];
     Part p;
-    if (!find_part(a, blockIdx.x, p)) return;
+    const bool there = find_part(a, blockIdx.x, p);
+    if (threadIdx.x == 0) {
+        if (there) a.parts[blockIdx.x] = p;
+        else a.parts[blockIdx.x].there = 0;
+    }
+    if (!there) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
@@ -626,9 +632,8 @@ template <class C, bool F32OUT, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
     __shared__ float s_m[16], s_r[16];
     __shared__ float s_acc[256];
-    Part p;
-    if (!find_part(a, blockIdx.x, p)) return;
-    if (!MASS && p.n == 1) return;
+    const Part p = a.parts[blockIdx.x];
+    if (!p.there || (!MASS && p.n == 1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int G = a.q_heads / a.kv_heads;
     const float* ml = a.part_ml + (int64_t)p.first * G * 2;
@@ -652,31 +657,61 @@ __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
         if (lane == 0) { s_m[h] = ref; s_r[h] = l == 0.f ? 0.f : 1.f / l; }
     }
     __syncthreads();
+    if constexpr (MASS) {
+        // 4 places a thread, 4 heads' scores at a time
+        float* mass = reinterpret_cast<float*>(a.mass.data)
+            + p.b * a.mass.slot_stride + p.head * a.mass.head_stride;
+        const float* sc = a.scores
+            + ((int64_t)p.b * a.q_heads + p.head * G) * a.ld;
+        for (int x = p.lo + tid * 4; x < p.hi; x += 1024) {
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            for (int h = 0; h < G; h += 4) {
+                f32x4 s[4];
+                #pragma unroll
+                for (int i = 0; i < 4; i++)
+                    s[i] = *reinterpret_cast<const f32x4*>(
+                        sc + min(h + i, G - 1) * a.ld + x);
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int hi = min(h + i, G - 1);
+                    const float m = s_m[hi], r = s_r[hi];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float w = exp2_fast(s[i][e] - m) * r;
+                        sum[e] += h + i < G ? w : 0.f;
+                    }
+                }
+            }
+            #pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x + e < p.hi) mass[x + e] += sum[e];
+        }
+    }
     if (p.n > 1) {
-        // outputs [j * each, ...) of the head's G * D, `lanes` threads each
+        // `each` of the head's G * D outputs; width (a power of two) of them
+        // at a time, the parts dealt to 256 / width threads of each
         const int each = (G * D + p.n - 1) / p.n;
         const int lo = p.j * each, hi = min(lo + each, G * D);
+        int width = 8;
+        while (width < each && width < 256) width <<= 1;
+        const int y = tid / width, deal = 256 / width;
         const float* po = a.part_o + (int64_t)p.first * G * D;
-        for (int x0 = lo; x0 < hi; x0 += 8) {
-            const int x = x0 + (tid & 7), y = tid >> 3;
+        for (int x0 = lo; x0 < hi; x0 += width) {
+            const int x = x0 + (tid & (width - 1)), h = x / D;
             float acc = 0.f;
             if (x < hi) {
-                const int h = x / D;
                 const float ref = s_m[h];
-                for (int j = y; j < p.n; j += 32)
+                #pragma unroll 4
+                for (int j = y; j < p.n; j += deal)
                     acc += po[(int64_t)j * G * D + x]
                         * exp2_fast(ml[((int64_t)j * G + h) * 2] - ref);
             }
+            __syncthreads();
             s_acc[tid] = acc;
             __syncthreads();
-            #pragma unroll
-            for (int m = 128; m >= 8; m >>= 1) {
-                if (tid < m) s_acc[tid] += s_acc[tid + m];
-                __syncthreads();
-            }
-            if (tid < 8 && x < hi) {
-                const int h = x / D;
-                const float v = s_acc[tid] * s_r[h];
+            if (tid < width && x < hi) {
+                for (int i = 1; i < deal; i++) acc += s_acc[i * width + tid];
+                const float v = acc * s_r[h];
                 const int64_t at = p.b * a.out.row_stride
                     + (int64_t)(p.head * G + h) * a.out.head_stride + x % D;
                 if constexpr (F32OUT)
@@ -685,19 +720,6 @@ __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
                     reinterpret_cast<uint16_t*>(a.out.data)[at] =
                         (uint16_t)C::pack(v, 0.f);
             }
-            __syncthreads();
-        }
-    }
-    if constexpr (MASS) {
-        float* mass = reinterpret_cast<float*>(a.mass.data)
-            + p.b * a.mass.slot_stride + p.head * a.mass.head_stride;
-        const float* sc = a.scores
-            + ((int64_t)p.b * a.q_heads + p.head * G) * a.ld;
-        for (int x = p.lo + tid; x < p.hi; x += 256) {
-            float sum = 0.f;
-            for (int h = 0; h < G; h++)
-                sum += exp2_fast(sc[h * a.ld + x] - s_m[h]) * s_r[h];
-            mass[x] += sum;
         }
     }
 }
@@ -1514,7 +1536,7 @@ size_t kv_attend_workspace(const KvPages& kv, int q_heads, int reach,
     check_pages(kv, q_heads, reach);
     const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
     return aligned(wgs * G * kv.dim * 4) + aligned(wgs * G * 2 * 4)
-        + (mass ? aligned((size_t)kv.slots * q_heads * scores_ld(reach) * 4)
+        + aligned(wgs * sizeof(Part)) + (mass ? aligned((size_t)kv.slots * q_heads * scores_ld(reach) * 4)
                 : 0);
 }
 
@@ -1528,11 +1550,13 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
     char* w = reinterpret_cast<char*>(ws);
     AttendArgs a{pages_of(kv), q, out, mass, lens, add, q_heads, kv.kv_heads,
                  kv.slots, reach, ATTEND_WGS, scale * LOG2E, nullptr,
-                 scores_ld(reach), nullptr, nullptr};
+                 scores_ld(reach), nullptr, nullptr, nullptr};
     a.part_o = reinterpret_cast<float*>(w);
     w += aligned(wgs * G * kv.dim * 4);
     a.part_ml = reinterpret_cast<float*>(w);
     w += aligned(wgs * G * 2 * 4);
+    a.parts = reinterpret_cast<Part*>(w);
+    w += aligned(wgs * sizeof(Part));
     a.scores = reinterpret_cast<float*>(w);
     const dim3 grid((uint32_t)wgs), block(256);
     #define ATTEND(M)                                                         \
