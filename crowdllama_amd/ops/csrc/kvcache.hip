@@ -320,8 +320,16 @@ constexpr int TILE = 32;          // places a wave takes at a time
 constexpr int WAVES = 4;
 constexpr int UNIT = TILE * WAVES;
 
-// How many workgroups the whole of the batch's places are split into, about.
-constexpr int ATTEND_WGS = 512;
+// How many workgroups the whole of the batch's places are split into, about:
+// two a CU, which stream as fast as more and leave less to join (one sequence
+// of 131071 places: 124 us, 128 with 2048). With as many rows (sequences x kv
+// heads) as CUs most rows would stay whole, and the CUs that get long ones
+// finish late: finer parts even that out (16 x 32 rows of up to 8191 places:
+// 175 us, 212 with 512; 64 x 4 of up to 4096: 40 us, 43 with 512; but 16 x 8
+// of up to 4096: 32 us, 28 with 512).
+inline int attend_target(const KvPages& kv) {
+    return (int64_t)kv.slots * kv.kv_heads >= 256 ? 2048 : 512;
+}
 
 // The lengths on the device decide how the work is split: every kv head's
 // places are cut into equally many units of 128 for each workgroup, as many
@@ -339,7 +347,7 @@ struct AttendArgs {
     const int32_t* lens;
     int32_t add, q_heads, kv_heads, slots, reach, target;
     float scale2;             // scale * log2(e)
-    float* scores;            // [slots][q heads][ld] in units of log2
+    float* scores;            // [slots][kv heads][ld / 32][G][32], of log2
     int64_t ld;
     float* part_o;            // [workgroup][G][D], relative to part_m
     float* part_ml;           // [workgroup][G][2]
@@ -501,7 +509,8 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
     #pragma unroll
     for (int e = 0; e < EL; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     float* scores = MASS && n < G
-        ? a.scores + ((int64_t)p.b * a.q_heads + head) * a.ld : nullptr;
+        ? a.scores + ((int64_t)p.b * a.kv_heads + p.head) * G * a.ld + n * 32
+        : nullptr;
     const int64_t to_v = (int64_t)a.kv.page * D;
 
     for (int p0 = p.lo + wave * TILE; p0 < p.hi; p0 += UNIT) {
@@ -540,9 +549,11 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
             }
         }
         if (MASS && scores) {
+            // a tile's scores lie together
             #pragma unroll
             for (int u = 0; u < 2; u++)
-                *reinterpret_cast<f32x4*>(scores + p0 + u * 16 + g * 4) =
+                *reinterpret_cast<f32x4*>(scores + (int64_t)p0 * G + u * 16
+                                          + g * 4) =
                     f32x4{s[u * 4], s[u * 4 + 1], s[u * 4 + 2], s[u * 4 + 3]};
         }
         float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
@@ -662,15 +673,16 @@ __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
         float* mass = reinterpret_cast<float*>(a.mass.data)
             + p.b * a.mass.slot_stride + p.head * a.mass.head_stride;
         const float* sc = a.scores
-            + ((int64_t)p.b * a.q_heads + p.head * G) * a.ld;
+            + ((int64_t)p.b * a.kv_heads + p.head) * G * a.ld;
         for (int x = p.lo + tid * 4; x < p.hi; x += 1024) {
+            const float* at = sc + (int64_t)(x & ~31) * G + (x & 31);
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
             for (int h = 0; h < G; h += 4) {
                 f32x4 s[4];
                 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     s[i] = *reinterpret_cast<const f32x4*>(
-                        sc + min(h + i, G - 1) * a.ld + x);
+                        at + min(h + i, G - 1) * 32);
                 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int hi = min(h + i, G - 1);
@@ -1525,7 +1537,7 @@ void launch_kv_step(int32_t* len, int32_t* step, const uint8_t* active,
 namespace {
 int64_t attend_wgs(const KvPages& kv, int reach) {
     const int64_t rows = (int64_t)kv.slots * kv.kv_heads;
-    return std::min(ATTEND_WGS + rows,
+    return std::min(attend_target(kv) + rows,
                     rows * std::max(1, (reach + UNIT - 1) / UNIT));
 }
 int64_t scores_ld(int reach) { return (int64_t)(reach + 31) / 32 * 32; }
@@ -1549,7 +1561,7 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
     const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
     char* w = reinterpret_cast<char*>(ws);
     AttendArgs a{pages_of(kv), q, out, mass, lens, add, q_heads, kv.kv_heads,
-                 kv.slots, reach, ATTEND_WGS, scale * LOG2E, nullptr,
+                 kv.slots, reach, attend_target(kv), scale * LOG2E, nullptr,
                  scores_ld(reach), nullptr, nullptr, nullptr};
     a.part_o = reinterpret_cast<float*>(w);
     w += aligned(wgs * G * kv.dim * 4);

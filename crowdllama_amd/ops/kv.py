@@ -88,13 +88,39 @@ def _dense(t, name: str, n: int):
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                _fail("no operator of the cache has a gradient")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad \
+                and torch.is_grad_enabled():
+            _fail("no operator of the cache has a gradient")
 
 
 def _pages(pool, table, layers: bool):
+    """What the kernels need of the pool and the table. Most calls pass the
+    first test; what does not is looked at piece by piece."""
+    try:
+        dev = pool.device
+        ps, st = pool.shape, pool.stride()
+        p, (heads, two, page, dim) = ps[0], ps[-4:]
+        per, ts = page * dim, table.shape
+        kind, at = _TYPES[pool.dtype], pool.data_ptr()
+        if (kind and two == 2 and st[-4:] == (2 * per, per, dim, 1)
+                and len(ps) == (6 if layers else 5)
+                and not (layers and (st[1] < st[2] * heads or st[1] % 8
+                                     or st[0] < st[1] * ps[1]))
+                and st[0] >= 2 * per * heads and not (st[0] % 8 or at % 16)
+                and p and heads and page and dim
+                and table.dtype is torch.int32 and len(ts) == 2
+                and ts[0] and ts[1] and table.stride()[1] == 1
+                and table.device == dev):
+            return dev, ts[1] * page, (
+                at, st[0], p, table.data_ptr(), table.stride()[0], ts[1],
+                page, ts[0], heads, dim, kind, dev.index)
+    except (AttributeError, KeyError, ValueError, IndexError, TypeError):
+        pass
+    return _pages_slowly(pool, table, layers)
+
+
+def _pages_slowly(pool, table, layers: bool):
     if not isinstance(pool, torch.Tensor):
         _fail(f"pool must be a tensor, not {type(pool).__name__}")
     if pool.dtype not in (torch.bfloat16, torch.float16):
@@ -130,6 +156,12 @@ def _pages(pool, table, layers: bool):
 
 
 def _vector(t, name: str, n: int, dev):
+    try:
+        if (t.dtype is torch.int32 and t.shape == (n,) and t.stride() == (1,)
+                and t.device == dev):
+            return t.data_ptr()
+    except (AttributeError, TypeError):
+        pass
     _on(t, name, torch.int32, 1, dev)
     if t.shape[0] != n:
         _fail(f"{name} must have {n} values, not {t.shape[0]}")
@@ -138,6 +170,17 @@ def _vector(t, name: str, n: int, dev):
 
 
 def _heads(t, name: str, rows, heads, dim: int, dtype, dev):
+    try:
+        n, h, d = t.shape
+        s0, s1, s2 = t.stride()
+        at = t.data_ptr()
+        if (d == dim and s2 == 1 and t.dtype is dtype and t.device == dev
+                and (rows is None or n == rows)
+                and (heads is None or h == heads)
+                and not (at % 16 or s0 % 8 or s1 % 8)):
+            return at, s0, s1
+    except (AttributeError, TypeError, ValueError):
+        pass
     _on(t, name, dtype, 3, dev)
     shape = t.shape
     if ((rows is not None and shape[0] != rows)
@@ -167,12 +210,13 @@ def _apart(t, name: str):
         span = step * n
 
 
-def _meet(a, b) -> bool:
-    """Whether the memory from a's first to its last value meets b's."""
-    ends = [(t.data_ptr(), t.data_ptr() + t.element_size() * (
-        1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
-        for t in (a, b)]
-    return ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
+def _ends(t):
+    """The addresses of a tensor's memory, from its first value to its last."""
+    at = t.data_ptr()
+    if t.is_contiguous():
+        return at, at + t.element_size() * t.numel()
+    return at, at + t.element_size() * (
+        1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
 def _same(a, b) -> bool:
@@ -180,6 +224,13 @@ def _same(a, b) -> bool:
 
 
 def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
+    try:
+        if (t.shape[:-1] == lead and 0 < t.shape[-1] <= reach
+                and t.dtype is dtype and t.is_contiguous()
+                and t.device == dev):
+            return (t.data_ptr(), *t.stride()[:-1])
+    except (AttributeError, TypeError):
+        pass
     _on(t, name, dtype, len(lead) + 1, dev)
     if tuple(t.shape[:-1]) != lead:
         _fail(f"{name} must be {list(lead)} x places, not {list(t.shape)}")
@@ -219,7 +270,13 @@ def _workspace(n: int, dev):
     return torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
 
 
+# the stream's handle without an object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
@@ -257,8 +314,10 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         if q_out is None:
             q_out = torch.empty((rows, q_heads, dim), dtype=q.dtype,
                                 device=dev)
-        qo = _heads(q_out, "q_out", rows, q_heads, dim, k.dtype, dev)
-        _apart(q_out, "q_out")
+            qo = (q_out.data_ptr(), q_heads * dim, dim)
+        else:
+            qo = _heads(q_out, "q_out", rows, q_heads, dim, k.dtype, dev)
+            _apart(q_out, "q_out")
     elif q_out is not None:
         _fail("q_out without q")
     if starts is None and rows != slots:
@@ -309,8 +368,10 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
         reach = mass.shape[-1]
     if out is None:
         out = torch.empty((slots, q_heads, dim), dtype=q.dtype, device=dev)
-    oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
-    _apart(out, "out")
+        oh = (out.data_ptr(), q_heads * dim, dim)
+    else:
+        oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
+        _apart(out, "out")
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
@@ -398,10 +459,12 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     lo = _vector(lens_out, "out's lens", slots, dev)
     if mass_out.shape[-1] != reach or pos_out.shape[-1] != reach:
         _fail("out's mass and pos must have as many places as mass")
-    for new in (mass_out, pos_out, lens_out):
-        for old, same in ((mass, mass_out), (pos, pos_out), (lens, lens_out),
-                          (next_pos, None)):
-            if _meet(new, old) and not (new is same and _same(new, old)):
+    olds = [(t, *_ends(t)) for t in (mass, pos, lens, next_pos)]
+    for i, new in enumerate((mass_out, pos_out, lens_out)):
+        lo_, hi_ = _ends(new)
+        for j, (old, first, last) in enumerate(olds):
+            if lo_ < last and first < hi_ and not (
+                    i == j and (new is old or _same(new, old))):
                 _fail("each of out must be the tensor that it replaces, or "
                       "apart from all of them")
     core = _get(dev)
