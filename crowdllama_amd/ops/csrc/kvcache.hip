@@ -1036,10 +1036,12 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
     const Seq s = sequence_at(a, blockIdx.z);
-    // late chunks are seen by more places than early ones: turned from block
-    // to block, so that no XCD (every eighth workgroup) gets the late ones
+    // late chunks are seen by more places than early ones, in steps with the
+    // blocks: turned by an arbitrary amount from block to block, so that no
+    // XCD (every eighth workgroup) gets the late ones
     const int block = blockIdx.x / a.chunks;
-    const int chunk = (blockIdx.x + block) % a.chunks;
+    const int chunk = (blockIdx.x + ((uint32_t)block * 0x9E3779B1u >> 24))
+        % a.chunks;
     const int first = block * OBS_PLACES, p0 = first + wave * 16 * PW;
     const int R = s.m * G;
     // rows from the first that sees the block's first place on
