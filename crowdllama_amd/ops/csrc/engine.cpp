@@ -595,12 +595,15 @@ void Engine::alloc_state() {
         kv_mass_ = (float*)dalloc(rows * cfg_.max_seq * 4);
         kv_pos_ = (int32_t*)dalloc(rows * cfg_.max_seq * 4);
         const KvPages all = kv_pages(0), one = kv_pages(0, 0);
-        kv_ws_ = dalloc(std::max(
-            {kv_attend_workspace(all, NH, cfg_.max_seq, true),
-             kv_observe_workspace(one, NH, cfg_.prefill_chunk, cfg_.max_seq,
-                                  KVT::F32),
-             kv_evict_workspace(all, meta_.layers, cfg_.kv_keep,
-                                cfg_.max_seq)}));
+        size_t ws = std::max(
+            kv_attend_workspace(all, NH, cfg_.max_seq, true),
+            kv_evict_workspace(all, meta_.layers, cfg_.kv_keep,
+                               cfg_.max_seq));
+        // a shorter chunk may be cut finer and need more
+        for (int m = 1; m <= cfg_.prefill_chunk; m++)
+            ws = std::max(ws, kv_observe_workspace(one, NH, m, cfg_.max_seq,
+                                                   KVT::F32));
+        kv_ws_ = dalloc(ws);
     }
     {   // i8-GEMM activation-quant scratch, sized for the widest input of
         // any projection at the bigger of decode batch / prefill chunk

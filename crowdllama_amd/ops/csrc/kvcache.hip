@@ -150,6 +150,12 @@ void check_scale(float scale) {
         throw std::runtime_error("scale must be positive and finite");
 }
 
+// a grid's threads must be fewer than 2^32
+void check_grid(int64_t workgroups) {
+    if (workgroups >= 1ll << 24)
+        throw std::runtime_error("too many rows or sequences in one call");
+}
+
 void check_launch() {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess)
@@ -1430,15 +1436,15 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
     }
 }
 
-// Pass 2, grid (blocks of moves, rows): the movers' keys and values, 16
+// Pass 2, grid (rows, blocks of moves): the movers' keys and values, 16
 // lanes a row. Sources are at or above keep and destinations below it, so
 // no order is needed.
 __global__ __launch_bounds__(256) void k_kv_evict_move(EvictArgs a, int dim) {
-    const int row = blockIdx.y;
+    const int row = blockIdx.x;
     const int h = row % a.kv_heads, b = row / a.kv_heads % a.slots,
               layer = row / a.kv_heads / a.slots;
     const int count = a.count[row];
-    if (blockIdx.x == 0 && h == 0 && layer == 0 && threadIdx.x == 0)
+    if (blockIdx.y == 0 && h == 0 && layer == 0 && threadIdx.x == 0)
         a.lens_out[b] = count < 0 ? a.lens[b] : a.keep;
     const int32_t* table = a.kv.table + (int64_t)b * a.kv.table_stride;
     const int l16 = threadIdx.x & 15;
@@ -1452,8 +1458,8 @@ __global__ __launch_bounds__(256) void k_kv_evict_move(EvictArgs a, int dim) {
             + (int64_t)(p % a.kv.page) * dim;
     };
     const int64_t to_v = (int64_t)a.kv.page * dim;
-    for (int i = blockIdx.x * 16 + (threadIdx.x >> 4); i < count;
-         i += gridDim.x * 16) {
+    for (int i = blockIdx.y * 16 + (threadIdx.x >> 4); i < count;
+         i += gridDim.y * 16) {
         const uint16_t* s = where(a.src[(int64_t)row * a.most + i]);
         uint16_t* d = where(a.dst[(int64_t)row * a.most + i]);
         if (!s || !d || l16 * 8 >= dim) continue;
@@ -1507,6 +1513,7 @@ void launch_kv_append(const KvPages& kv, const KvHeads& k, const KvHeads& v,
     if (rows <= 0) return;
     if (!starts && rows != kv.slots)
         throw std::runtime_error("append: one row for each sequence");
+    check_grid(rows);
     AppendArgs a{pages_of(kv), k, v, q, q_out, mass, pos, starts, lens,
                  next_pos, inv_freq, q.data ? q_heads : 0, kv.kv_heads,
                  kv.slots, reach};
@@ -1561,6 +1568,7 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
     check_pages(kv, q_heads, reach);
     check_scale(scale);
     const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
+    check_grid(wgs);
     char* w = reinterpret_cast<char*>(ws);
     AttendArgs a{pages_of(kv), q, out, mass, lens, add, q_heads, kv.kv_heads,
                  kv.slots, reach, attend_target(kv), scale * LOG2E, nullptr,
@@ -1643,6 +1651,9 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
     const ObserveCut c = observe_cut(kv, q_heads, rows, reach, type);
     if (c.parts > 65535 || kv.kv_heads > 65535 || kv.slots > 65535)
         throw std::runtime_error("observe: too many sequences or kv heads");
+    check_grid(c.blocks);
+    check_grid(c.place_blocks * c.chunks);
+    check_grid((int64_t)rows * q_heads / 256 + 1);
     char* w = reinterpret_cast<char*>(ws);
     ObserveArgs a{pages_of(kv), q, mass, starts, lens, q_heads, kv.kv_heads,
                   kv.slots, rows, reach, scale * LOG2E,
@@ -1692,9 +1703,9 @@ void launch_kv_evict(const KvPages& kv, int layers, int64_t layer_stride,
                      int reach, void* ws, hipStream_t stream) {
     check_pages(kv, 0, reach);
     const int64_t rows = (int64_t)layers * kv.slots * kv.kv_heads;
-    if (layers < 1 || rows > 65535)
-        throw std::runtime_error("evict: 1 to 65535 rows (layers x sequences "
-                                 "x kv heads)");
+    if (layers < 1 || rows >= 1 << 22)
+        throw std::runtime_error("evict: 1 to 2^22 - 1 rows (layers x "
+                                 "sequences x kv heads)");
     if (keep < 1 || recent < 0 || limit < keep)
         throw std::runtime_error("evict: keep >= 1, recent >= 0 and "
                                  "limit >= keep");
@@ -1716,7 +1727,8 @@ void launch_kv_evict(const KvPages& kv, int layers, int64_t layer_stride,
     else
         hipLaunchKernelGGL(k_kv_evict_select<0>, grid, block, 0, stream, a);
     hipLaunchKernelGGL(k_kv_evict_move,
-                       dim3(std::max(1, (most + 63) / 64), (uint32_t)rows),
+                       dim3((uint32_t)rows,
+                            std::min(65535, std::max(1, (most + 63) / 64))),
                        dim3(256), 0, stream, a, kv.dim);
     check_launch();
 }

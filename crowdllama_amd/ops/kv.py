@@ -302,7 +302,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(k, pool.dtype)
-    _no_grad(k, v, q)
+    _no_grad(k, v, q, pool, mass)
     rows = k.shape[0] if k.dim() else 0
     kh = _heads(k, "k", None, heads, dim, k.dtype, dev)
     vh = _heads(v, "v", rows, heads, dim, k.dtype, dev)
@@ -358,7 +358,7 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(q, pool.dtype)
-    _no_grad(q)
+    _no_grad(q, pool, mass)
     qh = _heads(q, "q", slots, None, dim, q.dtype, dev)
     q_heads = q.shape[1]
     _group(q_heads, heads)
@@ -393,7 +393,7 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(q, pool.dtype)
-    _no_grad(q)
+    _no_grad(q, pool, mass)
     qh = _heads(q, "q", None, None, dim, q.dtype, dev)
     rows, q_heads = q.shape[0], q.shape[1]
     _group(q_heads, heads)
@@ -424,11 +424,13 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     pool: `[pages, layers, kv_heads, 2, page, head_dim]`; mass, pos:
     `[layers, slots, kv_heads, places]`. Places with a pos of at least
     `next_pos[b] - recent` stay before all others, the others by mass; among
-    equals the lower place stays. Survivors below place `keep` stay where they
-    are; the free places there take the others, both in order. What lies at
-    and above `keep` afterwards is left as it was.
+    equals the lower place stays, and a NaN counts as less than any number.
+    Survivors below place `keep` stay where they are; the free places there
+    take the others, both in order. What lies at and above `keep` afterwards is
+    left as it was.
 
-    Keys and values move within the pool. mass, pos and lens are changed in
+    Keys and values move within the pool, so a page must not serve two places
+    of the table. mass, pos and lens are changed in
     place, or, with `out=(mass, pos, lens)`, written there whole while these
     stay as they were.
     """
@@ -442,13 +444,14 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     if max(keep, recent, limit) >= 1 << 31:
         _fail("keep, recent and limit must be below 2^31")
     lead = (layers, slots, heads)
+    _no_grad(pool, mass)
     ms = _places(mass, "mass", torch.float32, lead, reach, dev)
     ps = _places(pos, "pos", torch.int32, lead, reach, dev)
     reach = mass.shape[-1]
     if pos.shape[-1] != reach:
         _fail("mass and pos must have equally many places")
-    if layers * slots * heads > 65535:
-        _fail("layers x sequences x kv heads must be at most 65535")
+    if layers * slots * heads >= 1 << 22:
+        _fail("layers x sequences x kv heads must be below 2^22")
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
     if out is None:

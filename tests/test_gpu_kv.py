@@ -526,6 +526,28 @@ def test_evict_long(n, keep):
     check_evict(pool, table, lens, lens, mass, pos, keep, keep // 3, None)
 
 
+def test_evict_many_rows():
+    """More rows than a grid's second dimension holds."""
+    from crowdllama_amd.ops import kv
+    g = torch.Generator(device="cuda").manual_seed(0)
+    B, heads = 2200, 32
+    pool = torch.randn(B, 1, heads, 2, 16, 64, device="cuda").bfloat16()
+    table = torch.randperm(B, generator=g, device="cuda").int().view(B, 1)
+    mass = torch.rand(1, B, heads, 16, generator=g, device="cuda")
+    pos = torch.arange(16, dtype=torch.int32, device="cuda").expand(
+        1, B, heads, 16).contiguous()
+    lens = torch.full((B,), 16, dtype=torch.int32, device="cuda")
+    old, weight = pool.clone(), mass.clone()
+    kv.evict(pool, table, lens, lens.clone(), mass, pos, keep=6)
+    assert (lens == 6).all()
+    stay = weight.topk(6, -1)[1].sort(-1)[0]
+    assert torch.equal(pos[..., :6].long().sort(-1)[0], stay)
+    assert torch.equal(mass[..., :6], weight.gather(-1, pos[..., :6].long()))
+    rows = old[table[:, 0].long(), 0].gather(3, pos[0, :, :, None, :6, None]
+                                            .long().expand(-1, -1, 2, -1, 64))
+    assert torch.equal(pool[table[:, 0].long(), 0, :, :, :6], rows)
+
+
 def test_evict_ties_and_strange_masses():
     lens = [64]
     pool, table, mass, pos = make_evict(42, lens, 1, 4, 64, 16,

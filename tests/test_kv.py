@@ -138,8 +138,9 @@ def evict_args(**kw):
     (dict(out=(torch.zeros(3, 2, 2, 60),
                torch.zeros(3, 2, 2, 64, dtype=torch.int32), ints(0, 0))),
      "as many places"),
-    (dict(table=torch.zeros(22000, 1, dtype=torch.int32),
-          mass=torch.zeros(1).expand(3, 22000, 2, 1)), "overlap"),
+    (dict(mass=torch.zeros(1).expand(3, 2, 2, 64)), "contiguous"),
+    (dict(mass=torch.zeros(3, 2, 1, 64).expand(3, 2, 2, 64)), "overlap"),
+    (dict(mass=torch.zeros(3, 2, 2, 64, requires_grad=True)), "gradient"),
 ])
 def test_evict_refuses(kw, match):
     refused(kv.evict, evict_args(**kw), match)
@@ -174,6 +175,18 @@ def test_sizes_that_the_kernels_do_not_take(kw, reach, match):
     core = get_core()
     with pytest.raises(RuntimeError, match=match):
         core.kv_attend_workspace(pages_arg(**kw), 1, reach, True)
+
+
+def test_a_chunk_needs_no_more_than_the_most():
+    """The workspace of fewer rows may be larger (they are cut finer): the
+    engine takes the most over all chunks."""
+    core = get_core()
+    page = pages_arg(max_pages=8192, heads=8, dim=128)
+    need = [core.kv_observe_workspace(page, 32, m, 131072, 0)
+            for m in range(1, 1025)]
+    assert all(n > 0 for n in need) and max(need) < 64 << 20
+    with pytest.raises(RuntimeError, match="too many rows"):
+        core.kv_observe_workspace(page, 32, 1 << 27, 131072, 0)
 
 
 def test_pages_outside_the_pool_are_not_followed():
