@@ -183,6 +183,13 @@ __device__ __forceinline__ float wave_xor_sum(float x, int mask) {
     return x + __shfl_xor(x, mask, 64);
 }
 
+// x is there from here on: a loaded operand that a loop uses first is
+// otherwise waited for in the loop, along with the loop's own loads that
+// should still be on their way.
+__device__ __forceinline__ void arrive(u32x4& x) {
+    asm volatile("" : "+v"(x));
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
     return __builtin_amdgcn_exp2f(x);
 }
@@ -875,6 +882,12 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(Observe
                          there, g, q[w]);
         seen[w] = there ? s.len - s.m + i + 1 : 0;
     }
+    #pragma unroll
+    for (int w = 0; w < RW; w++)
+        #pragma unroll
+        for (int x = 0; x < NQ; x++)
+            #pragma unroll
+            for (int kk = 0; kk < D / 32; kk++) arrive(q[w][x][kk]);
 
     u32x4 next[PER];
     bool next_there;
@@ -1174,6 +1187,10 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     };
     fetch(begin);
     stage(0);
+    #pragma unroll
+    for (int u = 0; u < PW; u++)
+        #pragma unroll
+        for (int kk = 0; kk < D / 32; kk++) arrive(k[u][kk]);
     __syncthreads();
     int buf = 0;
     for (int r0 = begin; r0 < end; r0 += QT, buf ^= 1) {
