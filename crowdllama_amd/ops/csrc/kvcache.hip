@@ -1248,6 +1248,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_add(ObserveArgs a) {
         + ((int64_t)s.b * a.kv_heads + head) * a.ld + p;
     const int64_t step = (int64_t)a.slots * a.kv_heads * a.ld;
     float w = 0.f;
+    #pragma unroll 8
     for (int c = from / a.chunk; c <= (R - 1) / a.chunk; c++)
         w += part[c * step];
     reinterpret_cast<float*>(a.mass.data)[
@@ -1612,10 +1613,15 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
 
 namespace {
 
-// How the two passes of observe are cut: into at least OBSERVE_WGS
-// workgroups where there is the work for that, since a pass that has fewer
-// waits for its longest ones (causal rows and places are uneven).
-constexpr int OBSERVE_WGS = 4096;
+// How the two passes of observe are cut: into workgroups of OBSERVE_TILES
+// tiles (64 x 256 scores of a kv head) at least, but 512 and no more than 4096
+// of them: a pass with fewer waits for its longest ones (causal rows and
+// places are uneven), one with more begins too often.
+constexpr int OBSERVE_TILES_1 = 8, OBSERVE_TILES_2 = 8;
+
+inline int64_t observe_wgs(int64_t tiles, int per) {
+    return std::min<int64_t>(4096, std::max<int64_t>(512, tiles / per));
+}
 
 struct ObserveCut {
     int64_t blocks, parts, part, chunks, chunk, place_blocks;
@@ -1632,13 +1638,16 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     ObserveCut c;
     c.blocks = up(R, per) + kv.slots - 1;
     const int64_t places = std::max(reach, 1);
-    c.parts = std::min(up(OBSERVE_WGS, c.blocks * kv.kv_heads),
-                       up(places, 512));
+    const int64_t row_blocks = c.blocks * kv.kv_heads;
+    c.parts = std::min(
+        up(observe_wgs(row_blocks * up(places, 64), OBSERVE_TILES_1),
+           row_blocks), up(places, 512));
     c.part = up(up(places, c.parts), 64) * 64;
     c.parts = up(places, c.part);
     c.place_blocks = up(places, OBS_PLACES);
-    c.chunks = std::min(
-        up(OBSERVE_WGS, c.place_blocks * kv.kv_heads * kv.slots), up(R, 128));
+    const int64_t blocks = c.place_blocks * kv.kv_heads * kv.slots;
+    c.chunks = std::min(up(observe_wgs(blocks * up(R, 64), OBSERVE_TILES_2),
+                           blocks), up(R, 128));
     c.chunk = up(up(R, c.chunks), 64) * 64;
     c.chunks = up(R, c.chunk);
     c.sums = c.parts > 1 ? aligned((size_t)c.parts * rows * q_heads * 8) : 0;

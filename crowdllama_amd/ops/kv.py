@@ -88,10 +88,10 @@ def _dense(t, name: str, n: int):
 
 
 def _no_grad(*tensors):
-    for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad \
-                and torch.is_grad_enabled():
-            _fail("no operator of the cache has a gradient")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail("no operator of the cache has a gradient")
 
 
 def _pages(pool, table, layers: bool):
@@ -266,8 +266,8 @@ def _scale(scale, dim: int) -> float:
     return scale
 
 
-def _workspace(n: int, dev):
-    return torch.empty(max(n, 1), dtype=torch.uint8, device=dev)
+def _workspace(n: int, table):
+    return table.new_empty(n // 4 + 1)
 
 
 # the stream's handle without an object around it
@@ -302,7 +302,6 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(k, pool.dtype)
-    _no_grad(k, v, q, pool, mass)
     rows = k.shape[0] if k.dim() else 0
     kh = _heads(k, "k", None, heads, dim, k.dtype, dev)
     vh = _heads(v, "v", rows, heads, dim, k.dtype, dev)
@@ -312,8 +311,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         qh = _heads(q, "q", rows, None, dim, k.dtype, dev)
         q_heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((rows, q_heads, dim), dtype=q.dtype,
-                                device=dev)
+            q_out = q.new_empty((rows, q_heads, dim))
             qo = (q_out.data_ptr(), q_heads * dim, dim)
         else:
             qo = _heads(q_out, "q_out", rows, q_heads, dim, k.dtype, dev)
@@ -340,6 +338,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         reach = min(reach, pos.shape[-1])
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
+    _no_grad(k, v, q, pool, mass)
     _get(dev).kv_append(kv, kh, vh, qh, qo, q_heads, _TYPES[k.dtype], rows,
                         st, le, np, fr, ms, ps, reach, _stream(dev))
     return q_out
@@ -358,7 +357,6 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(q, pool.dtype)
-    _no_grad(q, pool, mass)
     qh = _heads(q, "q", slots, None, dim, q.dtype, dev)
     q_heads = q.shape[1]
     _group(q_heads, heads)
@@ -367,15 +365,16 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
         ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
         reach = mass.shape[-1]
     if out is None:
-        out = torch.empty((slots, q_heads, dim), dtype=q.dtype, device=dev)
+        out = q.new_empty((slots, q_heads, dim))
         oh = (out.data_ptr(), q_heads * dim, dim)
     else:
         oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
         _apart(out, "out")
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
+    _no_grad(q, pool, mass)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
-                                             mass is not None), dev)
+                                             mass is not None), table)
     core.kv_attend(kv, qh, oh, q_heads, _TYPES[q.dtype], le, ms, reach,
                    scale, ws.data_ptr(), _stream(dev))
     return out
@@ -393,7 +392,6 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
     _queries(q, pool.dtype)
-    _no_grad(q, pool, mass)
     qh = _heads(q, "q", None, None, dim, q.dtype, dev)
     rows, q_heads = q.shape[0], q.shape[1]
     _group(q_heads, heads)
@@ -406,9 +404,10 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
         starts = torch.arange(slots + 1, dtype=torch.int32, device=dev)
     st = _vector(starts, "starts", slots + 1, dev)
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
+    _no_grad(q, pool, mass)
     core = _get(dev)
     ws = _workspace(core.kv_observe_workspace(kv, q_heads, rows, reach,
-                                              _TYPES[q.dtype]), dev)
+                                              _TYPES[q.dtype]), table)
     core.kv_observe(kv, qh, q_heads, _TYPES[q.dtype], rows, st, le,
                     ms, reach,
                     scale, ws.data_ptr(), _stream(dev))
@@ -444,7 +443,6 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     if max(keep, recent, limit) >= 1 << 31:
         _fail("keep, recent and limit must be below 2^31")
     lead = (layers, slots, heads)
-    _no_grad(pool, mass)
     ms = _places(mass, "mass", torch.float32, lead, reach, dev)
     ps = _places(pos, "pos", torch.int32, lead, reach, dev)
     reach = mass.shape[-1]
@@ -462,6 +460,7 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     lo = _vector(lens_out, "out's lens", slots, dev)
     if mass_out.shape[-1] != reach or pos_out.shape[-1] != reach:
         _fail("out's mass and pos must have as many places as mass")
+    _no_grad(pool, mass)
     olds = [(t, *_ends(t)) for t in (mass, pos, lens, next_pos)]
     for i, new in enumerate((mass_out, pos_out, lens_out)):
         lo_, hi_ = _ends(new)
@@ -471,7 +470,7 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
                 _fail("each of out must be the tensor that it replaces, or "
                       "apart from all of them")
     core = _get(dev)
-    ws = _workspace(core.kv_evict_workspace(kv, layers, keep, reach), dev)
+    ws = _workspace(core.kv_evict_workspace(kv, layers, keep, reach), table)
     core.kv_evict(kv, layers, pool.stride(1), le, lo, np,
                   ms, ps, mo, po, keep, recent, limit, reach, ws.data_ptr(), _stream(dev))
     return mass_out, pos_out, lens_out
