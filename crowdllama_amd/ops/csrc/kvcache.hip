@@ -246,6 +246,8 @@ __device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
 // by side), 8 elements a thread and pass; the row's angles are shared by all
 // heads through LDS. position * inv_freq is taken and reduced in 64 bits: in
 // 32 it would be off by 2^-24 of the angle, 0.06 rad at position 10^6.
+// Bound by memory: 8632 rows of 32 + 16 heads of 128 (177 MB) take 30 us, 5.9
+// TB/s; few rows by latency (3.6 us).
 template <KVT T, KVT C, int D>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     __shared__ float cs[D / 2], sn[D / 2];
@@ -493,8 +495,12 @@ __device__ __forceinline__ void load_tile(const uint16_t* r0,
 // and V needs no transposition through LDS: a lane holds 8 places x EL
 // elements, and product e takes element e of each (MFMA row r is d = r*EL+e).
 //
-// Bound by the reads of K and V. Its scores go out as they are where a mass
-// is wanted, since the weights are known only once all parts are.
+// Bound by the reads of K and V: one sequence of 131071 places of 8 kv heads of
+// 128 (537 MB) takes 95 us without a mass, 5.6 TB/s, as fast as a stream that
+// is only read. Its scores go out as they are where a mass is wanted, since the
+// weights are known only once all parts are; those 17 MB cost another 15 us.
+// The products take a third of that (three pieces), so loading a tile ahead
+// gains nothing (119 us for 112).
 template <class C, int NQ, int NP, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
     constexpr int EL = D / 16;
@@ -651,7 +657,8 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
 
 // Join the parts: the same workgroups once more. Each makes its share of the
 // head's outputs (the parts' sums, in their order) and, from the scores, the
-// weights of its own places.
+// weights of its own places. Latency and the scores' 17 MB: 10.8 us for the
+// sequence above, 5 us for one of 601 places.
 template <class C, bool F32OUT, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
     __shared__ float s_m[16], s_r[16];
@@ -822,6 +829,10 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 // queries stay in registers, over the part's places, which the workgroup
 // stages 64 at a time. Each lane keeps a sum (and a maximum, where it needs
 // one) of its own for each of its columns; they meet at the end.
+//
+// A score costs a multiplication, an exponential and an addition: 16 + 32 + 16
+// cycles of the SIMD for 4 x 64 of them, beside 64 of matrix products, which
+// run at the same time in part. 375 us for 8192 rows of 32 heads (137 GFLOP).
 //
 // Three waves a SIMD for one piece (375 us for 8192 rows of 32 heads, 442 with
 // two), two for three (249 us for 3 x 500 rows over 16000 places, 290 with
@@ -1040,7 +1051,8 @@ __global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
 // Pass 2, grid (place blocks x chunks, kv heads, slots): 16 * PW places a
 // wave, whose keys stay in registers, over the chunk's rows, which the
 // workgroup stages QT at a time; a lane sums its columns' weights for its
-// places. Where the rows are one chunk the sums go to the mass, else to
+// places. The same work a score as in pass 1, 410 us for 8192 rows of 32 heads
+// at two waves a SIMD (the keys, sums and staged queries need 190 registers). Where the rows are one chunk the sums go to the mass, else to
 // `partial`, and the last kernel adds them in order.
 template <class C, int NQ, int D, int PW>
 __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
@@ -1456,7 +1468,8 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
 
 // Pass 2, grid (rows, blocks of moves): the movers' keys and values, 16
 // lanes a row. Sources are at or above keep and destinations below it, so
-// no order is needed.
+// no order is needed. 2048 places of 256 rows (537 MB read and written) take
+// 100 us, the rate of a large copy.
 __global__ __launch_bounds__(256) void k_kv_evict_move(EvictArgs a, int dim) {
     const int row = blockIdx.x;
     const int h = row % a.kv_heads, b = row / a.kv_heads % a.slots,
