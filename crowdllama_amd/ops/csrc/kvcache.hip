@@ -771,7 +771,13 @@ Div div_by(int d) {
             d > 1 ? (uint32_t)((0xFFFFFFFFull + (uint32_t)d) / d) : 0u};
 }
 
-constexpr int OBS_PLACES = 256;   // places of a workgroup of the second pass
+// Groups of 16 places that a wave of the second pass holds. Three leave room
+// for a third wave a SIMD with heads of 128 and one piece (8192 rows of 32
+// heads: 344 us, 422 with four); more pieces have more to do for each row that
+// is read (3 x 500 rows over 16000 places: 307 us, 355 with three).
+constexpr int obs_groups(bool one_piece, int dim) {
+    return one_piece && dim == 128 ? 3 : 4;
+}
 
 struct ObserveArgs {
     Pages kv;
@@ -783,8 +789,9 @@ struct ObserveArgs {
     Div group;
     // first pass: places in parts of `part`, of which there are `parts`
     int32_t part, parts;
-    // second pass: rows in chunks of `chunk`, of which there are `chunks`
-    int32_t chunk, chunks;
+    // second pass: rows in chunks of `chunk`, of which there are `chunks`, and
+    // places in blocks of `block`
+    int32_t chunk, chunks, block;
     float* sums;       // [parts][kv heads][rows][G][2]: maximum, sum
     float* lse;        // [kv heads][rows][G]: log2 of the sum of 2^scores
     float* partial;    // [chunks][slots][kv heads][ld]
@@ -923,8 +930,8 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(Observe
         if (lane == 0) s_there[buf][wave] = next_there;
     };
     // 32 places (the tile's half `half`) against the wave's rows. CUT: some
-    // row does not see them all, or a page is missing. MAX: relative to a
-    // running maximum, else to 0.
+    // row does not see them all, or (t0, t1) 16 of them have no page. MAX:
+    // relative to a running maximum, else to 0.
     auto half_tile = [&](int buf, int half, int pu, bool t0, bool t1,
                          auto CUT, auto MAX) {
         u32x4 k[2][D / 32];
@@ -968,7 +975,8 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(Observe
                 + ((e[4] + e[5]) + (e[6] + e[7]));
         }
     };
-    auto pass = [&](auto MAX) {
+    auto pass = [&](auto MAX_) {
+        constexpr bool MAX = MAX_;
         #pragma unroll
         for (int w = 0; w < RW; w++) {
             m[w] = MAX ? -INFINITY : 0.f;
@@ -986,29 +994,40 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(Observe
             #pragma unroll
             for (int half = 0; half < 2; half++) {
                 const int pu = p0 + half * 32;
-                const bool t0 = s_there[buf][half * 2];
-                const bool t1 = s_there[buf][half * 2 + 1];
-                if (t0 && t1 && pu + 32 <= least)
-                    half_tile(buf, half, pu, t0, t1, False{}, MAX);
-                else if (t0 || t1)
-                    half_tile(buf, half, pu, t0, t1, True{}, MAX);
+                if constexpr (MAX) {
+                    const bool t0 = s_there[buf][half * 2];
+                    const bool t1 = s_there[buf][half * 2 + 1];
+                    if (t0 || t1)
+                        half_tile(buf, half, pu, t0, t1, True{}, MAX_);
+                } else if (pu + 32 <= least) {
+                    half_tile(buf, half, pu, true, true, False{}, MAX_);
+                } else {
+                    half_tile(buf, half, pu, true, true, True{}, MAX_);
+                }
             }
             if (more) stage(buf ^ 1);
             __syncthreads();
         }
     };
     // Exponentials relative to 0 need no maximum, and are as exact where
-    // they neither overflow nor vanish; where some row's might have, the
-    // workgroup starts over with one.
-    pass(False{});
+    // they neither overflow nor vanish; where some row's might have, or where
+    // a page is missing, the workgroup goes the general way.
     bool odd = false;
-    #pragma unroll
-    for (int w = 0; w < RW; w++) {
-        const float sum = wave_xor_sum(wave_xor_sum(l[w], 16), 32);
-        odd |= begin < min(end, seen[w]) &&
-            !(sum > 0x1p-60f && sum < 0x1p120f);
+    for (int p = begin + tid * 16; p < end; p += 256 * 16)
+        odd |= !a.kv.rows16(s.b, p, head, D);
+    if (!__syncthreads_or(odd)) {
+        pass(False{});
+        #pragma unroll
+        for (int w = 0; w < RW; w++) {
+            const float sum = wave_xor_sum(wave_xor_sum(l[w], 16), 32);
+            odd |= begin < min(end, seen[w]) &&
+                !(sum > 0x1p-60f && sum < 0x1p120f);
+        }
+        odd = __syncthreads_or(odd);
+    } else {
+        odd = true;
     }
-    if (__syncthreads_or(odd)) pass(True{});
+    if (odd) pass(True{});
     #pragma unroll
     for (int w = 0; w < RW; w++) {
         const float top = wave_xor_max(wave_xor_max(m[w], 16), 32);
@@ -1051,14 +1070,12 @@ __global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
 // Pass 2, grid (place blocks x chunks, kv heads, slots): 16 * PW places a
 // wave, whose keys stay in registers, over the chunk's rows, which the
 // workgroup stages QT at a time; a lane sums its columns' weights for its
-// places. The same work a score as in pass 1, 410 us for 8192 rows of 32 heads
-// at two waves a SIMD (the keys, sums and staged queries need 190 registers). Where the rows are one chunk the sums go to the mass, else to
+// places. The same work a score as in pass 1. Where the rows are one chunk the sums go to the mass, else to
 // `partial`, and the last kernel adds them in order.
 template <class C, int NQ, int D, int PW>
 __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     constexpr int QT = NQ == 1 ? 64 : 32, UNITS = QT * D / 8;
     constexpr int PER = (UNITS + 255) / 256;
-    static_assert(16 * PW * WAVES == OBS_PLACES, "places of a workgroup");
     __shared__ __align__(16) uint16_t s_q[2][NQ][QT * LDS_ROW<D>];
     __shared__ float s_lse[2][QT];
     __shared__ int s_seen[2][QT];
@@ -1073,7 +1090,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int block = blockIdx.x / a.chunks;
     const int chunk = (blockIdx.x + ((uint32_t)block * 0x9E3779B1u >> 24))
         % a.chunks;
-    const int first = block * OBS_PLACES, p0 = first + wave * 16 * PW;
+    const int first = block * 16 * PW * WAVES, p0 = first + wave * 16 * PW;
     const int R = s.m * G;
     // rows from the first that sees the block's first place on
     const int from = max(0, first - (s.len - s.m)) * G;
@@ -1219,11 +1236,13 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
                                            kk * 4 + g);
             const float lse = s_lse[buf][t * 16 + n];
             const int seen = s_seen[buf][t * 16 + n];
-            // rows past the last see 0 places
-            if (__any(p0 + 16 * PW > seen))
-                rows16(q, lse, seen, True{});
-            else
+            // the first of 16 rows sees the least; rows past the last see none
+            const int r = r0 + t * 16;
+            if (r + 16 <= R &&
+                p0 + 16 * PW <= s.len - s.m + a.group.of(r) + 1)
                 rows16(q, lse, seen, False{});
+            else
+                rows16(q, lse, seen, True{});
         }
         if (more) stage(buf ^ 1);
         __syncthreads();
@@ -1254,7 +1273,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_add(ObserveArgs a) {
     const Seq s = sequence_at(a, blockIdx.z);
     const int G = a.group.d, R = s.m * G;
     if (p >= s.len || R == 0) return;
-    const int from = max(0, p / OBS_PLACES * OBS_PLACES - (s.len - s.m)) * G;
+    const int from = max(0, p / a.block * a.block - (s.len - s.m)) * G;
     if (from >= R) return;
     const float* part = a.partial
         + ((int64_t)s.b * a.kv_heads + head) * a.ld + p;
@@ -1637,7 +1656,7 @@ inline int64_t observe_wgs(int64_t tiles, int per) {
 }
 
 struct ObserveCut {
-    int64_t blocks, parts, part, chunks, chunk, place_blocks;
+    int64_t blocks, parts, part, chunks, chunk, block, place_blocks;
     int64_t sums, lse, partial;     // bytes
 };
 
@@ -1657,7 +1676,8 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
            row_blocks), up(places, 512));
     c.part = up(up(places, c.parts), 64) * 64;
     c.parts = up(places, c.part);
-    c.place_blocks = up(places, OBS_PLACES);
+    c.block = 16 * WAVES * obs_groups(type != KVT::F32, kv.dim);
+    c.place_blocks = up(places, c.block);
     const int64_t blocks = c.place_blocks * kv.kv_heads * kv.slots;
     c.chunks = std::min(up(observe_wgs(blocks * up(R, 64), OBSERVE_TILES_2),
                            blocks), up(R, 128));
@@ -1667,7 +1687,7 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     c.lse = aligned((size_t)std::max(rows, 1) * q_heads * 4);
     c.partial = c.chunks > 1
         ? aligned((size_t)c.chunks * kv.slots * kv.kv_heads
-                  * c.place_blocks * OBS_PLACES * 4) : 0;
+                  * c.place_blocks * c.block * 4) : 0;
     return c;
 }
 
@@ -1698,10 +1718,11 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                   kv.slots, rows, reach, scale * LOG2E,
                   div_by(q_heads / kv.kv_heads), (int32_t)c.part,
                   (int32_t)c.parts, (int32_t)c.chunk, (int32_t)c.chunks,
+                  (int32_t)c.block,
                   reinterpret_cast<float*>(w),
                   reinterpret_cast<float*>(w + c.sums),
                   reinterpret_cast<float*>(w + c.sums + c.lse),
-                  c.place_blocks * OBS_PLACES};
+                  c.place_blocks * c.block};
     KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
         constexpr int RW = NQ > 1 ? 2 : 4;
         hipLaunchKernelGGL((k_kv_observe_sums<C, NQ, D, RW>),
@@ -1714,13 +1735,13 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                                                / 256)),
                                dim3(256), 0, stream, a);
         hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D,
-                                              OBS_PLACES / 16 / WAVES>),
+                                              obs_groups(NQ == 1, D)>),
                            dim3((uint32_t)(c.place_blocks * c.chunks),
                                 kv.kv_heads, kv.slots),
                            dim3(256), 0, stream, a);
         if (c.chunks > 1)
             hipLaunchKernelGGL(k_kv_observe_add,
-                               dim3((uint32_t)c.place_blocks, kv.kv_heads,
+                               dim3((reach + 255) / 256, kv.kv_heads,
                                     kv.slots),
                                dim3(256), 0, stream, a);
     }));
