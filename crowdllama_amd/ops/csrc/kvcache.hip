@@ -845,7 +845,8 @@ __device__ __forceinline__ float row_lse(float m, float l) {
 // two), two for three (249 us for 3 x 500 rows over 16000 places, 290 with
 // three waves, which spill).
 template <class C, int NQ, int D, int RW>
-__global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(ObserveArgs a) {
+__global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
+    ObserveArgs a) {
     constexpr int ROWS = 16 * RW * WAVES, KT = 64, PER = 16 * D / 8 / 64;
     __shared__ __align__(16) uint16_t s_k[2][KT * LDS_ROW<D>];
     __shared__ int s_there[2][4];
@@ -1042,7 +1043,8 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(Observe
             } else {
                 float* d = a.sums + ((int64_t)blockIdx.z * a.q_heads * a.rows
                                      + at) * 2;
-                d[0] = top;
+                // a part without a weight must not set the others' reference
+                d[0] = sum == 0.f ? -INFINITY : top;
                 d[1] = sum;
             }
         }

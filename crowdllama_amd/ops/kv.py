@@ -39,24 +39,28 @@ _NONE = (0, 0, 0)
 _core = None
 
 
+def _one_runtime() -> None:
+    """torch brings its own HIP runtime, which the native module takes too if
+    it is there first; streams and memory of one are nothing to another."""
+    with open("/proc/self/maps") as f:
+        found = {line.split(None, 5)[5].strip() for line in f
+                 if "libamdhip64" in line}
+    if len(found) > 1:
+        raise RuntimeError(
+            "two HIP runtimes are loaded (%s): import torch before the first "
+            "use of crowdllama_amd's native module"
+            % ", ".join(sorted(found)))
+
+
 def _get(dev):
-    """The native module, in a process with one HIP runtime."""
+    """The native module, once all arguments are checked."""
     global _core
     if dev.type != "cuda":
         _fail(f"pool must be on a GPU, not on {dev}")
     if _core is None:
         from . import get_core
         core = get_core()
-        # torch brings its own HIP runtime, which the extension takes too if
-        # it is there first; streams and memory of one are nothing to another
-        with open("/proc/self/maps") as f:
-            found = {line.split(None, 5)[5].strip() for line in f
-                     if "libamdhip64" in line}
-        if len(found) > 1:
-            raise RuntimeError(
-                "two HIP runtimes are loaded (%s): import torch before the "
-                "first use of crowdllama_amd's native module"
-                % ", ".join(sorted(found)))
+        _one_runtime()
         _core = core
     return _core
 

@@ -432,6 +432,20 @@ def test_observe_far_scores(types, factor, shift):
                   [0, 70, 160], types)
 
 
+@pytest.mark.parametrize("types", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("shift", [-30., 30.])
+def test_observe_far_scores_in_parts(types, shift):
+    """The same over several parts of the places, the later of which most rows
+    do not see at all."""
+    lens, rows = [1700, 600], [1700, 10]
+    _, pool, table = make(37, lens, 2, 1, 64, 64, types, strange=False)
+    q = torch.randn(1710, 2, 64, generator=torch.Generator().manual_seed(2))
+    pool = pool.float()
+    q[..., 0], pool[:, :, 0, :, 0] = shift, 64.
+    check_observe(q.to(types[0]), pool.to(types[1]), table, lens,
+                  [0, 1700, 1710], types)
+
+
 def test_observe_nan_and_inf():
     """A row with NaN spoils what it sees, in its kv head; a key with NaN
     spoils every row that sees it."""

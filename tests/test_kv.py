@@ -189,6 +189,27 @@ def test_a_chunk_needs_no_more_than_the_most():
         core.kv_observe_workspace(page, 32, 1 << 27, 131072, 0)
 
 
+@pytest.mark.parametrize("first,then", [
+    ("import torch", "from crowdllama_amd.ops import get_core; get_core()"),
+    ("from crowdllama_amd.ops import get_core; get_core()", "import torch")])
+def test_one_hip_runtime(first, then):
+    """torch's runtime serves both if it is loaded first; otherwise the
+    operators would be handed streams of another runtime, and refuse."""
+    import subprocess
+    import sys
+    code = (f"{first}\n{then}\nfrom crowdllama_amd.ops import kv\n"
+            "try:\n    kv._one_runtime()\n    print('one')\n"
+            "except RuntimeError as e:\n    print(str(e)[:16])\n"
+            "print(sum('libamdhip64' in x and x.split()[2] == '00000000'\n"
+            "          for x in open('/proc/self/maps')))")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True,
+                         text=True, timeout=120, check=True).stdout.split("\n")
+    # where the system's and torch's libraries are one file, both orders work
+    assert out[0] == ("one" if out[1] == "1" else "two HIP runtimes")
+    if first == "import torch":
+        assert out[0] == "one"
+
+
 def test_pages_outside_the_pool_are_not_followed():
     find = get_core().test_kv_page_of
     row = [3, -1, 5, 4, 2 ** 31 - 1, -2 ** 31]
