@@ -832,6 +832,47 @@ __device__ __forceinline__ float row_lse(float m, float l) {
     return l == 0.f ? INFINITY : m + __log2f(l);
 }
 
+// Which sequence's block of ROWS rows workgroup x has, and which of them: a
+// sequence's last rows, which see the most, go first. -1: there is no such.
+template <int ROWS>
+__device__ __forceinline__ int row_block(const ObserveArgs& a, Seq& s) {
+    const int lane = threadIdx.x & 63;
+    for (int base = 0, before = 0; base < a.slots; base += 64) {
+        const int b = base + lane;
+        int upto = 0;
+        if (b < a.slots)
+            upto = (sequence_at(a, b).m * (int)a.group.d + ROWS - 1) / ROWS;
+        #pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int x = __shfl_up(upto, m, 64);
+            if (lane >= m) upto += x;
+        }
+        const uint64_t over = __ballot(before + upto > (int)blockIdx.x);
+        if (over) {
+            const int at = __builtin_ctzll(over);
+            s = sequence_at(a, base + at);
+            return before + __shfl(upto, at, 64) - 1 - blockIdx.x;
+        }
+        before += __shfl(upto, 63, 64);
+    }
+    return -1;
+}
+
+// A row's sum over a part of the places, to where it belongs.
+__device__ __forceinline__ void store_sum(const ObserveArgs& a, const Seq& s,
+                                          int head, int r, float top,
+                                          float sum) {
+    const int64_t at = ((int64_t)head * a.rows + s.t0) * a.group.d + r;
+    if (a.parts == 1) {
+        a.lse[at] = row_lse(top, sum);
+    } else {
+        float* d = a.sums + ((int64_t)blockIdx.z * a.q_heads * a.rows + at) * 2;
+        // a part without a weight must not set the others' reference
+        d[0] = sum == 0.f ? -INFINITY : top;
+        d[1] = sum;
+    }
+}
+
 // Pass 1, grid (row blocks, kv heads, parts): 16 * RW rows a wave, whose
 // queries stay in registers, over the part's places, which the workgroup
 // stages 64 at a time. Each lane keeps a sum (and a maximum, where it needs
@@ -854,32 +895,8 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
-    // which sequence's block this is; a sequence's last rows, which see the
-    // most, go first
-    int id = -1;
     Seq s{};
-    for (int base = 0, before = 0; base < a.slots; base += 64) {
-        const int b = base + lane;
-        int blocks = 0;
-        if (b < a.slots) {
-            const Seq x = sequence_at(a, b);
-            blocks = (x.m * G + ROWS - 1) / ROWS;
-        }
-        int upto = blocks;
-        #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int x = __shfl_up(upto, m, 64);
-            if (lane >= m) upto += x;
-        }
-        const uint64_t over = __ballot(before + upto > (int)blockIdx.x);
-        if (over) {
-            const int at = __builtin_ctzll(over);
-            s = sequence_at(a, base + at);
-            id = before + __shfl(upto, at, 64) - 1 - blockIdx.x;
-            break;
-        }
-        before += __shfl(upto, 63, 64);
-    }
+    const int id = row_block<ROWS>(a, s);
     if (id < 0) return;
     const int R = s.m * G;
     const int r0 = id * ROWS + wave * 16 * RW;
@@ -1036,36 +1053,134 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
         float sum = l[w] * exp2_fast(m[w] - ref);
         sum = wave_xor_sum(wave_xor_sum(sum, 16), 32);
         const int r = r0 + w * 16 + n;
-        if (g == 0 && r < R) {
-            const int64_t at = ((int64_t)head * a.rows + s.t0) * G + r;
-            if (a.parts == 1) {
-                a.lse[at] = row_lse(top, sum);
-            } else {
-                float* d = a.sums + ((int64_t)blockIdx.z * a.q_heads * a.rows
-                                     + at) * 2;
-                // a part without a weight must not set the others' reference
-                d[0] = sum == 0.f ? -INFINITY : top;
-                d[1] = sum;
-            }
-        }
+        if (g == 0 && r < R) store_sum(a, s, head, r, top, sum);
     }
 }
 
-// Join the parts of the rows' sums. Which parts there are goes by the row's
-// workgroup in pass 1, but a part that its row does not see gave (-inf, 0).
+// Pass 1 for few rows, grid as above: 16 * RW rows a workgroup, whose four
+// waves take 32 places each in turn, with keys that go straight to registers.
+// Bound by the reads of the keys.
+template <class C, int NQ, int D, int RW>
+__global__ __launch_bounds__(256) void k_kv_observe_few(ObserveArgs a) {
+    constexpr int ROWS = 16 * RW;
+    __shared__ float s_m[WAVES][ROWS], s_l[WAVES][ROWS];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
+    const int G = a.group.d;
+    Seq s{};
+    const int id = row_block<ROWS>(a, s);
+    if (id < 0) return;
+    const int R = s.m * G, r0 = id * ROWS;
+    const int most = s.len - s.m + a.group.of(min(r0 + ROWS, R) - 1) + 1;
+    const int least = s.len - s.m + a.group.of(r0) + 1;
+    const int begin = blockIdx.z * a.part, end = min(begin + a.part, most);
+
+    u32x4 q[RW][NQ][D / 32];
+    float m[RW], l[RW];
+    int seen[RW];
+    #pragma unroll
+    for (int w = 0; w < RW; w++) {
+        const int r = r0 + w * 16 + n, i = a.group.of(r), h = r - i * G;
+        load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
+                             + (int64_t)(head * G + h) * a.q.head_stride,
+                         r < R, g, q[w]);
+        seen[w] = r < R ? s.len - s.m + i + 1 : 0;
+        m[w] = -INFINITY;
+        l[w] = 0.f;
+    }
+    for (int p0 = begin + wave * TILE; p0 < end; p0 += UNIT) {
+        const uint16_t* rows[2];
+        rows[0] = a.kv.rows16(s.b, p0, head, D);
+        rows[1] = p0 + 16 < end ? a.kv.rows16(s.b, p0 + 16, head, D)
+                                : nullptr;
+        u32x4 k[2][D / 32];
+        #pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint16_t* kp = (rows[u] ? rows[u] : a.kv.pool) + n * D
+                + g * 8;
+            #pragma unroll
+            for (int kk = 0; kk < D / 32; kk++)
+                k[u][kk] = *reinterpret_cast<const u32x4*>(kp + kk * 32);
+        }
+        const bool whole = rows[0] && rows[1] && p0 + TILE <= least;
+        #pragma unroll
+        for (int w = 0; w < RW; w++) {
+            f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            #pragma unroll
+            for (int x = NQ - 1; x >= 0; x--)
+                #pragma unroll
+                for (int kk = 0; kk < D / 32; kk++)
+                    #pragma unroll
+                    for (int u = 0; u < 2; u++)
+                        acc[u] = C::mfma(k[u][kk], q[w][x][kk], acc[u]);
+            float e[8], top = m[w];
+            #pragma unroll
+            for (int j = 0; j < 8; j++) {
+                e[j] = acc[j >> 2][j & 3] * a.scale2;
+                if (!whole && (!rows[j >> 2] ||
+                        p0 + (j >> 2) * 16 + g * 4 + (j & 3) >= seen[w]))
+                    e[j] = -INFINITY;
+                top = fmaxf(top, e[j]);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+            l[w] *= exp2_fast(m[w] - ref);
+            m[w] = top;
+            #pragma unroll
+            for (int j = 0; j < 8; j++) l[w] += exp2_fast(e[j] - ref);
+        }
+    }
+    #pragma unroll
+    for (int w = 0; w < RW; w++) {
+        const float top = wave_xor_max(wave_xor_max(m[w], 16), 32);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = l[w] * exp2_fast(m[w] - ref);
+        sum = wave_xor_sum(wave_xor_sum(sum, 16), 32);
+        if (g == 0) {
+            s_m[wave][w * 16 + n] = top;
+            s_l[wave][w * 16 + n] = sum;
+        }
+    }
+    __syncthreads();
+    if (tid < ROWS && r0 + tid < R) {
+        float top = -INFINITY, sum = 0.f;
+        #pragma unroll
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, s_m[w][tid]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        #pragma unroll
+        for (int w = 0; w < WAVES; w++)
+            sum += s_l[w][tid] * exp2_fast(s_m[w][tid] - ref);
+        store_sum(a, s, head, r0 + tid, top, sum);
+    }
+}
+
+// Join the parts of the rows' sums: 32 rows a workgroup, the parts dealt to 8
+// threads of each. A part that its row does not see gave (-inf, 0).
 __global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    __shared__ float s_m[8][32], s_l[8][32];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const int64_t at = (int64_t)blockIdx.x * 32 + x;
     const int64_t all = (int64_t)a.q_heads * a.rows;
-    if (at >= all) return;
     float m = -INFINITY, l = 0.f;
-    for (int p = 0; p < a.parts; p++) {
-        const float mp = a.sums[(p * all + at) * 2];
-        const float lp = a.sums[(p * all + at) * 2 + 1];
+    auto join = [&](float mp, float lp) {
         const float now = fmaxf(m, mp);
         const float ref = now == -INFINITY ? 0.f : now;
         l = l * exp2_fast(m - ref) + lp * exp2_fast(mp - ref);
         m = now;
+    };
+    if (at < all) {
+        #pragma unroll 4
+        for (int p = y; p < a.parts; p += 8) {
+            const f32x2 s = *reinterpret_cast<const f32x2*>(
+                a.sums + (p * all + at) * 2);
+            join(s.x, s.y);
+        }
     }
+    s_m[y][x] = m;
+    s_l[y][x] = l;
+    __syncthreads();
+    if (y || at >= all) return;
+    for (int i = 1; i < 8; i++) join(s_m[i][x], s_l[i][x]);
     a.lse[at] = row_lse(m, l);
 }
 
@@ -1229,6 +1344,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
         if (more) fetch(r0 + QT);
         #pragma unroll
         for (int t = 0; t < QT / 16; t++) {
+            const int r = r0 + t * 16;
             u32x4 q[NQ][D / 32];
             #pragma unroll
             for (int x = 0; x < NQ; x++)
@@ -1239,7 +1355,6 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
             const float lse = s_lse[buf][t * 16 + n];
             const int seen = s_seen[buf][t * 16 + n];
             // the first of 16 rows sees the least; rows past the last see none
-            const int r = r0 + t * 16;
             if (r + 16 <= R &&
                 p0 + 16 * PW <= s.len - s.m + a.group.of(r) + 1)
                 rows16(q, lse, seen, False{});
@@ -1305,12 +1420,13 @@ __device__ __forceinline__ int64_t row_at(const KvLayers& t, int layer, int b,
     return layer * t.layer_stride + b * t.slot_stride + h * t.head_stride;
 }
 
-// Who moves: the places of a row go by in blocks of 1024, in order, one place
-// a thread. Sums over the workgroup's 16 waves, in their order.
+// Who moves: the places of a row go by in blocks of one place a thread, in
+// order. Sums over the workgroup's NW waves, in theirs.
 struct WaveSums {
     uint32_t before, all;
 };
 
+template <int NW>
 __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
                                               int wave) {
     __syncthreads();
@@ -1318,7 +1434,7 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
     __syncthreads();
     WaveSums s{0, 0};
     #pragma unroll
-    for (int w = 0; w < 16; w++) {
+    for (int w = 0; w < NW; w++) {
         const uint32_t y = red[w];
         if (w < wave) s.before += y;
         s.all += y;
@@ -1326,20 +1442,23 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
     return s;
 }
 
-// Pass 1, one workgroup of 1024 a row (layer, sequence, kv head): which
-// places stay, and who moves where. A thread holds the keys of KPT places
-// (place = k * 1024 + thread), or, with KPT = 0, computes them each time it
+// Pass 1, one workgroup of NT a row (layer, sequence, kv head): which places
+// stay, and who moves where. A thread holds the keys of KPT places
+// (place = k * NT + thread), or, with KPT = 0, computes them each time it
 // goes through the row. The keep-th largest key is found two bits at a time,
 // counting the keys at or above three candidates with ballots; it ends early
 // once exactly `keep` keys are at or above one. Then one walk in the order of
 // places numbers the free ones and those that come into them.
 //
-// KPT 8 serves rows of up to 8192 places (256 rows of 8192: 33 us, 42 with
-// KPT 32, 60 with 0), 32 up to 32768 (of 20000: 67 us, 185 with 0).
-template <int KPT>
-__global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
-    __shared__ uint32_t red[2][3][16];
-    __shared__ uint32_t tot[16];
+// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 33 us, 42
+// with KPT 32, 60 with 0), 32 up to 32768 (of 20000: 67 us, 185 with 0).
+// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 24 us, 98 with 1024
+// threads).
+template <int NT, int KPT>
+__global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
+    constexpr int NW = NT / 64;
+    __shared__ uint32_t red[2][3][NW];
+    __shared__ uint32_t tot[NW];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row = blockIdx.x;
@@ -1367,7 +1486,7 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
     if constexpr (KPT > 0) {
         #pragma unroll
         for (int k = 0; k < KPT; k++) {
-            const int p = k * 1024 + tid;
+            const int p = k * NT + tid;
             held[k] = 0;
             if (p < a.reach && (p < len || copies || copied)) {
                 const float m = mass[p];
@@ -1378,13 +1497,13 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
             }
         }
     } else {
-        for (int p = tid; p < a.reach; p += 1024) {
+        for (int p = tid; p < a.reach; p += NT) {
             if (copies) mass_out[p] = mass[p];
             if (copied) pos_out[p] = pos[p];
         }
     }
     if (!full) return;
-    const int blocks = (len + 1023) / 1024;
+    const int blocks = (len + NT - 1) / NT;
 
     // keys past the end are 0 and `least` is at least 1 where it decides:
     // a candidate always has a bit set
@@ -1404,7 +1523,7 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
             for (int k = 0; k < KPT; k++)
                 if (k < blocks) count(held[k]);
         } else {
-            for (int base = 0; base < len; base += 1024)
+            for (int base = 0; base < len; base += NT)
                 count(base + tid < len ? key_at(base + tid) : 0);
         }
         if (lane == 0) {
@@ -1415,7 +1534,7 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
         __syncthreads();
         n1 = n2 = n3 = 0;
         #pragma unroll
-        for (int w = 0; w < 16; w++) {
+        for (int w = 0; w < NW; w++) {
             n1 += red[turn][0][w];
             n2 += red[turn][1][w];
             n3 += red[turn][2][w];
@@ -1436,11 +1555,11 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
             for (int k = 0; k < KPT; k++)
                 if (k < blocks) above += __popcll(__ballot(held[k] > least));
         } else {
-            for (int base = 0; base < len; base += 1024)
+            for (int base = 0; base < len; base += NT)
                 above += __popcll(__ballot(base + tid < len &&
                                            key_at(base + tid) > least));
         }
-        ties = a.keep - wave_sums(above, tot, wave).all;
+        ties = a.keep - wave_sums<NW>(above, tot, wave).all;
     }
 
     int32_t* dst = a.dst + (int64_t)row * a.most;
@@ -1453,16 +1572,16 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
         bool stays = here && key >= least;
         if (!exact) {
             const uint64_t eqs = __ballot(here && key == least);
-            const WaveSums s = wave_sums(__popcll(eqs), tot, wave);
+            const WaveSums s = wave_sums<NW>(__popcll(eqs), tot, wave);
             if (here && key == least)
                 stays = equal + s.before + __popcll(eqs & below) < ties;
             equal += s.all;
         }
-        // both counts in one word: a block has at most 1024 of each
+        // both counts in one word: a block has at most NT of each
         const uint64_t fs = __ballot(here && p < a.keep && !stays);
         const uint64_t cs = __ballot(stays && p >= a.keep);
         const WaveSums s =
-            wave_sums(__popcll(fs) | __popcll(cs) << 16, tot, wave);
+            wave_sums<NW>(__popcll(fs) | __popcll(cs) << 16, tot, wave);
         if (here && p < a.keep && !stays)
             dst[free + (s.before & 0xFFFF) + __popcll(fs & below)] = p;
         if (stays && p >= a.keep)
@@ -1473,14 +1592,14 @@ __global__ __launch_bounds__(1024) void k_kv_evict_select(EvictArgs a) {
     if constexpr (KPT > 0) {
         #pragma unroll
         for (int k = 0; k < KPT; k++)
-            if (k < blocks) walk(k * 1024, held[k]);
+            if (k < blocks) walk(k * NT, held[k]);
     } else {
-        for (int base = 0; base < len; base += 1024)
+        for (int base = 0; base < len; base += NT)
             walk(base, base + tid < len ? key_at(base + tid) : 0);
     }
     if (tid == 0) a.count[row] = come;
     __syncthreads();
-    for (uint32_t i = tid; i < come; i += 1024) {
+    for (uint32_t i = tid; i < come; i += NT) {
         const int d = dst[i], s = src[i];
         mass_out[d] = mass[s];
         pos_out[d] = pos[s];
@@ -1662,12 +1781,23 @@ struct ObserveCut {
     int64_t sums, lse, partial;     // bytes
 };
 
+// Rows of a workgroup of the first pass in its form for few rows, by the rows
+// that a sequence has on average; 0: the other form. (4 rows of 8 sequences of
+// up to 3867 places, 32 kv heads: 27 us, 69 in the other form; 16 x 4 rows over
+// 131071 places, 8 kv heads: 56 us, 79.)
+int64_t observe_few(const KvPages& kv, int q_heads, int rows, KVT type) {
+    const int64_t R = (int64_t)rows * (q_heads / kv.kv_heads);
+    const int64_t most = type == KVT::F32 ? 32 : 64;   // what registers hold
+    return R <= 16ll * kv.slots ? 16 : R <= most * kv.slots ? most : 0;
+}
+
 ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
                        KVT type) {
     if ((int64_t)rows * (q_heads / kv.kv_heads) >= (1ll << 28))
         throw std::runtime_error("observe: too many rows");
     const int64_t G = q_heads / kv.kv_heads, R = std::max<int64_t>(rows, 1) * G;
-    const int64_t per = 16 * WAVES * (type == KVT::F32 ? 2 : 4);
+    const int64_t few = observe_few(kv, q_heads, rows, type);
+    const int64_t per = few ? few : 16 * WAVES * (type == KVT::F32 ? 2 : 4);
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     ObserveCut c;
     c.blocks = up(R, per) + kv.slots - 1;
@@ -1714,7 +1844,7 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
         throw std::runtime_error("observe: too many sequences or kv heads");
     check_grid(c.blocks);
     check_grid(c.place_blocks * c.chunks);
-    check_grid((int64_t)rows * q_heads / 256 + 1);
+    check_grid((int64_t)rows * q_heads / 32 + 1);
     char* w = reinterpret_cast<char*>(ws);
     ObserveArgs a{pages_of(kv), q, mass, starts, lens, q_heads, kv.kv_heads,
                   kv.slots, rows, reach, scale * LOG2E,
@@ -1726,18 +1856,20 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                   reinterpret_cast<float*>(w + c.sums + c.lse),
                   c.place_blocks * c.block};
     KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
-        constexpr int RW = NQ > 1 ? 2 : 4;
-        hipLaunchKernelGGL((k_kv_observe_sums<C, NQ, D, RW>),
-                           dim3((uint32_t)c.blocks, kv.kv_heads,
-                                (uint32_t)c.parts),
+        constexpr int RW = NQ > 1 ? 2 : 4, PW = obs_groups(NQ == 1, D);
+        const int64_t few = observe_few(kv, q_heads, rows, type);
+        auto* sums = few == 16 ? k_kv_observe_few<C, NQ, D, 1>
+            : few ? k_kv_observe_few<C, NQ, D, RW>
+                  : k_kv_observe_sums<C, NQ, D, RW>;
+        hipLaunchKernelGGL(sums, dim3((uint32_t)c.blocks, kv.kv_heads,
+                                      (uint32_t)c.parts),
                            dim3(256), 0, stream, a);
         if (c.parts > 1)
             hipLaunchKernelGGL(k_kv_observe_join,
-                               dim3((uint32_t)(((int64_t)rows * q_heads + 255)
-                                               / 256)),
+                               dim3((uint32_t)(((int64_t)rows * q_heads + 31)
+                                               / 32)),
                                dim3(256), 0, stream, a);
-        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D,
-                                              obs_groups(NQ == 1, D)>),
+        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D, PW>),
                            dim3((uint32_t)(c.place_blocks * c.chunks),
                                 kv.kv_heads, kv.slots),
                            dim3(256), 0, stream, a);
@@ -1782,12 +1914,18 @@ void launch_kv_evict(const KvPages& kv, int layers, int64_t layer_stride,
     w += aligned((size_t)rows * most * 4 + 4);
     a.src = reinterpret_cast<int32_t*>(w);
     const dim3 grid((uint32_t)rows), block(1024);
-    if (reach <= 8 * 1024)
-        hipLaunchKernelGGL(k_kv_evict_select<8>, grid, block, 0, stream, a);
+    if (reach <= 8 * 256)
+        hipLaunchKernelGGL((k_kv_evict_select<256, 8>), grid, dim3(256), 0,
+                           stream, a);
+    else if (reach <= 8 * 1024)
+        hipLaunchKernelGGL((k_kv_evict_select<1024, 8>), grid, block, 0,
+                           stream, a);
     else if (reach <= 32 * 1024)
-        hipLaunchKernelGGL(k_kv_evict_select<32>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_kv_evict_select<1024, 32>), grid, block, 0,
+                           stream, a);
     else
-        hipLaunchKernelGGL(k_kv_evict_select<0>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL((k_kv_evict_select<1024, 0>), grid, block, 0,
+                           stream, a);
     hipLaunchKernelGGL(k_kv_evict_move,
                        dim3((uint32_t)rows,
                             std::min(65535, std::max(1, (most + 63) / 64))),

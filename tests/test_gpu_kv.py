@@ -384,6 +384,22 @@ def test_observe_as_attend():
 
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("long_,n", [(1, 1), (9, 700), (70, 2100)])
+def test_observe_few_rows(types, dim, long_, n):
+    """Few rows a sequence on average: one may have many more."""
+    lens, rows = [n] + [5, 0, 1500, 33, 40, 7, 8], [long_, 1, 0, 3, 2, 2, 1, 8]
+    _, pool, table = make(38, lens, 4, 2, dim, 32, types,
+                          strange=n < 1000)
+    table[4, 0] = -1
+    q = torch.randn(sum(rows), 4, dim,
+                    generator=torch.Generator().manual_seed(2)).to(types[0])
+    q[long_:] *= 8                       # and scores far from 0
+    check_observe(q, pool, table, lens,
+                  [sum(rows[:b]) for b in range(9)], types)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
 def test_observe_longer(types):
     lens = [1500, 777]
     rows = [1030, 777]
