@@ -789,12 +789,12 @@ struct ObserveArgs {
     Div group;
     // first pass: places in parts of `part`, of which there are `parts`
     int32_t part, parts;
-    // second pass: rows in chunks of `chunk`, of which there are `chunks`, and
-    // places in blocks of `block`
+    // second pass: a sequence's rows in chunks of `chunk`, at most `chunks` in
+    // the batch, and places in blocks of `block`
     int32_t chunk, chunks, block;
     float* sums;       // [parts][kv heads][rows][G][2]: maximum, sum
     float* lse;        // [kv heads][rows][G]: log2 of the sum of 2^scores
-    float* partial;    // [chunks][slots][kv heads][ld]
+    float* partial;    // [chunks][kv heads][ld]
     int64_t ld;
 };
 
@@ -832,30 +832,49 @@ __device__ __forceinline__ float row_lse(float m, float l) {
     return l == 0.f ? INFINITY : m + __log2f(l);
 }
 
-// Which sequence's block of ROWS rows workgroup x has, and which of them: a
-// sequence's last rows, which see the most, go first. -1: there is no such.
-template <int ROWS>
-__device__ __forceinline__ int row_block(const ObserveArgs& a, Seq& s) {
+// The x-th block of `rows` rows, counted over the batch: which sequence's it
+// is, which of its blocks, and of how many. -1: there is no such.
+struct RowBlock {
+    int id, all;
+};
+
+__device__ __forceinline__ RowBlock row_block(const ObserveArgs& a, int rows,
+                                              int at_x, Seq& s) {
+    if (a.slots == 1) {
+        s = sequence_at(a, 0);
+        const int all = (s.m * (int)a.group.d + rows - 1) / rows;
+        return {at_x < all ? at_x : -1, all};
+    }
     const int lane = threadIdx.x & 63;
     for (int base = 0, before = 0; base < a.slots; base += 64) {
-        const int b = base + lane;
-        int upto = 0;
-        if (b < a.slots)
-            upto = (sequence_at(a, b).m * (int)a.group.d + ROWS - 1) / ROWS;
+        const int b = min(base + lane, a.slots - 1);
+        const Seq own = sequence_at(a, b);
+        const int all = base + lane < a.slots
+            ? (own.m * (int)a.group.d + rows - 1) / rows : 0;
+        int upto = all;
         #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
             const int x = __shfl_up(upto, m, 64);
             if (lane >= m) upto += x;
         }
-        const uint64_t over = __ballot(before + upto > (int)blockIdx.x);
+        const uint64_t over = __ballot(before + upto > at_x);
         if (over) {
+            // scalars, as all that follows from them
             const int at = __builtin_ctzll(over);
-            s = sequence_at(a, base + at);
-            return before + __shfl(upto, at, 64) - 1 - blockIdx.x;
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+            s = {base + at, of(own.t0), of(own.m), of(own.len)};
+            return {at_x - before - of(upto) + of(all), of(all)};
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return -1;
+    return {-1, 0};
+}
+
+// The first pass's: a sequence's last rows, which see the most, go first.
+template <int ROWS>
+__device__ __forceinline__ int late_block(const ObserveArgs& a, Seq& s) {
+    const RowBlock x = row_block(a, ROWS, blockIdx.x, s);
+    return x.id < 0 ? -1 : x.all - 1 - x.id;
 }
 
 // A row's sum over a part of the places, to where it belongs.
@@ -896,7 +915,7 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
     Seq s{};
-    const int id = row_block<ROWS>(a, s);
+    const int id = late_block<ROWS>(a, s);
     if (id < 0) return;
     const int R = s.m * G;
     const int r0 = id * ROWS + wave * 16 * RW;
@@ -1069,7 +1088,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_few(ObserveArgs a) {
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
     Seq s{};
-    const int id = row_block<ROWS>(a, s);
+    const int id = late_block<ROWS>(a, s);
     if (id < 0) return;
     const int R = s.m * G, r0 = id * ROWS;
     const int most = s.len - s.m + a.group.of(min(r0 + ROWS, R) - 1) + 1;
@@ -1184,11 +1203,12 @@ __global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
     a.lse[at] = row_lse(m, l);
 }
 
-// Pass 2, grid (place blocks x chunks, kv heads, slots): 16 * PW places a
+// Pass 2, grid (place blocks x chunks, kv heads): 16 * PW places a
 // wave, whose keys stay in registers, over the chunk's rows, which the
 // workgroup stages QT at a time; a lane sums its columns' weights for its
-// places. The same work a score as in pass 1. Where the rows are one chunk the sums go to the mass, else to
-// `partial`, and the last kernel adds them in order.
+// places. The same work a score as in pass 1. Where a sequence's rows are one
+// chunk the sums go to the mass, else to `partial`, and the last kernel adds
+// them in order.
 template <class C, int NQ, int D, int PW>
 __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     constexpr int QT = NQ == 1 ? 64 : 32, UNITS = QT * D / 8;
@@ -1200,13 +1220,16 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
-    const Seq s = sequence_at(a, blockIdx.z);
     // late chunks are seen by more places than early ones, in steps with the
     // blocks: turned by an arbitrary amount from block to block, so that no
     // XCD (every eighth workgroup) gets the late ones
     const int block = blockIdx.x / a.chunks;
-    const int chunk = (blockIdx.x + ((uint32_t)block * 0x9E3779B1u >> 24))
+    const int at = (blockIdx.x + ((uint32_t)block * 0x9E3779B1u >> 24))
         % a.chunks;
+    Seq s{};
+    const RowBlock x = row_block(a, a.chunk, at, s);
+    if (x.id < 0) return;
+    const int chunk = x.id;
     const int first = block * 16 * PW * WAVES, p0 = first + wave * 16 * PW;
     const int R = s.m * G;
     // rows from the first that sees the block's first place on
@@ -1364,11 +1387,10 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
         if (more) stage(buf ^ 1);
         __syncthreads();
     }
-    float* to = a.chunks == 1
+    float* to = x.all == 1
         ? reinterpret_cast<float*>(a.mass.data) + s.b * a.mass.slot_stride
             + head * a.mass.head_stride
-        : a.partial + (((int64_t)chunk * a.slots + s.b) * a.kv_heads + head)
-            * a.ld;
+        : a.partial + ((int64_t)at * a.kv_heads + head) * a.ld;
     #pragma unroll
     for (int u = 0; u < PW; u++)
         #pragma unroll
@@ -1378,27 +1400,35 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
             for (int x = 1; x < 16; x <<= 1) w = wave_xor_sum(w, x);
             const int p = p0 + u * 16 + g * 4 + e;
             if (n == 0 && p < s.len) {
-                if (a.chunks > 1) to[p] = there[u] ? w : 0.f;
+                if (x.all > 1) to[p] = there[u] ? w : 0.f;
                 else if (there[u]) to[p] += w;
             }
         }
 }
 
-// Add the chunks of rows: those that the second pass made, in their order.
+// Add a sequence's chunks, of which it has more than one: those that the second
+// pass made, in their order.
 __global__ __launch_bounds__(256) void k_kv_observe_add(ObserveArgs a) {
     const int p = blockIdx.x * 256 + threadIdx.x, head = blockIdx.y;
-    const Seq s = sequence_at(a, blockIdx.z);
+    const int lane = threadIdx.x & 63, b = blockIdx.z;
+    const Seq s = sequence_at(a, b);
     const int G = a.group.d, R = s.m * G;
-    if (p >= s.len || R == 0) return;
+    if ((int)blockIdx.x * 256 >= s.len || R <= a.chunk) return;
+    // (`starts` out of order may make more chunks than there are)
+    int before = 0;
+    for (int x = lane; x < b; x += 64)
+        before = min(before + (sequence_at(a, x).m * G + a.chunk - 1) / a.chunk,
+                     a.chunks);
+    #pragma unroll
+    for (int x = 1; x < 64; x <<= 1) before += __shfl_xor(before, x, 64);
     const int from = max(0, p / a.block * a.block - (s.len - s.m)) * G;
-    if (from >= R) return;
-    const float* part = a.partial
-        + ((int64_t)s.b * a.kv_heads + head) * a.ld + p;
-    const int64_t step = (int64_t)a.slots * a.kv_heads * a.ld;
+    if (p >= s.len || from >= R) return;
+    const int64_t step = (int64_t)a.kv_heads * a.ld;
+    const float* part = a.partial + before * step + (int64_t)head * a.ld + p;
+    const int end = min((R - 1) / a.chunk + 1, a.chunks - before);
     float w = 0.f;
     #pragma unroll 8
-    for (int c = from / a.chunk; c <= (R - 1) / a.chunk; c++)
-        w += part[c * step];
+    for (int c = from / a.chunk; c < end; c++) w += part[c * step];
     reinterpret_cast<float*>(a.mass.data)[
         s.b * a.mass.slot_stride + head * a.mass.head_stride + p] += w;
 }
@@ -1452,7 +1482,7 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
 //
 // NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 33 us, 42
 // with KPT 32, 60 with 0), 32 up to 32768 (of 20000: 67 us, 185 with 0).
-// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 24 us, 98 with 1024
+// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 19 us, 98 with 1024
 // threads).
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
@@ -1778,17 +1808,26 @@ inline int64_t observe_wgs(int64_t tiles, int per) {
 
 struct ObserveCut {
     int64_t blocks, parts, part, chunks, chunk, block, place_blocks;
+    bool several;                   // a sequence may have several chunks
     int64_t sums, lse, partial;     // bytes
 };
 
-// Rows of a workgroup of the first pass in its form for few rows, by the rows
-// that a sequence has on average; 0: the other form. (4 rows of 8 sequences of
-// up to 3867 places, 32 kv heads: 27 us, 69 in the other form; 16 x 4 rows over
-// 131071 places, 8 kv heads: 56 us, 79.)
-int64_t observe_few(const KvPages& kv, int q_heads, int rows, KVT type) {
+// Rows of a workgroup of the first pass in its form for few rows; 0: the other
+// form. For few rows a sequence on average (4 rows of 8 sequences of up to 3867
+// places, 32 kv heads: 27 us, 69 in the other form; 16 x 4 rows over 131071
+// places, 8 kv heads: 56 us, 79), and where the other form would not have 256
+// workgroups (4 x 100 x 4 rows, 500 places, 8 kv heads: 13 us, 19 in the other
+// form; 500 rows, 2000 places, 16 heads of 64: 13 us, 16; with more of them it
+// loses, 512 x 4 rows over 8000 places: 98 us, 50).
+int64_t observe_few(const KvPages& kv, int q_heads, int rows, int reach,
+                    KVT type) {
     const int64_t R = (int64_t)rows * (q_heads / kv.kv_heads);
     const int64_t most = type == KVT::F32 ? 32 : 64;   // what registers hold
-    return R <= 16ll * kv.slots ? 16 : R <= most * kv.slots ? most : 0;
+    if (R <= 16ll * kv.slots) return 16;
+    const int64_t per = 4 * most;                      // the other form's
+    const int64_t wgs = ((R + per - 1) / per + kv.slots - 1) * kv.kv_heads
+        * ((reach + 511) / 512);
+    return R <= most * kv.slots || wgs < 256 ? most : 0;
 }
 
 ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
@@ -1796,7 +1835,7 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     if ((int64_t)rows * (q_heads / kv.kv_heads) >= (1ll << 28))
         throw std::runtime_error("observe: too many rows");
     const int64_t G = q_heads / kv.kv_heads, R = std::max<int64_t>(rows, 1) * G;
-    const int64_t few = observe_few(kv, q_heads, rows, type);
+    const int64_t few = observe_few(kv, q_heads, rows, reach, type);
     const int64_t per = few ? few : 16 * WAVES * (type == KVT::F32 ? 2 : 4);
     auto up = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     ObserveCut c;
@@ -1810,16 +1849,17 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     c.parts = up(places, c.part);
     c.block = 16 * WAVES * obs_groups(type != KVT::F32, kv.dim);
     c.place_blocks = up(places, c.block);
-    const int64_t blocks = c.place_blocks * kv.kv_heads * kv.slots;
-    c.chunks = std::min(up(observe_wgs(blocks * up(R, 64), OBSERVE_TILES_2),
-                           blocks), up(R, 128));
-    c.chunk = up(up(R, c.chunks), 64) * 64;
-    c.chunks = up(R, c.chunk);
+    const int64_t blocks = c.place_blocks * kv.kv_heads;
+    const int64_t cuts = up(observe_wgs(blocks * up(R, 64), OBSERVE_TILES_2),
+                            blocks);
+    c.chunk = up(up(R, cuts), 64) * 64;
+    c.several = R > c.chunk;
+    c.chunks = up(R, c.chunk) + kv.slots - 1;
     c.sums = c.parts > 1 ? aligned((size_t)c.parts * rows * q_heads * 8) : 0;
     c.lse = aligned((size_t)std::max(rows, 1) * q_heads * 4);
-    c.partial = c.chunks > 1
-        ? aligned((size_t)c.chunks * kv.slots * kv.kv_heads
-                  * c.place_blocks * c.block * 4) : 0;
+    c.partial = c.several
+        ? aligned((size_t)c.chunks * kv.kv_heads * c.place_blocks * c.block
+                  * 4) : 0;
     return c;
 }
 
@@ -1857,7 +1897,7 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                   c.place_blocks * c.block};
     KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
         constexpr int RW = NQ > 1 ? 2 : 4, PW = obs_groups(NQ == 1, D);
-        const int64_t few = observe_few(kv, q_heads, rows, type);
+        const int64_t few = observe_few(kv, q_heads, rows, reach, type);
         auto* sums = few == 16 ? k_kv_observe_few<C, NQ, D, 1>
             : few ? k_kv_observe_few<C, NQ, D, RW>
                   : k_kv_observe_sums<C, NQ, D, RW>;
@@ -1871,9 +1911,9 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                                dim3(256), 0, stream, a);
         hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D, PW>),
                            dim3((uint32_t)(c.place_blocks * c.chunks),
-                                kv.kv_heads, kv.slots),
+                                kv.kv_heads),
                            dim3(256), 0, stream, a);
-        if (c.chunks > 1)
+        if (c.several)
             hipLaunchKernelGGL(k_kv_observe_add,
                                dim3((reach + 255) / 256, kv.kv_heads,
                                     kv.slots),

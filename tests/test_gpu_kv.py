@@ -409,6 +409,42 @@ def test_observe_longer(types):
     check_observe(q, pool, table, lens, [0, 1030, 1807], types)
 
 
+@pytest.mark.parametrize("types", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("heads,rows", [(2, 1300), (16, 1300)])
+def test_observe_uneven_batch(types, heads, rows):
+    """One of 70 sequences has nearly all the rows: several chunks of them,
+    which the others' one or none go before and come after."""
+    B, long_ = 70, 66
+    m = [b % 4 for b in range(B)]
+    lens = [x + 5 * (b % 7) for b, x in enumerate(m)]
+    m[long_], lens[long_] = rows, rows + 200
+    _, pool, table = make(39, lens, heads, 2, 64, 32, types, strange=False)
+    q = torch.randn(sum(m) + 2, heads, 64,
+                    generator=torch.Generator().manual_seed(2)).to(types[0])
+    starts = [sum(m[:b]) for b in range(B + 1)]
+    assert torch.equal(check_observe(q, pool, table, lens, starts, types),
+                       check_observe(q, pool, table, lens, starts, types))
+
+
+def test_observe_starts_out_of_order():
+    """Nothing is added behind a sequence's places, or to one without rows."""
+    from crowdllama_amd.ops import kv
+    lens = [900, 40, 700, 0, 64]
+    _, pool, table = make(40, lens, 16, 4, 64, 32, TYPES[1], strange=False)
+    q = torch.randn(600, 16, 64).bfloat16().cuda()
+    cap = table.shape[1] * 32
+    for starts in ([0, 600, 0, 600, 0, 600], [2**31 - 1, 0, 600, 5, -7, 900],
+                   [0, 600, 600, 600, 600, -2**31]):
+        mass = torch.ones(5, 4, cap, device="cuda")
+        kv.observe(q, pool.cuda(), table.cuda(), ints(lens), mass,
+                   starts=ints(starts))
+        mass = mass.cpu()
+        for b, n in enumerate(lens):
+            assert (mass[b, :, n:] == 1).all()
+            if starts[b + 1] <= max(starts[b], 0):
+                assert (mass[b] == 1).all()
+
+
 def test_observe_more_rows_than_places():
     """A row before the first place sees nothing, and adds nothing."""
     from crowdllama_amd.ops import kv
@@ -494,6 +530,60 @@ def test_observe_nan_and_inf():
     kv.observe(q.cuda(), *args(), got, starts=ints([0, 80]))
     assert got[0, 0, :120].isnan().all() and torch.equal(got[0, 1],
                                                          clean[0, 1])
+
+
+def many(types, n, m, seed=41, **kw):
+    """24 sequences and 8 heads: enough rows for a pass that stages its keys."""
+    lens, rows = [n - b for b in range(24)], [m - 2 * b for b in range(24)]
+    _, pool, table = make(seed, lens, 8, 8, 64, 16, types, **kw)
+    q = torch.randn(sum(rows), 8, 64,
+                    generator=torch.Generator().manual_seed(2))
+    return q, pool, table, lens, [sum(rows[:b]) for b in range(25)]
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("n,m", [(200, 170), (700, 160)])
+@pytest.mark.parametrize("missing", [False, True])
+def test_observe_many_rows(types, n, m, missing):
+    q, pool, table, lens, starts = many(types, n, m)
+    if missing:
+        table[0, 1], table[2, :], table[5, 3], table[7, 0] = -7, 1 << 30, -1, -1
+    check_observe(q.to(types[0]), pool, table, lens, starts, types)
+
+
+@pytest.mark.parametrize("types", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("factor,shift", [(20., 0.), (1., -30.), (1., 30.),
+                                          (6., -12.)])
+@pytest.mark.parametrize("n,m", [(200, 170), (700, 160)])
+def test_observe_many_far_rows(types, factor, shift, n, m):
+    q, pool, table, lens, starts = many(types, n, m, strange=False)
+    q, pool = factor * q, pool.float()
+    q[..., 0], pool[:, :, 0, :, 0] = shift, 64.
+    check_observe(q.to(types[0]), pool.to(types[1]), table, lens, starts, types)
+
+
+def test_observe_nan_among_many_rows():
+    from crowdllama_amd.ops import kv
+    q, pool, table, lens, starts = many(TYPES[1], 200, 170, strange=False)
+    q = q.bfloat16()
+    cap = table.shape[1] * 16
+
+    def run():
+        got = torch.zeros(24, 8, cap, device="cuda")
+        return kv.observe(q.cuda(), pool.cuda(), table.cuda(), ints(lens), got,
+                          starts=ints(starts)).cpu()
+    clean = run()
+    q[starts[4] - 1, 2, 5] = math.nan          # sequence 3's last token
+    q[starts[9], 6, 5] = math.inf              # 9's first: sees 191 - 152 + 1
+    at = oracle.place(table, pool.shape[0], 16, 20, 179)
+    pool[at[0], 7, 0, at[1], 3] = math.nan     # 20's last token sees it alone
+    got = run()
+    assert got[3, 2, :197].isnan().all() and got[9, 6, :40].isnan().all()
+    assert got[20, 7, :180].isnan().all()
+    # rows of the same workgroup: summed another way, as above
+    assert torch.allclose(got[9, 6, 40:], clean[9, 6, 40:], rtol=2e-4)
+    got[3, 2], got[9, 6], got[20, 7] = clean[3, 2], clean[9, 6], clean[20, 7]
+    assert torch.equal(got, clean)
 
 
 # -------------------------------------------------------------------- evict
