@@ -771,10 +771,11 @@ Div div_by(int d) {
             d > 1 ? (uint32_t)((0xFFFFFFFFull + (uint32_t)d) / d) : 0u};
 }
 
-// Groups of 16 places that a wave of the second pass holds. Three leave room
-// for a third wave a SIMD with heads of 128 and one piece (8192 rows of 32
-// heads: 344 us, 422 with four); more pieces have more to do for each row that
-// is read (3 x 500 rows over 16000 places: 307 us, 355 with three).
+// Groups of 16 places that a wave of the second pass holds, where there is
+// work for many. Three leave room for a third wave a SIMD with heads of 128 and
+// one piece (8192 rows of 32 heads: 350 us, 422 with four); more pieces have
+// more to do for each row that is read (3 x 500 rows over 16000 places: 307 us,
+// 355 with three).
 constexpr int obs_groups(bool one_piece, int dim) {
     return one_piece && dim == 128 ? 3 : 4;
 }
@@ -1808,6 +1809,7 @@ inline int64_t observe_wgs(int64_t tiles, int per) {
 
 struct ObserveCut {
     int64_t blocks, parts, part, chunks, chunk, block, place_blocks;
+    bool two;                       // a wave holds two groups of places
     bool several;                   // a sequence may have several chunks
     int64_t sums, lse, partial;     // bytes
 };
@@ -1847,9 +1849,19 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
            row_blocks), up(places, 512));
     c.part = up(up(places, c.parts), 64) * 64;
     c.parts = up(places, c.part);
-    c.block = 16 * WAVES * obs_groups(type != KVT::F32, kv.dim);
-    c.place_blocks = up(places, c.block);
-    const int64_t blocks = c.place_blocks * kv.kv_heads;
+    // Two groups of 16 places a wave where that many workgroups' worth of
+    // tiles of 64 rows would leave most of the chip idle (300 x 4 float32 rows
+    // of 8 kv heads: 9 us, 14 with four; 500 rows of 2000 places, 16 heads of
+    // 64: 9.5 us, 12 with four; 900 x 4 float32 rows, 1824 tiles: 35 us, 30
+    // with four).
+    int64_t blocks;
+    for (int groups : {obs_groups(type != KVT::F32, kv.dim), 2}) {
+        c.block = 16 * WAVES * groups;
+        c.place_blocks = up(places, c.block);
+        blocks = c.place_blocks * kv.kv_heads;
+        c.two = groups == 2;
+        if (blocks * up(R, 64) > 1024) break;
+    }
     const int64_t cuts = up(observe_wgs(blocks * up(R, 64), OBSERVE_TILES_2),
                             blocks);
     c.chunk = up(up(R, cuts), 64) * 64;
@@ -1909,7 +1921,9 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                                dim3((uint32_t)(((int64_t)rows * q_heads + 31)
                                                / 32)),
                                dim3(256), 0, stream, a);
-        hipLaunchKernelGGL((k_kv_observe_mass<C, NQ, D, PW>),
+        auto* mass_of = c.two ? k_kv_observe_mass<C, NQ, D, 2>
+                              : k_kv_observe_mass<C, NQ, D, PW>;
+        hipLaunchKernelGGL(mass_of,
                            dim3((uint32_t)(c.place_blocks * c.chunks),
                                 kv.kv_heads),
                            dim3(256), 0, stream, a);

@@ -532,20 +532,21 @@ def test_observe_nan_and_inf():
                                                          clean[0, 1])
 
 
-def many(types, n, m, seed=41, **kw):
+def many(types, n, m, seed=41, dim=64, **kw):
     """24 sequences and 8 heads: enough rows for a pass that stages its keys."""
     lens, rows = [n - b for b in range(24)], [m - 2 * b for b in range(24)]
-    _, pool, table = make(seed, lens, 8, 8, 64, 16, types, **kw)
-    q = torch.randn(sum(rows), 8, 64,
+    _, pool, table = make(seed, lens, 8, 8, dim, 16, types, **kw)
+    q = torch.randn(sum(rows), 8, dim,
                     generator=torch.Generator().manual_seed(2))
     return q, pool, table, lens, [sum(rows[:b]) for b in range(25)]
 
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
-@pytest.mark.parametrize("n,m", [(200, 170), (700, 160)])
+@pytest.mark.parametrize("n,m,dim", [(200, 170, 64), (700, 160, 64),
+                                     (700, 160, 96), (700, 160, 128)])
 @pytest.mark.parametrize("missing", [False, True])
-def test_observe_many_rows(types, n, m, missing):
-    q, pool, table, lens, starts = many(types, n, m)
+def test_observe_many_rows(types, n, m, dim, missing):
+    q, pool, table, lens, starts = many(types, n, m, dim=dim)
     if missing:
         table[0, 1], table[2, :], table[5, 3], table[7, 0] = -7, 1 << 30, -1, -1
     check_observe(q.to(types[0]), pool, table, lens, starts, types)
