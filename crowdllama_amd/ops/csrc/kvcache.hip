@@ -381,6 +381,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
         all += (len_of(b) + UNIT - 1) / UNIT;
     #pragma unroll
     for (int m = 32; m; m >>= 1) all += __shfl_xor(all, m, 64);
+    all = __builtin_amdgcn_readfirstlane(all);
     const int per = max(1u, ((uint32_t)all * a.kv_heads + a.target - 1)
                                 / (uint32_t)a.target);
     int before = 0;
@@ -397,12 +398,13 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
         }
         const uint64_t over = __ballot(before + upto > id);
         if (over) {
+            // scalars, as all that follows from them
             const int at = __builtin_ctzll(over);
-            const int len_b = __shfl(len, at, 64);
+            auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+            const int len_b = of(len);
             p.b = base + at;
-            p.n = __shfl(n, at, 64);
-            const int rest = id - before
-                - (__shfl(upto, at, 64) - p.n * a.kv_heads);
+            p.n = of(n);
+            const int rest = id - before - (of(upto) - p.n * a.kv_heads);
             p.head = rest / p.n;
             p.j = rest - p.head * p.n;
             p.first = id - p.j;
@@ -414,7 +416,7 @@ __device__ __forceinline__ bool find_part(const AttendArgs& a, int id,
             p.there = 1;
             return true;
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return false;
 }
