@@ -490,12 +490,131 @@ __device__ __forceinline__ void load_tile(const uint16_t* r0,
     }
 }
 
-// One workgroup takes one part of one kv head's places, its four waves 32 at
-// a time in turn. S = K Q^T and O^T = V^T P^T, so that in both results a
+// What a lane has of its query head: the maximum of the wave's places, the sum
+// of its own places' weights, and its outputs.
+template <int D>
+struct Softmax {
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[D / 16];
+    __device__ Softmax() {
+        #pragma unroll
+        for (int e = 0; e < D / 16; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+};
+
+// 32 places from p0 on: S = K Q^T and O^T = V^T P^T, so that in both results a
 // lane's column is its query head: maximum, sum and rescaling stay in the
 // lane. S's rows (places) then are just the k index of the second product,
 // and V needs no transposition through LDS: a lane holds 8 places x EL
 // elements, and product e takes element e of each (MFMA row r is d = r*EL+e).
+// t0, t1: whether the first and the second 16 have a page. Scores go to
+// put(place, 4 of them).
+template <class C, int NQ, int NP, int D, class Put>
+__device__ __forceinline__ void use_tile(Tile<D>& t, bool t0, bool t1, int p0,
+                                         int hi, float scale2, int g,
+                                         const u32x4 (*q)[D / 32],
+                                         Softmax<D>& x, Put put) {
+    constexpr int EL = D / 16;
+    float &m = x.m, &l = x.l;
+    f32x4* o = x.o;
+    const bool whole = t0 && t1 && p0 + TILE <= hi;
+    float s[8];
+    #pragma unroll
+    for (int u = 0; u < 2; u++) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        #pragma unroll
+        for (int y = NQ - 1; y >= 0; y--)
+            #pragma unroll
+            for (int kk = 0; kk < D / 32; kk++)
+                acc = C::mfma(t.k[u][kk], q[y][kk], acc);
+        #pragma unroll
+        for (int i = 0; i < 4; i++) s[u * 4 + i] = acc[i] * scale2;
+    }
+    if (!whole) {
+        #pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int u = j >> 2;
+            const bool seen = (u ? t1 : t0) &&
+                p0 + u * 16 + g * 4 + (j & 3) < hi;
+            if (!seen) {
+                s[j] = -INFINITY;
+                // what lies there may be anything: 0 * inf is NaN
+                #pragma unroll
+                for (int e = 0; e < EL / 2; e++) t.v[j][e] = 0;
+            }
+        }
+    }
+    #pragma unroll
+    for (int u = 0; u < 2; u++)
+        put(u * 16 + g * 4, f32x4{s[u * 4], s[u * 4 + 1], s[u * 4 + 2],
+                                  s[u * 4 + 3]});
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                      fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    top = wave_xor_max(wave_xor_max(top, 16), 32);
+    if (__any(top > m)) {
+        const float now = fmaxf(m, top);
+        const float f = exp2_fast(m - now);   // 0 from -inf
+        m = now;
+        if (now > -INFINITY) {
+            l *= f;
+            #pragma unroll
+            for (int e = 0; e < EL; e++) o[e] *= f;
+        }
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float w[8];
+    #pragma unroll
+    for (int j = 0; j < 8; j++) {
+        w[j] = exp2_fast(s[j] - ref);
+        l += w[j];
+    }
+    u32x4 pf[NP];
+    #pragma unroll
+    for (int y = 0; y < NP; y++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            pf[y][i] = C::piece(w[2 * i], w[2 * i + 1]);
+    #pragma unroll
+    for (int e = 0; e < EL; e++) {
+        u32x4 vf;
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            vf[i] = __builtin_amdgcn_perm(
+                t.v[2 * i + 1][e >> 1], t.v[2 * i][e >> 1],
+                (e & 1) ? 0x07060302u : 0x05040100u);
+        #pragma unroll
+        for (int y = NP - 1; y >= 0; y--) o[e] = C::mfma(vf, pf[y], o[e]);
+    }
+}
+
+template <class C, bool F32>
+__device__ __forceinline__ void put_out(const AttendArgs& a, int b, int head,
+                                        int d, float y) {
+    const int64_t at = b * a.out.row_stride
+        + (int64_t)head * a.out.head_stride + d;
+    if constexpr (F32)
+        reinterpret_cast<float*>(a.out.data)[at] = y;
+    else
+        reinterpret_cast<uint16_t*>(a.out.data)[at] =
+            (uint16_t)C::pack(y, 0.f);
+}
+
+// A workgroup's waves join: s_m, s_l, s_o take what its lanes have, a lane's
+// l being of its own places only.
+template <int D>
+__device__ __forceinline__ void give(const Softmax<D>& x, int n, int g,
+                                     float* s_m, float* s_l, float (*s_o)[D]) {
+    const float l = wave_xor_sum(wave_xor_sum(x.l, 16), 32);
+    if (g == 0) { s_m[n] = x.m; s_l[n] = l; }
+    #pragma unroll
+    for (int e = 0; e < D / 16; e++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+            s_o[n][(g * 4 + i) * (D / 16) + e] = x.o[e][i];
+}
+
+// One workgroup takes one part of one kv head's places, its four waves 32 at
+// a time in turn.
 //
 // Bound by the reads of K and V: one sequence of 131071 places of 8 kv heads of
 // 128 (537 MB) takes 95 us without a mass, 5.6 TB/s, as fast as a stream that
@@ -505,7 +624,6 @@ __device__ __forceinline__ void load_tile(const uint16_t* r0,
 // gains nothing (119 us for 112).
 template <class C, int NQ, int NP, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
-    constexpr int EL = D / 16;
     __shared__ float s_m[WAVES][16], s_l[WAVES][16];
     __shared__ float s_o[WAVES][16][D];
     Part p;
@@ -525,10 +643,7 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
     load_q<C, NQ, D>(a.q.data,
                      p.b * a.q.row_stride + head * a.q.head_stride, n < G, g,
                      q);
-    float m = -INFINITY, l = 0.f;
-    f32x4 o[EL];
-    #pragma unroll
-    for (int e = 0; e < EL; e++) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Softmax<D> sm;
     float* scores = MASS && n < G
         ? a.scores + ((int64_t)p.b * a.kv_heads + p.head) * G * a.ld + n * 32
         : nullptr;
@@ -542,88 +657,15 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
         // and count for nothing
         Tile<D> t;
         load_tile<D>(r0 ? r0 : a.kv.pool, r1 ? r1 : a.kv.pool, to_v, n, g, t);
-        const bool whole = r0 && r1 && p0 + TILE <= p.hi;
-        float s[8];
-        #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            #pragma unroll
-            for (int x = NQ - 1; x >= 0; x--)
-                #pragma unroll
-                for (int kk = 0; kk < D / 32; kk++)
-                    acc = C::mfma(t.k[u][kk], q[x][kk], acc);
-            #pragma unroll
-            for (int i = 0; i < 4; i++) s[u * 4 + i] = acc[i] * a.scale2;
-        }
-        if (!whole) {
-            #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int u = j >> 2;
-                const bool seen = (u ? r1 : r0) &&
-                    p0 + u * 16 + g * 4 + (j & 3) < p.hi;
-                if (!seen) {
-                    s[j] = -INFINITY;
-                    // what lies there may be anything: 0 * inf is NaN
-                    #pragma unroll
-                    for (int e = 0; e < EL / 2; e++) t.v[j][e] = 0;
-                }
-            }
-        }
-        if (MASS && scores) {
-            // a tile's scores lie together
-            #pragma unroll
-            for (int u = 0; u < 2; u++)
-                *reinterpret_cast<f32x4*>(scores + (int64_t)p0 * G + u * 16
-                                          + g * 4) =
-                    f32x4{s[u * 4], s[u * 4 + 1], s[u * 4 + 2], s[u * 4 + 3]};
-        }
-        float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
-                          fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-        top = wave_xor_max(wave_xor_max(top, 16), 32);
-        if (__any(top > m)) {
-            const float now = fmaxf(m, top);
-            const float f = exp2_fast(m - now);   // 0 from -inf
-            m = now;
-            if (now > -INFINITY) {
-                l *= f;
-                #pragma unroll
-                for (int e = 0; e < EL; e++) o[e] *= f;
-            }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float w[8];
-        #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            w[j] = exp2_fast(s[j] - ref);
-            l += w[j];
-        }
-        u32x4 pf[NP];
-        #pragma unroll
-        for (int x = 0; x < NP; x++)
-            #pragma unroll
-            for (int i = 0; i < 4; i++)
-                pf[x][i] = C::piece(w[2 * i], w[2 * i + 1]);
-        #pragma unroll
-        for (int e = 0; e < EL; e++) {
-            u32x4 vf;
-            #pragma unroll
-            for (int i = 0; i < 4; i++)
-                vf[i] = __builtin_amdgcn_perm(
-                    t.v[2 * i + 1][e >> 1], t.v[2 * i][e >> 1],
-                    (e & 1) ? 0x07060302u : 0x05040100u);
-            #pragma unroll
-            for (int x = NP - 1; x >= 0; x--) o[e] = C::mfma(vf, pf[x], o[e]);
-        }
+        use_tile<C, NQ, NP, D>(
+            t, r0, r1, p0, p.hi, a.scale2, g, q, sm, [&](int x, f32x4 s) {
+                // a tile's scores lie together
+                if (MASS && scores)
+                    *reinterpret_cast<f32x4*>(scores + (int64_t)p0 * G + x) = s;
+            });
     }
 
-    // join the four waves; a lane's l is of its own places only
-    l = wave_xor_sum(wave_xor_sum(l, 16), 32);
-    if (g == 0) { s_m[wave][n] = m; s_l[wave][n] = l; }
-    #pragma unroll
-    for (int e = 0; e < EL; e++)
-        #pragma unroll
-        for (int i = 0; i < 4; i++)
-            s_o[wave][n][(g * 4 + i) * EL + e] = o[e][i];
+    give<D>(sm, n, g, s_m[wave], s_l[wave], s_o[wave]);
     __syncthreads();
     for (int x = tid; x < G * D; x += 256) {
         const int h = x / D, d = x % D;
@@ -639,20 +681,83 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
             acc += f * s_o[w][h][d];
         }
         if (p.n == 1) {
-            const float y = sum == 0.f ? 0.f : acc / sum;
-            const int64_t at = p.b * a.out.row_stride
-                + (int64_t)(p.head * G + h) * a.out.head_stride + d;
-            if constexpr (NQ == 1)
-                reinterpret_cast<uint16_t*>(a.out.data)[at] =
-                    (uint16_t)C::pack(y, 0.f);
-            else
-                reinterpret_cast<float*>(a.out.data)[at] = y;
+            put_out<C, (NQ > 1)>(a, p.b, p.head * G + h, d,
+                                 sum == 0.f ? 0.f : acc / sum);
         } else {
             a.part_o[((int64_t)blockIdx.x * G + h) * D + d] = acc;
         }
         if (d == 0) {
             a.part_ml[((int64_t)blockIdx.x * G + h) * 2] = top;
             a.part_ml[((int64_t)blockIdx.x * G + h) * 2 + 1] = sum;
+        }
+    }
+}
+
+// Short rows, grid (kv heads, slots): eight waves take all of a row's places,
+// and its mass in the same launch, from scores in LDS. Bound by what one CU can
+// have under way, about 2.4 us for each 256 places of heads of 128; the next
+// tile's loads ahead of a tile's products gain nothing.
+constexpr int ROW_WAVES = 8, ROW_PLACES = 1024;
+
+template <class C, int NQ, int NP, int D, bool MASS>
+__global__ __launch_bounds__(64 * ROW_WAVES) void k_kv_attend_row(
+    AttendArgs a) {
+    __shared__ float s_m[ROW_WAVES][16], s_l[ROW_WAVES][16];
+    __shared__ float s_ref[16], s_r[16];
+    __shared__ float s_o[ROW_WAVES][16][D];
+    __shared__ __align__(16) float s_s[MASS ? ROW_PLACES * 16 : 4];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15, g = lane >> 4, b = blockIdx.y;
+    const int G = a.q_heads / a.kv_heads, first = blockIdx.x * G;
+    const int len = kv_clamp_len(a.lens[b] + a.add, a.reach);
+    u32x4 q[NQ][D / 32];
+    load_q<C, NQ, D>(a.q.data, b * a.q.row_stride
+                         + (int64_t)(first + n) * a.q.head_stride, n < G, g, q);
+    const int64_t to_v = (int64_t)a.kv.page * D;
+    Softmax<D> sm;
+    for (int p0 = wave * TILE; p0 < len; p0 += TILE * ROW_WAVES) {
+        const uint16_t* r0 = a.kv.rows16(b, p0, blockIdx.x, D);
+        const uint16_t* r1 = p0 + 16 < len
+            ? a.kv.rows16(b, p0 + 16, blockIdx.x, D) : nullptr;
+        Tile<D> t;
+        load_tile<D>(r0 ? r0 : a.kv.pool, r1 ? r1 : a.kv.pool, to_v, n, g, t);
+        use_tile<C, NQ, NP, D>(
+            t, r0, r1, p0, len, a.scale2, g, q, sm, [&](int x, f32x4 s) {
+                if (MASS && n < G)
+                    *reinterpret_cast<f32x4*>(s_s + p0 * G + n * 32 + x) = s;
+            });
+    }
+    give<D>(sm, n, g, s_m[wave], s_l[wave], s_o[wave]);
+    __syncthreads();
+    for (int x = tid; x < G * D; x += 64 * ROW_WAVES) {
+        const int h = x / D, d = x % D;
+        float top = s_m[0][h];
+        #pragma unroll
+        for (int w = 1; w < ROW_WAVES; w++) top = fmaxf(top, s_m[w][h]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, acc = 0.f;
+        #pragma unroll
+        for (int w = 0; w < ROW_WAVES; w++) {
+            const float f = exp2_fast(s_m[w][h] - ref);
+            sum += f * s_l[w][h];
+            acc += f * s_o[w][h][d];
+        }
+        const float r = sum == 0.f ? 0.f : 1.f / sum;
+        if (d == 0) { s_ref[h] = ref; s_r[h] = r; }
+        put_out<C, (NQ > 1)>(a, b, first + h, d,
+                             sum == 0.f ? 0.f : acc / sum);
+    }
+    if constexpr (MASS) {
+        __syncthreads();
+        float* mass = reinterpret_cast<float*>(a.mass.data)
+            + b * a.mass.slot_stride + blockIdx.x * a.mass.head_stride;
+        for (int x = tid; x < len; x += 64 * ROW_WAVES) {
+            const float* sc = s_s + (x & ~31) * G + (x & 31);
+            float w = 0.f;
+            for (int h = 0; h < G; h++)
+                w += exp2_fast(sc[h * 32] - s_ref[h]) * s_r[h];
+            mass[x] += w;
         }
     }
 }
@@ -745,14 +850,8 @@ __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
             __syncthreads();
             if (tid < width && x < hi) {
                 for (int i = 1; i < deal; i++) acc += s_acc[i * width + tid];
-                const float v = acc * s_r[h];
-                const int64_t at = p.b * a.out.row_stride
-                    + (int64_t)(p.head * G + h) * a.out.head_stride + x % D;
-                if constexpr (F32OUT)
-                    reinterpret_cast<float*>(a.out.data)[at] = v;
-                else
-                    reinterpret_cast<uint16_t*>(a.out.data)[at] =
-                        (uint16_t)C::pack(v, 0.f);
+                put_out<C, F32OUT>(a, p.b, p.head * G + h, x % D,
+                                   acc * s_r[h]);
             }
         }
     }
@@ -1753,12 +1852,22 @@ int64_t attend_wgs(const KvPages& kv, int reach) {
     return std::min(attend_target(kv) + rows,
                     rows * std::max(1, (reach + UNIT - 1) / UNIT));
 }
+// Whether a row's places, which `reach` bounds, are one workgroup's: one launch
+// and no join then take less time than more workgroups save. 8 rows of 300
+// places 9 us, 13.5 in parts; 64 of 700, 13 and 13; 8 of 1000, 16 and 12.5; 128
+// of 1000, 18 and 19.5; 256 of 1000, 18 and 25; 1024 of 300, 21 and 26; but
+// 2048 of 200, 45 and 37 (its LDS leaves a CU one workgroup).
+bool attend_rows(const KvPages& kv, int reach) {
+    const int64_t rows = (int64_t)kv.slots * kv.kv_heads;
+    return rows <= 1024 && reach <= (rows < 128 ? 768 : ROW_PLACES);
+}
 int64_t scores_ld(int reach) { return (int64_t)(reach + 31) / 32 * 32; }
 }  // namespace
 
 size_t kv_attend_workspace(const KvPages& kv, int q_heads, int reach,
                            bool mass) {
     check_pages(kv, q_heads, reach);
+    if (attend_rows(kv, reach)) return 0;
     const int64_t wgs = attend_wgs(kv, reach), G = q_heads / kv.kv_heads;
     return aligned(wgs * G * kv.dim * 4) + aligned(wgs * G * 2 * 4)
         + aligned(wgs * sizeof(Part)) + (mass ? aligned((size_t)kv.slots * q_heads * scores_ld(reach) * 4)
@@ -1784,6 +1893,17 @@ void launch_kv_attend(const KvPages& kv, const KvHeads& q, const KvHeads& out,
     a.parts = reinterpret_cast<Part*>(w);
     w += aligned(wgs * sizeof(Part));
     a.scores = reinterpret_cast<float*>(w);
+    if (attend_rows(kv, reach)) {
+        #define ATTEND(M)                                                     \
+            KV_TYPES(type, kv.type, KV_DIM(kv.dim,                            \
+                hipLaunchKernelGGL((k_kv_attend_row<C, NQ, NP, D, M>),        \
+                                   dim3(kv.kv_heads, kv.slots),               \
+                                   dim3(64 * ROW_WAVES), 0, stream, a)))
+        if (mass.data) ATTEND(true); else ATTEND(false);
+        #undef ATTEND
+        check_launch();
+        return;
+    }
     const dim3 grid((uint32_t)wgs), block(256);
     #define ATTEND(M)                                                         \
         KV_TYPES(type, kv.type, KV_DIM(kv.dim, {                              \

@@ -271,7 +271,11 @@ def _scale(scale, dim: int) -> float:
 
 
 def _workspace(n: int, table):
-    return table.new_empty(n // 4 + 1)
+    return table.new_empty(n // 4 + 1) if n else None
+
+
+def _at(ws) -> int:
+    return 0 if ws is None else ws.data_ptr()
 
 
 # the stream's handle without an object around it
@@ -380,7 +384,7 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
                                              mass is not None), table)
     core.kv_attend(kv, qh, oh, q_heads, _TYPES[q.dtype], le, ms, reach,
-                   scale, ws.data_ptr(), _stream(dev))
+                   scale, _at(ws), _stream(dev))
     return out
 
 
@@ -414,7 +418,7 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
                                               _TYPES[q.dtype]), table)
     core.kv_observe(kv, qh, q_heads, _TYPES[q.dtype], rows, st, le,
                     ms, reach,
-                    scale, ws.data_ptr(), _stream(dev))
+                    scale, _at(ws), _stream(dev))
     return mass
 
 
@@ -476,5 +480,6 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     core = _get(dev)
     ws = _workspace(core.kv_evict_workspace(kv, layers, keep, reach), table)
     core.kv_evict(kv, layers, pool.stride(1), le, lo, np,
-                  ms, ps, mo, po, keep, recent, limit, reach, ws.data_ptr(), _stream(dev))
+                  ms, ps, mo, po, keep, recent, limit, reach, _at(ws),
+                  _stream(dev))
     return mass_out, pos_out, lens_out

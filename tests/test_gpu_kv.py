@@ -230,6 +230,75 @@ def test_attend_past_32_bits():
                                       ints(lens)))
 
 
+def longer(table, page):
+    """Room for more places than one workgroup takes: rows go in parts."""
+    more = torch.full((table.shape[0], 2048 // page), -1, dtype=torch.int32)
+    return torch.cat([table, more], 1)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (3, 3), (16, 1)])
+def test_attend_in_parts(types, dim, heads, kv_heads):
+    lens = [70, 0, 1, 16, 17, 33, 128, 129, 300]
+    q, pool, table = make(1, lens, heads, kv_heads, dim, 32, types)
+    check_attend(q, pool, longer(table, 32), lens)
+
+
+def test_attend_in_parts_odd_pages_and_lengths():
+    from crowdllama_amd.ops import kv
+    lens = [100, 60, 50, 400]
+    q, pool, table = make(8, lens, 4, 2, 64, 16, TYPES[0])
+    table[0, 2], table[0, 5] = -1, pool.shape[0]
+    table[1, :] = 2 ** 30
+    got, _ = check_attend(q, pool, longer(table, 16), lens)
+    assert (got[1] == 0).all()
+    a = [x.cuda() for x in (q, pool, longer(table, 16))]
+    # 10^9 is as many as the table holds, NaN in unused places among them:
+    # off - off is NaN where it should be, so not check_attend's comparison
+    b = kv.attend(*a, ints([10 ** 9, -5, 50, 0]))
+    full, _, _, _ = oracle.attend(q, pool, longer(table, 16),
+                                  [10 ** 9, -5, 50, 0], 64 ** -.5)
+    assert torch.allclose(b.double().cpu(), full, atol=1e-5, equal_nan=True)
+    assert (b[[1, 3]] == 0).all() and torch.equal(b[2], got[2])
+    want = kv.attend(*a, ints(lens))
+    kv.attend(*a, ints(lens), out=a[0])              # into its queries
+    assert torch.equal(a[0], want)
+
+
+def test_attend_in_parts_nan_and_inf():
+    from crowdllama_amd.ops import kv
+    lens = [50, 50]
+    q, pool, table = make(11, lens, 4, 2, 64, 16, TYPES[1], strange=False)
+    want, _, _, _ = oracle.attend(q, pool, table, lens, 64 ** -.5)
+    pool[table[0, 1], 1, 0, 3] = math.nan
+    pool[table[1, 2], 0, 1, 2, 5] = math.inf
+    table = longer(table, 16)
+    mass = torch.zeros(2, 2, table.shape[1] * 16, device="cuda")
+    got = kv.attend(q.cuda(), pool.cuda(), table.cuda(), ints(lens),
+                    mass=mass).double().cpu()
+    assert got[0, 2:].isnan().all() and mass[0, 1, :50].isnan().all()
+    assert torch.allclose(got[0, :2], want[0, :2], atol=2.0 ** -7)
+    assert (got[1, :2, 5] == math.inf).all()
+    assert not mass[1].isnan().any() and not mass[0, 0].isnan().any()
+    assert (mass[..., 50:] == 0).all()
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("B,kv_heads,cap", [(16, 8, 1024), (2, 2, 768),
+                                            (257, 1, 96), (16, 8, 1040),
+                                            (1025, 1, 32)])
+def test_attend_full_rows(types, B, kv_heads, cap):
+    """Full caches at the sizes where one form gives way to the other."""
+    lens = [cap - 3 * (b % 7) for b in range(B)]
+    q, pool, table = make(13, lens, 2 * kv_heads, kv_heads, 64, 16, types,
+                          strange=False)
+    table = table[:, :cap // 16].contiguous()
+    a, m = check_attend(q, pool, table, lens)
+    b, n = check_attend(q, pool, table, lens)
+    assert torch.equal(a, b) and torch.equal(m, n)
+
+
 # ------------------------------------------------------------------- append
 
 @pytest.mark.parametrize("types", TYPES, ids=IDS)
