@@ -218,13 +218,9 @@ def _ends(t):
     """The addresses of a tensor's memory, from its first value to its last."""
     at = t.data_ptr()
     if t.is_contiguous():
-        return at, at + t.element_size() * t.numel()
+        return at, at + t.nbytes
     return at, at + t.element_size() * (
         1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-
-
-def _same(a, b) -> bool:
-    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
 
 def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
@@ -460,23 +456,33 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
         _fail("layers x sequences x kv heads must be below 2^22")
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
-    if out is None:
-        out = (mass, pos, lens)
-    mass_out, pos_out, lens_out = out
-    mo = _places(mass_out, "out's mass", torch.float32, lead, reach, dev)
-    po = _places(pos_out, "out's pos", torch.int32, lead, reach, dev)
-    lo = _vector(lens_out, "out's lens", slots, dev)
-    if mass_out.shape[-1] != reach or pos_out.shape[-1] != reach:
-        _fail("out's mass and pos must have as many places as mass")
     _no_grad(pool, mass)
-    olds = [(t, *_ends(t)) for t in (mass, pos, lens, next_pos)]
-    for i, new in enumerate((mass_out, pos_out, lens_out)):
-        lo_, hi_ = _ends(new)
-        for j, (old, first, last) in enumerate(olds):
-            if lo_ < last and first < hi_ and not (
-                    i == j and (new is old or _same(new, old))):
-                _fail("each of out must be the tensor that it replaces, or "
-                      "apart from all of them")
+    spans = [_ends(mass), _ends(pos), _ends(lens)]
+    if out is None:
+        mass_out, pos_out, lens_out = mass, pos, lens
+        mo, po, lo = ms, ps, le
+    else:
+        mass_out, pos_out, lens_out = out
+        mo = _places(mass_out, "out's mass", torch.float32, lead, reach, dev)
+        po = _places(pos_out, "out's pos", torch.int32, lead, reach, dev)
+        lo = _vector(lens_out, "out's lens", slots, dev)
+        if mass_out.shape[-1] != reach or pos_out.shape[-1] != reach:
+            _fail("out's mass and pos must have as many places as mass")
+        if mo != ms:
+            spans.append(_ends(mass_out))
+        if po != ps:
+            spans.append(_ends(pos_out))
+        if lo != le:
+            spans.append(_ends(lens_out))
+    if np != le or lo == le:       # both are only read, else
+        spans.append(_ends(next_pos))
+    spans.sort()
+    end = 0
+    for first, last in spans:
+        if first < end:
+            _fail("mass, pos, lens and next_pos must be apart from each "
+                  "other, and from each of out that does not replace one")
+        end = last
     core = _get(dev)
     ws = _workspace(core.kv_evict_workspace(kv, layers, keep, reach), table)
     core.kv_evict(kv, layers, pool.stride(1), le, lo, np,

@@ -159,6 +159,29 @@ def test_evict_refuses_a_mixed_out():
                                     ints(0, 0))}, "must be on a GPU")
 
 
+def test_evict_refuses_what_overlaps():
+    a = evict_args()
+    refused(kv.evict, {**a, "next_pos": a["lens"]}, "apart")
+    refused(kv.evict, {**a, "pos": a["mass"].view(torch.int32)}, "apart")
+    both = ints(1, 2, 3)
+    refused(kv.evict, {**a, "lens": both[:2], "next_pos": both[1:]}, "apart")
+    both = ints(1, 2, 3, 4)
+    refused(kv.evict, {**a, "lens": both[2:], "next_pos": both[:2]},
+            "must be on a GPU")
+
+
+def test_evict_refuses_an_out_that_overlaps():
+    a, t = evict_args(), torch.zeros(3, 2, 2, 64)
+    refused(kv.evict, {**a, "out": (t, t.view(torch.int32), ints(0, 0))},
+            "apart")
+    refused(kv.evict, {**a, "out": (a["pos"].view(torch.float32), a["pos"],
+                                    a["lens"])}, "apart")
+    refused(kv.evict, {**a, "next_pos": a["lens"],
+                       "out": (t, a["pos"], a["lens"])}, "apart")
+    refused(kv.evict, {**a, "next_pos": a["lens"],
+                       "out": (t, a["pos"], ints(0, 0))}, "must be on a GPU")
+
+
 def pages_arg(page=16, dim=64, slots=1, heads=1, kind=2, max_pages=4):
     return (0, 0, 1, 0, 0, max_pages, page, slots, heads, dim, kind, 0)
 
