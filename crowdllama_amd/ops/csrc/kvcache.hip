@@ -1552,8 +1552,16 @@ __device__ __forceinline__ int64_t row_at(const KvLayers& t, int layer, int b,
     return layer * t.layer_stride + b * t.slot_stride + h * t.head_stride;
 }
 
-// Who moves: the places of a row go by in blocks of one place a thread, in
-// order. Sums over the workgroup's NW waves, in theirs.
+// Each 16 lanes' sum, in all of them.
+__device__ __forceinline__ uint32_t sum_of_16(uint32_t x) {
+    x += __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);    // 1 0 3 2
+    x += __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);    // 2 3 0 1
+    x += __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, true);   // 8 mirrored
+    x += __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, true);   // 16 mirrored
+    return x;
+}
+
+// Sums over the workgroup's NW waves, in their order.
 struct WaveSums {
     uint32_t before, all;
 };
@@ -1575,21 +1583,24 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
 }
 
 // Pass 1, one workgroup of NT a row (layer, sequence, kv head): which places
-// stay, and who moves where. A thread holds the keys of KPT places
-// (place = k * NT + thread), or, with KPT = 0, computes them each time it
-// goes through the row. The keep-th largest key is found two bits at a time,
-// counting the keys at or above three candidates with ballots; it ends early
-// once exactly `keep` keys are at or above one. Then one walk in the order of
-// places numbers the free ones and those that come into them.
+// stay, and who moves where. Each wave has a stretch of the row, of which a
+// thread holds the keys of up to KPT places, or, with KPT = 0, computes them
+// each time it goes through them. The keep-th largest key is found two bits at
+// a time, counting the keys at or above three candidates with ballots; it ends
+// early once exactly `keep` keys are at or above one. Then each wave counts its
+// free places and those that come into them, and numbers them on from the
+// counts of the waves before it.
 //
-// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 33 us, 42
-// with KPT 32, 60 with 0), 32 up to 32768 (of 20000: 67 us, 185 with 0).
-// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 19 us, 98 with 1024
-// threads).
+// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 28 us, 30
+// with KPT 32, 65 with 0), 32 up to 32768 (128 of 20000: 55 us, 179 with 0).
+// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 19 us, 88 with 1024
+// threads; 192 of 2048: 17 us either way). Bound by the rounds: 11 to 16, each
+// with a barrier and LDS between the waves.
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
     constexpr int NW = NT / 64;
-    __shared__ uint32_t red[2][3][NW];
+    // a round's counts: [candidate][wave]; two, for rounds in turn
+    __shared__ uint32_t red[2][64];
     __shared__ uint32_t tot[NW];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1611,31 +1622,60 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
     if (!full && tid == 0) a.count[row] = -1;
     if (!full && !copies && !copied) return;
 
-    uint32_t held[KPT ? KPT : 1];
+    const int blocks = (len + NT - 1) / NT;
+    const int p0 = wave * blocks * 64 + lane;     // places p0 + k * 64
     auto key_at = [&](int p) {
         return kv_rank_key(mass[p], pos[p] >= late);
     };
+    uint32_t held[KPT ? KPT : 1];
+    int copied_to = 0;
     if constexpr (KPT > 0) {
+        // eight at a time without a branch between their loads
         #pragma unroll
-        for (int k = 0; k < KPT; k++) {
-            const int p = k * NT + tid;
-            held[k] = 0;
-            if (p < a.reach && (p < len || copies || copied)) {
-                const float m = mass[p];
-                const int32_t at = pos[p];
-                if (copies) mass_out[p] = m;
-                if (copied) pos_out[p] = at;
-                if (p < len) held[k] = kv_rank_key(m, at >= late);
+        for (int k0 = 0; k0 < KPT; k0 += 8) {
+            #pragma unroll
+            for (int k = k0; k < k0 + 8; k++) held[k] = 0;
+            if (k0 >= blocks) continue;
+            float m[8];
+            int32_t at[8];
+            #pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int p = min(p0 + (k0 + k) * 64, len - 1);
+                m[k] = mass[p];
+                at[k] = pos[p];
+            }
+            #pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int p = p0 + (k0 + k) * 64;
+                if (k0 + k < blocks && p < len) {
+                    if (copies) mass_out[p] = m[k];
+                    if (copied) pos_out[p] = at[k];
+                    held[k0 + k] = kv_rank_key(m[k], at[k] >= late);
+                }
             }
         }
-    } else {
-        for (int p = tid; p < a.reach; p += NT) {
-            if (copies) mass_out[p] = mass[p];
-            if (copied) pos_out[p] = pos[p];
-        }
+        copied_to = len;
+    }
+    for (int p = copied_to + tid; p < a.reach; p += NT) {
+        if (copies) mass_out[p] = mass[p];
+        if (copied) pos_out[p] = pos[p];
     }
     if (!full) return;
-    const int blocks = (len + NT - 1) / NT;
+    if (tid < 128) red[tid >> 6][lane] = 0;
+    __syncthreads();
+    // the wave's keys in order
+    auto each = [&](auto f) {
+        if constexpr (KPT > 0) {
+            #pragma unroll
+            for (int k = 0; k < KPT; k++)
+                if (k < blocks) f(p0 + k * 64, held[k]);
+        } else {
+            for (int k = 0; k < blocks; k++) {
+                const int p = p0 + k * 64;
+                f(p, p < len ? key_at(p) : 0u);
+            }
+        }
+    };
 
     // keys past the end are 0 and `least` is at least 1 where it decides:
     // a candidate always has a bit set
@@ -1645,31 +1685,27 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
         const uint32_t c1 = least | (1u << bit), c2 = least | (2u << bit),
                        c3 = least | (3u << bit);
         uint32_t n1 = 0, n2 = 0, n3 = 0;
-        auto count = [&](uint32_t key) {
+        each([&](int, uint32_t key) {
             n1 += __popcll(__ballot(key >= c1));
             n2 += __popcll(__ballot(key >= c2));
             n3 += __popcll(__ballot(key >= c3));
-        };
-        if constexpr (KPT > 0) {
-            #pragma unroll
-            for (int k = 0; k < KPT; k++)
-                if (k < blocks) count(held[k]);
-        } else {
-            for (int base = 0; base < len; base += NT)
-                count(base + tid < len ? key_at(base + tid) : 0);
-        }
-        if (lane == 0) {
-            red[turn][0][wave] = n1;
-            red[turn][1][wave] = n2;
-            red[turn][2][wave] = n3;
-        }
+        });
+        if (lane < 3)
+            red[turn][lane * 16 + wave] = lane == 0 ? n1 : lane == 1 ? n2 : n3;
         __syncthreads();
-        n1 = n2 = n3 = 0;
-        #pragma unroll
-        for (int w = 0; w < NW; w++) {
-            n1 += red[turn][0][w];
-            n2 += red[turn][1][w];
-            n3 += red[turn][2][w];
+        if constexpr (NW == 4) {
+            auto sum = [&](int c) {
+                const uint32_t* r = red[turn] + c * 16;
+                return r[0] + r[1] + r[2] + r[3];
+            };
+            n1 = sum(0);
+            n2 = sum(1);
+            n3 = sum(2);
+        } else {
+            const uint32_t sums = sum_of_16(red[turn][lane]);
+            n1 = __builtin_amdgcn_readlane(sums, 0);
+            n2 = __builtin_amdgcn_readlane(sums, 16);
+            n3 = __builtin_amdgcn_readlane(sums, 32);
         }
         const uint32_t keep = a.keep;
         const uint32_t n = n3 >= keep ? n3 : n2 >= keep ? n2 : n1;
@@ -1678,57 +1714,52 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
         else if (n1 >= keep) least = c1;
         exact = n == keep;
     }
-    // of the keys equal to `least`, the first `ties` stay
-    uint32_t ties = 0xFFFFFFFFu;
+    // of the keys equal to `least`, the first `ties` of the wave's stay
+    int ties = INT_MAX;
     if (!exact) {
-        uint32_t above = 0;
-        if constexpr (KPT > 0) {
-            #pragma unroll
-            for (int k = 0; k < KPT; k++)
-                if (k < blocks) above += __popcll(__ballot(held[k] > least));
-        } else {
-            for (int base = 0; base < len; base += NT)
-                above += __popcll(__ballot(base + tid < len &&
-                                           key_at(base + tid) > least));
-        }
-        ties = a.keep - wave_sums<NW>(above, tot, wave).all;
+        uint32_t above = 0, equal = 0;
+        each([&](int p, uint32_t key) {
+            above += __popcll(__ballot(key > least));
+            equal += __popcll(__ballot(p < len && key == least));
+        });
+        above = wave_sums<NW>(above, tot, wave).all;
+        ties = a.keep - (int)above
+            - (int)wave_sums<NW>(equal, tot, wave).before;
     }
 
+    const uint64_t below = (1ull << lane) - 1;
+    // f(place, whether it is free, whether it comes): ballots of the two
+    auto walk = [&](auto f) {
+        int left = ties;
+        each([&](int p, uint32_t key) {
+            bool stays = p < len && key >= least;
+            if (!exact) {
+                const uint64_t eqs = __ballot(p < len && key == least);
+                // negative where the waves before have them all
+                if (key == least) stays &= (int)__popcll(eqs & below) < left;
+                left -= (int)__popcll(eqs);
+            }
+            f(p, __ballot(p < min(len, a.keep) && !stays),
+              __ballot(stays && p >= a.keep));
+        });
+    };
+    uint32_t free = 0, come = 0;
+    walk([&](int, uint64_t fs, uint64_t cs) {
+        free += __popcll(fs);
+        come += __popcll(cs);
+    });
+    free = wave_sums<NW>(free, tot, wave).before;
+    const WaveSums comes = wave_sums<NW>(come, tot, wave);
+    come = comes.before;
     int32_t* dst = a.dst + (int64_t)row * a.most;
     int32_t* src = a.src + (int64_t)row * a.most;
-    const uint64_t below = (1ull << lane) - 1;
-    uint32_t equal = 0, free = 0, come = 0;        // so far, in all places
-    auto walk = [&](int base, uint32_t key) {
-        const int p = base + tid;
-        const bool here = p < len;
-        bool stays = here && key >= least;
-        if (!exact) {
-            const uint64_t eqs = __ballot(here && key == least);
-            const WaveSums s = wave_sums<NW>(__popcll(eqs), tot, wave);
-            if (here && key == least)
-                stays = equal + s.before + __popcll(eqs & below) < ties;
-            equal += s.all;
-        }
-        // both counts in one word: a block has at most NT of each
-        const uint64_t fs = __ballot(here && p < a.keep && !stays);
-        const uint64_t cs = __ballot(stays && p >= a.keep);
-        const WaveSums s =
-            wave_sums<NW>(__popcll(fs) | __popcll(cs) << 16, tot, wave);
-        if (here && p < a.keep && !stays)
-            dst[free + (s.before & 0xFFFF) + __popcll(fs & below)] = p;
-        if (stays && p >= a.keep)
-            src[come + (s.before >> 16) + __popcll(cs & below)] = p;
-        free += s.all & 0xFFFF;
-        come += s.all >> 16;
-    };
-    if constexpr (KPT > 0) {
-        #pragma unroll
-        for (int k = 0; k < KPT; k++)
-            if (k < blocks) walk(k * NT, held[k]);
-    } else {
-        for (int base = 0; base < len; base += NT)
-            walk(base, base + tid < len ? key_at(base + tid) : 0);
-    }
+    walk([&](int p, uint64_t fs, uint64_t cs) {
+        if (fs >> lane & 1) dst[free + __popcll(fs & below)] = p;
+        if (cs >> lane & 1) src[come + __popcll(cs & below)] = p;
+        free += __popcll(fs);
+        come += __popcll(cs);
+    });
+    come = comes.all;
     if (tid == 0) a.count[row] = come;
     __syncthreads();
     for (uint32_t i = tid; i < come; i += NT) {
