@@ -122,6 +122,27 @@ def test_without_a_full_cache_nothing_changes(core, gguf):
     assert a.kv_lens() == b.kv_lens() == [30]
 
 
+def test_a_cache_longer_than_one_workgroup_takes(core, gguf):
+    """The attention's form for long rows: the logits of the engine without
+    eviction, and weights that sum to one for each query head of each token."""
+    a = engine(core, gguf, keep=1000, max_seq=1100)
+    b = engine(core, gguf, keep=0, max_seq=1100)
+    ids = np.array([prompt(700)], dtype=np.int32)
+    for e in (a, b):
+        e.prefill(ids)
+    for _ in range(10):
+        x, y = np.asarray(a.logits(0)), np.asarray(b.logits(0))
+        assert np.abs(x - y).max() < LOGITS * np.abs(y).max()
+        b.set_cur_token(0, a.cur_token(0))
+        a.decode(1)
+        b.decode(1)
+    sums = [a.kv_places(layer, 0)[1].sum(-1) for layer in (0, 1)]
+    # the last token's own weights count too; 710 sums of up to 710 weights
+    ref = reference(gguf)
+    group = ref.heads // ref.kv_heads
+    np.testing.assert_allclose(sums, 710 * group, rtol=1e-3)
+
+
 @pytest.mark.parametrize("batch", [2, 5])
 def test_slots_evict_on_their_own(core, gguf, batch):
     """Slots of other lengths, one parked on the way: each is as it would be
