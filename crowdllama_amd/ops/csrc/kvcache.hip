@@ -1552,15 +1552,6 @@ __device__ __forceinline__ int64_t row_at(const KvLayers& t, int layer, int b,
     return layer * t.layer_stride + b * t.slot_stride + h * t.head_stride;
 }
 
-// Each 16 lanes' sum, in all of them.
-__device__ __forceinline__ uint32_t sum_of_16(uint32_t x) {
-    x += __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true);    // 1 0 3 2
-    x += __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true);    // 2 3 0 1
-    x += __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, true);   // 8 mirrored
-    x += __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, true);   // 16 mirrored
-    return x;
-}
-
 // Sums over the workgroup's NW waves, in their order.
 struct WaveSums {
     uint32_t before, all;
@@ -1585,22 +1576,22 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
 // Pass 1, one workgroup of NT a row (layer, sequence, kv head): which places
 // stay, and who moves where. Each wave has a stretch of the row, of which a
 // thread holds the keys of up to KPT places, or, with KPT = 0, computes them
-// each time it goes through them. The keep-th largest key is found two bits at
-// a time, counting the keys at or above three candidates with ballots; it ends
-// early once exactly `keep` keys are at or above one. Then each wave counts its
-// free places and those that come into them, and numbers them on from the
-// counts of the waves before it.
+// each time it goes through them. The keep-th largest key is found eight bits
+// at a time, by counting the digits of the keys that begin as it does in LDS;
+// that ends early once exactly `keep` keys are at or above a digit. Then each
+// wave counts its free places and those that come into them, and numbers them
+// on from the counts of the waves before it.
 //
-// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 28 us, 30
-// with KPT 32, 65 with 0), 32 up to 32768 (128 of 20000: 55 us, 179 with 0).
-// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 19 us, 88 with 1024
-// threads; 192 of 2048: 17 us either way). Bound by the rounds: 11 to 16, each
-// with a barrier and LDS between the waves.
+// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 22 us, 24
+// with KPT 32, 38 with 0), 32 up to 32768 (128 of 20000: 43 us, 87 with 0).
+// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 17 us, 68 with 1024
+// threads; 192 of 2048: 13.5 us either way). Bound by the counting: keys of one
+// exponent meet in few digits (the first one's lanes are added at once). Two
+// bits a round, by ballots over three candidates, takes 28 us for 256 x 8192.
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
     constexpr int NW = NT / 64;
-    // a round's counts: [candidate][wave]; two, for rounds in turn
-    __shared__ uint32_t red[2][64];
+    __shared__ __align__(16) uint32_t digits[4][256];
     __shared__ uint32_t tot[NW];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1661,7 +1652,7 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
         if (copied) pos_out[p] = pos[p];
     }
     if (!full) return;
-    if (tid < 128) red[tid >> 6][lane] = 0;
+    for (int i = tid; i < 4 * 256; i += NT) digits[i >> 8][i & 255] = 0;
     __syncthreads();
     // the wave's keys in order
     auto each = [&](auto f) {
@@ -1677,54 +1668,63 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
         }
     };
 
-    // keys past the end are 0 and `least` is at least 1 where it decides:
-    // a candidate always has a bit set
-    uint32_t least = 0;
+    // `want` of the keys that begin as `least` does are still to be found. A
+    // key past the end is 0, as a NaN's: as there are more than `keep` places,
+    // counting it too makes no group of the lowest keys exact
+    uint32_t least = 0, want = a.keep;
     bool exact = false;
-    for (int bit = 30, turn = 0; bit >= 0 && !exact; bit -= 2, turn ^= 1) {
-        const uint32_t c1 = least | (1u << bit), c2 = least | (2u << bit),
-                       c3 = least | (3u << bit);
-        uint32_t n1 = 0, n2 = 0, n3 = 0;
+    #pragma unroll 1
+    for (int turn = 0; turn < 4 && !exact; turn++) {
+        const int shift = 24 - 8 * turn;
         each([&](int, uint32_t key) {
-            n1 += __popcll(__ballot(key >= c1));
-            n2 += __popcll(__ballot(key >= c2));
-            n3 += __popcll(__ballot(key >= c3));
+            // 64 bits: in the first turn nothing is left to compare
+            const bool of = !((uint64_t)(key ^ least) >> (shift + 8));
+            const uint32_t digit = key >> shift & 255;
+            const uint64_t all = __ballot(of);
+            if (!all) return;
+            // the first one's digit, which many may share, is added at once
+            const int first = __builtin_ctzll(all);
+            const bool same =
+                digit == (uint32_t)__builtin_amdgcn_readlane(digit, first);
+            const uint64_t sames = __ballot(of && same);
+            if (of && (!same || lane == first))
+                atomicAdd(&digits[turn][digit],
+                          same ? (uint32_t)__popcll(sames) : 1u);
         });
-        if (lane < 3)
-            red[turn][lane * 16 + wave] = lane == 0 ? n1 : lane == 1 ? n2 : n3;
         __syncthreads();
-        if constexpr (NW == 4) {
-            auto sum = [&](int c) {
-                const uint32_t* r = red[turn] + c * 16;
-                return r[0] + r[1] + r[2] + r[3];
-            };
-            n1 = sum(0);
-            n2 = sum(1);
-            n3 = sum(2);
-        } else {
-            const uint32_t sums = sum_of_16(red[turn][lane]);
-            n1 = __builtin_amdgcn_readlane(sums, 0);
-            n2 = __builtin_amdgcn_readlane(sums, 16);
-            n3 = __builtin_amdgcn_readlane(sums, 32);
+        // the digit at which the count from the highest down reaches `want`:
+        // four digits a lane
+        const u32x4 n =
+            *reinterpret_cast<const u32x4*>(&digits[turn][lane * 4]);
+        uint32_t from = n.x + n.y + n.z + n.w;
+        #pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t x = __shfl_down(from, m, 64);
+            if (lane + m < 64) from += x;
         }
-        const uint32_t keep = a.keep;
-        const uint32_t n = n3 >= keep ? n3 : n2 >= keep ? n2 : n1;
-        if (n3 >= keep) least = c3;
-        else if (n2 >= keep) least = c2;
-        else if (n1 >= keep) least = c1;
-        exact = n == keep;
+        const int at = 63 - __builtin_clzll(__ballot(from >= want));
+        const uint32_t n3 = __builtin_amdgcn_readlane(n.w, at),
+                       n2 = __builtin_amdgcn_readlane(n.z, at),
+                       n1 = __builtin_amdgcn_readlane(n.y, at),
+                       n0 = __builtin_amdgcn_readlane(n.x, at);
+        uint32_t left = want - (__builtin_amdgcn_readlane(from, at)
+                                - n0 - n1 - n2 - n3);
+        uint32_t digit = at * 4 + 3, count = n3;
+        if (left > count) { left -= count; digit--; count = n2; }
+        if (left > count) { left -= count; digit--; count = n1; }
+        if (left > count) { left -= count; digit--; count = n0; }
+        least |= digit << shift;
+        want = left;
+        exact = count == left;
     }
     // of the keys equal to `least`, the first `ties` of the wave's stay
     int ties = INT_MAX;
     if (!exact) {
-        uint32_t above = 0, equal = 0;
+        uint32_t equal = 0;
         each([&](int p, uint32_t key) {
-            above += __popcll(__ballot(key > least));
             equal += __popcll(__ballot(p < len && key == least));
         });
-        above = wave_sums<NW>(above, tot, wave).all;
-        ties = a.keep - (int)above
-            - (int)wave_sums<NW>(equal, tot, wave).before;
+        ties = (int)want - (int)wave_sums<NW>(equal, tot, wave).before;
     }
 
     const uint64_t below = (1ull << lane) - 1;

@@ -752,6 +752,26 @@ def test_evict_ties_and_strange_masses():
     check_evict(pool, table, lens, [64], mass, pos, 60, 7, None)
 
 
+@pytest.mark.parametrize("n", [300, 3000, 33000])
+@pytest.mark.parametrize("kind", ["one", "two", "late", "nan", "near"])
+def test_evict_rows_of_equals(n, kind):
+    """Ties over several waves, and keys that differ in their last bits."""
+    lens = [n, n - 65]
+    pool, table, mass, pos = make_evict(45, lens, 1, 2, 64, 64,
+                                        torch.bfloat16)
+    g = torch.Generator().manual_seed(5)
+    pick = torch.rand(mass.shape, generator=g)
+    late = [0, 0] if kind == "late" else [1 << 30] * 2
+    if kind == "nan":
+        mass[pick < .8] = math.nan
+    elif kind == "near":
+        mass = 1 + torch.floor(pick * 300) * 2.0 ** -23
+    else:
+        mass = torch.full_like(mass, .5) + (pick < .4) * (kind == "two")
+    for keep in (n // 3, n - 70):
+        check_evict(pool, table, lens, late, mass, pos, keep, 5, None)
+
+
 def test_evict_limit():
     lens = [50, 51, 30]
     pool, table, mass, pos = make_evict(43, lens, 2, 1, 64, 16,
