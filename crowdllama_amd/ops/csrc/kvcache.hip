@@ -1322,12 +1322,13 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4, head = blockIdx.y;
     const int G = a.group.d;
-    // late chunks are seen by more places than early ones, in steps with the
-    // blocks: turned by an arbitrary amount from block to block, so that no
-    // XCD (every eighth workgroup) gets the late ones
+    // chunks differ in their work (late ones are seen by more places, short
+    // sequences have less): turned by one from block to block and from head to
+    // head, so that no XCD (every eighth workgroup) gets the long ones (4 x 282
+    // float32 rows: 48 us, 61 turned by block alone, 62 by an arbitrary amount a
+    // block; 7 x 251 rows of 32 kv heads 168, 178 and 170, 275 not turned)
     const int block = blockIdx.x / a.chunks;
-    const int at = (blockIdx.x + ((uint32_t)block * 0x9E3779B1u >> 24))
-        % a.chunks;
+    const int at = (blockIdx.x + block + head) % a.chunks;
     Seq s{};
     const RowBlock x = row_block(a, a.chunk, at, s);
     if (x.id < 0) return;
