@@ -874,7 +874,7 @@ Div div_by(int d) {
 
 // Groups of 16 places that a wave of the second pass holds, where there is
 // work for many. Three leave room for a third wave a SIMD with heads of 128 and
-// one piece (8192 rows of 32 heads: 350 us, 422 with four); more pieces have
+// one piece (8192 rows of 32 heads: 345 us, 422 with four); more pieces have
 // more to do for each row that is read (3 x 500 rows over 16000 places: 307 us,
 // 355 with three).
 constexpr int obs_groups(bool one_piece, int dim) {
@@ -1001,7 +1001,7 @@ __device__ __forceinline__ void store_sum(const ObserveArgs& a, const Seq& s,
 //
 // A score costs a multiplication, an exponential and an addition: 16 + 32 + 16
 // cycles of the SIMD for 4 x 64 of them, beside 64 of matrix products, which
-// run at the same time in part. 365 us for 8192 rows of 32 heads (275 GFLOP).
+// run at the same time in part. 355 us for 8192 rows of 32 heads (275 GFLOP).
 //
 // Three waves a SIMD for one piece (375 us for 8192 rows of 32 heads, 442 with
 // two), two for three (249 us for 3 x 500 rows over 16000 places, 290 with
