@@ -18,7 +18,7 @@ from dataclasses import dataclass, field
 from ..config import Config
 from ..keys import load_identity
 from ..logutil import new_app_logger
-from .wire import PROTO_RENDEZVOUS, secure_accept
+from .wire import PROTO_RENDEZVOUS, end_tasks, secure_accept
 
 
 @dataclass
@@ -70,14 +70,7 @@ class DHTServer:
         return self.port
 
     async def stop(self):
-        for t in self._tasks:
-            t.cancel()
-        for t in self._tasks:
-            try:
-                await t
-            except (asyncio.CancelledError, Exception):
-                pass
-        self._tasks.clear()
+        await end_tasks(self._tasks)
         if self._server:
             self._server.close()
         # asyncio's Server.close() only stops ACCEPTING; live connection

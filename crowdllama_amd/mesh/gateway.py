@@ -21,7 +21,7 @@ from ..logutil import new_app_logger
 from . import pb
 from .discovery import parse_addr
 from .peer import Peer
-from .wire import PROTO_INFERENCE, secure_open
+from .wire import PROTO_INFERENCE, end_tasks, secure_open
 
 
 class Gateway:
@@ -62,14 +62,7 @@ class Gateway:
             for ss in pool:
                 ss.close()
         self._conns.clear()
-        for t in self._tasks:
-            t.cancel()
-        for t in self._tasks:
-            try:
-                await t
-            except (asyncio.CancelledError, Exception):
-                pass
-        self._tasks.clear()
+        await end_tasks(self._tasks)
         if self._runner:
             await self._runner.cleanup()
             self._runner = None

@@ -24,7 +24,7 @@ from .discovery import Discovery
 from .peermanager import PeerManager
 from .resource import Resource
 from .wire import (NAMESPACE, PROTO_INFERENCE, PROTO_METADATA,
-                   PROTO_RENDEZVOUS, secure_accept)
+                   PROTO_RENDEZVOUS, end_tasks, secure_accept)
 
 
 class Peer:
@@ -91,14 +91,7 @@ class Peer:
                       "consumer", self.port, self.cfg.bootstrap_peers)
 
     async def stop(self) -> None:
-        for t in self._tasks:
-            t.cancel()
-        for t in self._tasks:
-            try:
-                await t
-            except (asyncio.CancelledError, Exception):
-                pass
-        self._tasks.clear()
+        await end_tasks(self._tasks)
         await self.peer_manager.stop()
         await self.discovery.close()
         if self._dht is not None:

@@ -17,6 +17,7 @@ from dataclasses import dataclass, field
 from ..config import Intervals
 from .discovery import Discovery
 from .resource import Resource
+from .wire import end_tasks
 
 
 @dataclass
@@ -142,14 +143,7 @@ class PeerManager:
         ]
 
     async def stop(self) -> None:
-        for t in self._tasks:
-            t.cancel()
-        for t in self._tasks:
-            try:
-                await t
-            except (asyncio.CancelledError, Exception):
-                pass
-        self._tasks.clear()
+        await end_tasks(self._tasks)
 
     async def _discovery_loop(self) -> None:
         while True:

@@ -26,6 +26,21 @@ class WireError(Exception):
     pass
 
 
+async def end_tasks(tasks: list[asyncio.Task]) -> None:
+    """Cancel background tasks and wait for their end. One cancellation is not
+    enough: asyncio.wait_for drops it (up to Python 3.11) if what it waits for
+    is done at the same time, and the task's loop goes on."""
+    left = set(tasks)
+    while left:
+        for t in left:
+            t.cancel()
+        done, left = await asyncio.wait(left, timeout=0.5)
+        for t in done:
+            if not t.cancelled():
+                t.exception()       # seen: an error here ends nothing else
+    tasks.clear()
+
+
 async def write_frame(writer: asyncio.StreamWriter, payload: bytes) -> None:
     if len(payload) > MAX_FRAME:
         raise WireError(f"frame too large: {len(payload)}")
