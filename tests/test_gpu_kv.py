@@ -972,3 +972,56 @@ def test_captured_and_replayed():
         for k in a:
             assert torch.equal(a[k], b[k]), (i, k)
     assert int(a["lens"].max()) <= 60 and a["now"].tolist() == [90, 80]
+
+
+@pytest.mark.parametrize("n,m", [(1500, 700), (700, 30)])
+def test_captured_with_workspaces(n, m):
+    """attend in parts, observe in parts and chunks, and evict of long rows, in
+    two graphs whose replays take turns, with lengths that change between them;
+    each replay is what eager calls give, bit for bit."""
+    from crowdllama_amd.ops import kv
+    B, H, heads, D = 3, 8, 4, 64
+    lens = [[n, 20, n // 2], [n // 3, n, 1], [0, n - 1, n]]
+    starts = [[0, m, m + 20, 2 * m], [0, 3, m, m + 1], [0, 0, m, 2 * m]]
+    _, pool, table = make(62, [n] * B, H, heads, D, 64, TYPES[0], layers=1,
+                          strange=False)
+    table = longer(table, 64)
+    cap = table.shape[1] * 64
+    g = torch.Generator().manual_seed(63)
+    mass = torch.rand(1, B, heads, cap, generator=g)
+    pos = torch.arange(cap, dtype=torch.int32).expand(1, B, heads, cap)
+    one = torch.randn(B, H, D, generator=g).cuda()
+    q = torch.randn(2 * m, H, D, generator=g).cuda()
+    dt = table.cuda()
+
+    def fresh(i):
+        return dict(pool=pool.cuda(), mass=mass.cuda(), lens=ints(lens[i]),
+                    starts=ints(starts[i]), pos=pos.contiguous().cuda(),
+                    out=torch.zeros(B, H, D, device="cuda"))
+
+    def step(s):
+        kv.observe(q, s["pool"][:, 0], dt, s["lens"], s["mass"][0],
+                   starts=s["starts"])
+        kv.attend(one, s["pool"][:, 0], dt, s["lens"], mass=s["mass"][0],
+                  out=s["out"])
+        kv.evict(s["pool"], dt, s["lens"], s["lens"] + 5, s["mass"], s["pos"],
+                 keep=n // 2 - 3, recent=9)
+
+    step(fresh(0))                 # loaded before the capture
+    held = [fresh(0), fresh(1)]
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    for graph, s in zip(graphs, held):
+        with torch.cuda.graph(graph):
+            step(s)
+    for i in (0, 1, 2, 0):
+        for s, new in zip(held, (fresh(i), fresh((i + 1) % 3))):
+            for k in s:
+                s[k].copy_(new[k])
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for s, want in zip(held, (fresh(i), fresh((i + 1) % 3))):
+            step(want)
+            for k in s:
+                assert torch.equal(s[k], want[k]), k
