@@ -1,0 +1,68 @@
+"""The paged cache's operators at the edges of their arithmetic and of what a
+call may look like, against the definitions in 64 bits.
+
+Where a query is one 1 among zeros, its scores are one element of each key and
+exact but for the scale: a product of three float32 factors, 3 half steps.
+"""
+import math
+
+import pytest
+import torch
+
+import kv_oracle as oracle
+from test_gpu_kv import IDS, TYPES, check_attend, ints, longer, make
+
+pytestmark = pytest.mark.gpu
+
+
+def one_hot(B, heads, dim, dtype):
+    """Queries whose scores are element 0 of the keys times the scale."""
+    q = torch.zeros(B, heads, dim, dtype=dtype)
+    q[..., 0] = 1
+    return q
+
+
+def at(pool, table, b, p):
+    """Place p of sequence b in the pool: [kv heads, 2, dim]."""
+    page = pool.shape[-2]
+    return pool[table[b, p // page], :, :, p % page]
+
+
+both_forms = pytest.mark.parametrize("parts", [False, True],
+                                     ids=["row", "parts"])
+
+
+@both_forms
+def test_attend_bfloat16_is_rounded_once(parts):
+    """Each output is the bfloat16 next to a value that is off by float32's
+    roundings alone.
+
+    All weights but one lose 0.9 x 2^-15 of themselves if they are cut to two
+    pieces of 8 bits; the one has no value. In half steps of
+    float32 (2^-24): with scores of at most 1 (their factors 3, their
+    difference from the maximum 1 more: 4 ln 2 = 3) and an exponential that is
+    off by 2, a weight is off by 5; so is their sum, with 10 additions of its
+    own; the products' sum has at most 3 x 32, and the joins and the division
+    at most 10. Values of one sign do not cancel.
+    """
+    from crowdllama_amd.ops import kv
+    lens, heads, dim = [32, 31, 17, 9, 30, 25, 5, 28], 16, 128
+    _, pool, table = make(70, lens, heads, heads, dim, 16, TYPES[1],
+                          strange=False)
+    q = one_hot(len(lens), heads, dim, torch.bfloat16)
+    pool[:, :, 0, :, 0] = -1.
+    pool[:, :, 1] = 1 + pool[:, :, 1].abs() % 1
+    for b in range(len(lens)):
+        at(pool, table, b, 2)[:, 0, 0] = 0.
+        at(pool, table, b, 2)[:, 1] = 0.
+    scale = -math.log(.5 * (1 + 2.0 ** -8 + .9 * 2.0 ** -15))
+    if parts:
+        table = longer(table, 16)
+    got = kv.attend(q.cuda(), pool.cuda(), table.cuda(), ints(lens),
+                    scale=scale)
+    want, _, big, _ = oracle.attend(q, pool, table, lens, scale)
+    e = (5 + 5 + 10 + 96 + 10) * 2.0 ** -24 * big
+    low, high = (want - e).bfloat16(), (want + e).bfloat16()
+    got = got.cpu()
+    assert ((low <= got) & (got <= high)).all(), \
+        int(((low > got) | (got > high)).sum())
