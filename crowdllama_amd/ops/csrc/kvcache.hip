@@ -42,6 +42,8 @@ __device__ __forceinline__ To bits(const From& x) {
 // ------------------------------------------------------------- 16-bit types
 
 struct Bf16 {
+    // attention weights are taken relative to 2^-AHEAD of the largest
+    static constexpr float AHEAD = 0.f;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
             bits<bf16x8>(a), bits<bf16x8>(b), c, 0, 0, 0);
@@ -65,6 +67,9 @@ struct Bf16 {
 };
 
 struct F16 {
+    // A weight of 1 would leave float16 only 24 bits of range below it: weights
+    // go up to 2^14 (the type holds 2^16), so that 2^-39 of the largest counts.
+    static constexpr float AHEAD = 14.f;
     static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(
             bits<f16x8>(a), bits<f16x8>(b), c, 0, 0, 0);
@@ -77,8 +82,8 @@ struct F16 {
         const f16x2 v = bits<f16x2>(w);
         return f32x2{(float)v.x, (float)v.y};
     }
-    // As above, 11 bits a call; for values of [0, 1] (attention weights),
-    // whose remainder float16 holds to 2^-25 of the largest.
+    // As above, 11 bits a call, down to 2^-25; for attention weights, of
+    // [0, 2^14].
     static __device__ __forceinline__ uint32_t piece(float& x, float& y) {
         const f16x2 v = {(_Float16)x, (_Float16)y};
         x -= (float)v.x;
@@ -490,8 +495,9 @@ __device__ __forceinline__ void load_tile(const uint16_t* r0,
     }
 }
 
-// What a lane has of its query head: the maximum of the wave's places, the sum
-// of its own places' weights, and its outputs.
+// What a lane has of its query head: the reference m of its weights 2^(score -
+// m), which is AHEAD below the maximum of the wave's places; the sum of its own
+// places' weights; and its outputs.
 template <int D>
 struct Softmax {
     float m = -INFINITY, l = 0.f;
@@ -550,7 +556,7 @@ __device__ __forceinline__ void use_tile(Tile<D>& t, bool t0, bool t1, int p0,
                                   s[u * 4 + 3]});
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                       fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    top = wave_xor_max(wave_xor_max(top, 16), 32);
+    top = wave_xor_max(wave_xor_max(top, 16), 32) - C::AHEAD;
     if (__any(top > m)) {
         const float now = fmaxf(m, top);
         const float f = exp2_fast(m - now);   // 0 from -inf

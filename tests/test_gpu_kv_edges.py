@@ -66,3 +66,22 @@ def test_attend_bfloat16_is_rounded_once(parts):
     got = got.cpu()
     assert ((low <= got) & (got <= high)).all(), \
         int(((low > got) | (got > high)).sum())
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("far", [16, 20, 24, 26, 30])
+@both_forms
+def test_attend_far_below_one_place(types, far, parts):
+    """One place has nearly all the weight and no value (an attention sink);
+    the outputs are those of the others, each 2^-far of it."""
+    lens = [700, 300, 40]
+    q, pool, table = make(71, lens, 4, 2, 64, 16, types, strange=False)
+    q = one_hot(3, 4, 64, types[0])
+    pool[:, :, 0, :, 0] = 0.
+    pool[:, :, 1] = 1 + pool[:, :, 1].abs() % 1
+    for b, n in enumerate(lens):
+        sink = at(pool, table, b, n // 3)
+        sink[:, 0, 0], sink[:, 1] = far, 0.
+    if parts:
+        table = longer(table, 16)
+    check_attend(q, pool, table, lens, scale=math.log(2.))
