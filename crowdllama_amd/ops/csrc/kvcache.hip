@@ -55,13 +55,15 @@ struct Bf16 {
     static __device__ __forceinline__ f32x2 unpack(uint32_t w) {
         return f32x2{bits<float>(w << 16), bits<float>(w & 0xFFFF0000u)};
     }
-    // The leading 8 bits of x and y as a packed pair; x and y become what
-    // is left, without error. Three calls take all 24 bits.
+    // The leading 8 bits of x and y as a packed pair; x and y become what is
+    // left. Three calls take all 24 bits. What is left gets 2^-30 of x more: a
+    // piece is then never 0, and of x's sign, so that it makes infinity of an
+    // infinite operand as x does, and not NaN.
     static __device__ __forceinline__ uint32_t piece(float& x, float& y) {
         const uint32_t ux = bits<uint32_t>(x) & 0xFFFF0000u;
         const uint32_t uy = bits<uint32_t>(y) & 0xFFFF0000u;
-        x -= bits<float>(ux);
-        y -= bits<float>(uy);
+        x = fmaf(x, 0x1p-30f, x - bits<float>(ux));
+        y = fmaf(y, 0x1p-30f, y - bits<float>(uy));
         return (ux >> 16) | uy;
     }
 };
@@ -82,12 +84,13 @@ struct F16 {
         const f16x2 v = bits<f16x2>(w);
         return f32x2{(float)v.x, (float)v.y};
     }
-    // As above, 11 bits a call, down to 2^-25; for attention weights, of
-    // [0, 2^14].
+    // As above, 11 bits a call, for attention weights: of [0, 2^14], in two
+    // pieces. The second is at least 2^-24, the type's smallest (2^-38 of the
+    // largest weight); weights below that are 0 or 2^-24 in all.
     static __device__ __forceinline__ uint32_t piece(float& x, float& y) {
-        const f16x2 v = {(_Float16)x, (_Float16)y};
-        x -= (float)v.x;
-        y -= (float)v.y;
+        const auto v = __builtin_amdgcn_cvt_pkrtz(x, y);
+        x = fmaxf(x - (float)v.x, fminf(x, 0x1p-24f));
+        y = fmaxf(y - (float)v.y, fminf(y, 0x1p-24f));
         return bits<uint32_t>(v);
     }
 };
@@ -579,7 +582,8 @@ __device__ __forceinline__ void use_tile(Tile<D>& t, bool t0, bool t1, int p0,
     for (int y = 0; y < NP; y++)
         #pragma unroll
         for (int i = 0; i < 4; i++)
-            pf[y][i] = C::piece(w[2 * i], w[2 * i + 1]);
+            pf[y][i] = y + 1 < NP ? C::piece(w[2 * i], w[2 * i + 1])
+                                  : C::pack(w[2 * i], w[2 * i + 1]);
     #pragma unroll
     for (int e = 0; e < EL; e++) {
         u32x4 vf;

@@ -85,3 +85,70 @@ def test_attend_far_below_one_place(types, far, parts):
     if parts:
         table = longer(table, 16)
     check_attend(q, pool, table, lens, scale=math.log(2.))
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@both_forms
+def test_attend_infinite_values(types, parts):
+    """Infinite wherever a weight meets an infinite value of one sign, also at
+    the place with the largest weight, whose 1 is one 16-bit piece."""
+    from crowdllama_amd.ops import kv
+    lens = [1, 1, 50, 50, 300, 17]
+    q, pool, table = make(72, lens, 4, 2, 64, 16, types, strange=False)
+    at(pool, table, 0, 0)[:, 1, 3] = math.inf
+    at(pool, table, 1, 0)[0, 1, 5] = -math.inf
+    for p in range(50):                        # equal weights: all of them 1
+        at(pool, table, 2, p)[:, 0] = at(pool, table, 2, 0)[:, 0]
+    at(pool, table, 2, 20)[:, 1, 7] = math.inf
+    at(pool, table, 3, 11)[1, 1, 9] = -math.inf
+    at(pool, table, 4, 250)[:, 1, ::2] = math.inf
+    at(pool, table, 4, 3)[:, 1, ::2] = math.inf
+    at(pool, table, 5, 2)[:, 1, 1] = math.inf   # both signs: NaN
+    at(pool, table, 5, 16)[:, 1, 1] = -math.inf
+    if parts:
+        table = longer(table, 16)
+    mass = torch.zeros(6, 2, table.shape[1] * 16, device="cuda")
+    got = kv.attend(q.cuda(), pool.cuda(), table.cuda(), ints(lens),
+                    mass=mass).double().cpu()
+    want, add, _, _ = oracle.attend(q, pool, table, lens, 64 ** -.5)
+    assert want.isinf().sum() == 4 * 1 + 2 * 1 + 4 * 1 + 2 * 1 + 4 * 32
+    assert torch.equal(got.isnan(), want.isnan()) and want.isnan().any()
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    fine = want.isfinite()
+    # half a step of the coarsest type, of values below 4
+    assert torch.allclose(got[fine], want[fine], rtol=0, atol=2.0 ** -6)
+    assert torch.allclose(mass.double().cpu(), add, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@both_forms
+def test_infinite_keys(types, parts):
+    """A score of -inf is a weight of 0, whatever the pieces of the query;
+    what attend adds to the mass, observe adds too."""
+    from crowdllama_amd.ops import kv
+    lens = [40, 300]
+    q, pool, table = make(73, lens, 4, 2, 64, 16, types, strange=False)
+    q[..., 5] = -1.                  # its second and third pieces are 0
+    q[..., 6] = 0.75
+    at(pool, table, 0, 7)[:, 0, 5] = math.inf
+    at(pool, table, 1, 299)[1, 0, 6] = -math.inf
+    at(pool, table, 1, 120)[0, 0, 5:7] = torch.tensor([math.inf, -math.inf])
+    # the definition, with the largest negative number for the infinity
+    low = pool.double().clamp(-1e9, 1e9)
+    if parts:
+        table = longer(table, 16)
+    args = q.cuda(), pool.cuda(), table.cuda(), ints(lens)
+    mass = torch.zeros(2, 2, table.shape[1] * 16, device="cuda")
+    got = kv.attend(*args, mass=mass).double().cpu()
+    want, add, big, _ = oracle.attend(q, low, table, lens, 64 ** -.5)
+    assert (add[0, :, 7] == 0).all() and add[1, 1, 299] == 0
+    assert torch.allclose(got, want, rtol=0, atol=2.0 ** -6)
+    assert torch.allclose(mass.double().cpu(), add, rtol=1e-4, atol=1e-6)
+    for rows in (1, 3):
+        many = q.repeat_interleave(rows, 0)
+        again = torch.zeros_like(mass)
+        kv.observe(many.cuda(), *args[1:], again,
+                   starts=ints([0, rows, 2 * rows]))
+        add, _ = oracle.observe(many, low, table, lens, [0, rows, 2 * rows],
+                                64 ** -.5)
+        assert torch.allclose(again.double().cpu(), add, rtol=1e-4, atol=1e-6)
