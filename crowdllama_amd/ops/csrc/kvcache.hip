@@ -905,7 +905,7 @@ struct ObserveArgs {
     // the batch, and places in blocks of `block`
     int32_t chunk, chunks, block;
     float* sums;       // [parts][kv heads][rows][G][2]: maximum, sum
-    float* lse;        // [kv heads][rows][G]: log2 of the sum of 2^scores
+    float* norm;       // [kv heads][rows][G][2]: what a row's weights are of
     float* partial;    // [chunks][kv heads][ld]
     int64_t ld;
 };
@@ -939,9 +939,15 @@ __device__ __forceinline__ u32x4 lds_unit(const uint16_t* rows, int r,
     return *reinterpret_cast<const u32x4*>(rows + r * LDS_ROW<D> + unit * 8);
 }
 
-__device__ __forceinline__ float row_lse(float m, float l) {
-    // a row that sees nothing gives nothing: 2^(s - inf)
-    return l == 0.f ? INFINITY : m + __log2f(l);
+// A row whose weights 2^(s - m) sum to l: each is 2^(s - x) * y of it, x a whole
+// number, so that the exponent is as exact as s is near to it. (One number,
+// m + log2(l), would be rounded to 2^-20 for a sum of thousands, and so would
+// all of a row's weights, the same way.) A row that sees nothing gives nothing:
+// x is infinite.
+__device__ __forceinline__ f32x2 row_norm(float m, float l) {
+    if (l == 0.f) return f32x2{INFINITY, 0.f};
+    const float x = rintf(m + __log2f(l));
+    return f32x2{x, exp2_fast(x - m) / l};
 }
 
 // The x-th block of `rows` rows, counted over the batch: which sequence's it
@@ -995,7 +1001,7 @@ __device__ __forceinline__ void store_sum(const ObserveArgs& a, const Seq& s,
                                           float sum) {
     const int64_t at = ((int64_t)head * a.rows + s.t0) * a.group.d + r;
     if (a.parts == 1) {
-        a.lse[at] = row_lse(top, sum);
+        *reinterpret_cast<f32x2*>(a.norm + at * 2) = row_norm(top, sum);
     } else {
         float* d = a.sums + ((int64_t)blockIdx.z * a.q_heads * a.rows + at) * 2;
         // a part without a weight must not set the others' reference
@@ -1312,7 +1318,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_join(ObserveArgs a) {
     __syncthreads();
     if (y || at >= all) return;
     for (int i = 1; i < 8; i++) join(s_m[i][x], s_l[i][x]);
-    a.lse[at] = row_lse(m, l);
+    *reinterpret_cast<f32x2*>(a.norm + at * 2) = row_norm(m, l);
 }
 
 // Pass 2, grid (place blocks x chunks, kv heads): 16 * PW places a
@@ -1326,7 +1332,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     constexpr int QT = NQ == 1 ? 64 : 32, UNITS = QT * D / 8;
     constexpr int PER = (UNITS + 255) / 256;
     __shared__ __align__(16) uint16_t s_q[2][NQ][QT * LDS_ROW<D>];
-    __shared__ float s_lse[2][QT];
+    __shared__ f32x2 s_norm[2][QT];
     __shared__ int s_seen[2][QT];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1389,8 +1395,9 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
                + (int64_t)(head * G + h_of[x]) * a.q.head_stride
                + u % (D / 8) * 8) * size;
     }
-    const float* from_lse = a.lse + ((int64_t)head * a.rows + s.t0) * G;
-    float next_lse = INFINITY;
+    const f32x2* from_norm = reinterpret_cast<const f32x2*>(a.norm)
+        + ((int64_t)head * a.rows + s.t0) * G;
+    f32x2 next_norm = {INFINITY, 0.f};
     int next_seen = 0;
     auto fetch = [&](int r0) {
         #pragma unroll
@@ -1414,7 +1421,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
         }
         if (tid < QT) {
             const int r = r0 + tid;
-            next_lse = r < R ? from_lse[r] : INFINITY;
+            next_norm = r < R ? from_norm[r] : f32x2{INFINITY, 0.f};
             next_seen = r < R ? s.len - s.m + a.group.of(r) + 1 : 0;
         }
     };
@@ -1442,12 +1449,12 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
             }
         }
         if (tid < QT) {
-            s_lse[buf][tid] = next_lse;
+            s_norm[buf][tid] = next_norm;
             s_seen[buf][tid] = next_seen;
         }
     };
     // 16 rows against the wave's places. CUT: some row does not see them all
-    auto rows16 = [&](const u32x4 (*q)[D / 32], float lse, int seen,
+    auto rows16 = [&](const u32x4 (*q)[D / 32], f32x2 norm, int seen,
                       auto CUT) {
         f32x4 acc[PW];
         #pragma unroll
@@ -1463,8 +1470,9 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
         for (int u = 0; u < PW; u++)
             #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float w = exp2_fast(fmaf(acc[u][e], a.scale2, -lse));
-                sum[u][e] += !CUT || p0 + u * 16 + g * 4 + e < seen ? w : 0.f;
+                const float w = exp2_fast(fmaf(acc[u][e], a.scale2, -norm.x));
+                if (!CUT || p0 + u * 16 + g * 4 + e < seen)
+                    sum[u][e] = fmaf(w, norm.y, sum[u][e]);
             }
     };
     fetch(begin);
@@ -1488,14 +1496,14 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
                 for (int kk = 0; kk < D / 32; kk++)
                     q[x][kk] = lds_unit<D>(s_q[buf][x], t * 16 + n,
                                            kk * 4 + g);
-            const float lse = s_lse[buf][t * 16 + n];
+            const f32x2 norm = s_norm[buf][t * 16 + n];
             const int seen = s_seen[buf][t * 16 + n];
             // the first of 16 rows sees the least; rows past the last see none
             if (r + 16 <= R &&
                 p0 + 16 * PW <= s.len - s.m + a.group.of(r) + 1)
-                rows16(q, lse, seen, False{});
+                rows16(q, norm, seen, False{});
             else
-                rows16(q, lse, seen, True{});
+                rows16(q, norm, seen, True{});
         }
         if (more) stage(buf ^ 1);
         __syncthreads();
@@ -1979,7 +1987,7 @@ struct ObserveCut {
     int64_t blocks, parts, part, chunks, chunk, block, place_blocks;
     bool two;                       // a wave holds two groups of places
     bool several;                   // a sequence may have several chunks
-    int64_t sums, lse, partial;     // bytes
+    int64_t sums, norm, partial;    // bytes
 };
 
 // Rows of a workgroup of the first pass in its form for few rows; 0: the other
@@ -2036,7 +2044,7 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     c.several = R > c.chunk;
     c.chunks = up(R, c.chunk) + kv.slots - 1;
     c.sums = c.parts > 1 ? aligned((size_t)c.parts * rows * q_heads * 8) : 0;
-    c.lse = aligned((size_t)std::max(rows, 1) * q_heads * 4);
+    c.norm = aligned((size_t)std::max(rows, 1) * q_heads * 8);
     c.partial = c.several
         ? aligned((size_t)c.chunks * kv.kv_heads * c.place_blocks * c.block
                   * 4) : 0;
@@ -2049,7 +2057,7 @@ size_t kv_observe_workspace(const KvPages& kv, int q_heads, int rows,
                             int reach, KVT type) {
     check_pages(kv, q_heads, reach);
     const ObserveCut c = observe_cut(kv, q_heads, rows, reach, type);
-    return c.sums + c.lse + c.partial;
+    return c.sums + c.norm + c.partial;
 }
 
 void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
@@ -2073,7 +2081,7 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
                   (int32_t)c.block,
                   reinterpret_cast<float*>(w),
                   reinterpret_cast<float*>(w + c.sums),
-                  reinterpret_cast<float*>(w + c.sums + c.lse),
+                  reinterpret_cast<float*>(w + c.sums + c.norm),
                   c.place_blocks * c.block};
     KV_TYPES(type, kv.type, KV_DIM(kv.dim, {
         constexpr int RW = NQ > 1 ? 2 : 4, PW = obs_groups(NQ == 1, D);

@@ -152,3 +152,32 @@ def test_infinite_keys(types, parts):
         add, _ = oracle.observe(many, low, table, lens, [0, rows, 2 * rows],
                                 64 ** -.5)
         assert torch.allclose(again.double().cpu(), add, rtol=1e-4, atol=1e-6)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows,n", [(40, 3000), (600, 2000)])
+@pytest.mark.parametrize("far", [False, True])
+def test_observe_rows_add_up_to_one(types, rows, n, far):
+    """The weights that a row gives sum to 1, on average over rows with no
+    more than the roundings of their exponentials: the row's own sum must not
+    be rounded to fewer bits than they have.
+
+    Scores of at most 8 in base 2 below a sum of n: an exponent of at most 20
+    is off by 2^-21 (half a step) one way or the other, and an exponential by
+    2^-23; over the row's many places these average to a tenth of that at
+    most, as do the additions (a few units of 2^-24 each). A row's logarithm in
+    float32 (a sum of 2^11 to 2^19) would be off by up to 2^-20 one way. Far
+    scores, of -184 in base 2, are rounded in one pass and not in the other, by
+    2^-17 at most: over 160 rows x 1000 places, 2^-17 / 400.
+    """
+    from crowdllama_amd.ops import kv
+    _, pool, table = make(74, [n], 8, 2, 64, 64, types, strange=False)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(rows, 8, 64, generator=g)
+    if far:                         # scores far below 0: with a maximum
+        q[..., 0], pool[:, :, 0, :, 0] = -64., 16.
+    mass = torch.zeros(1, 2, table.shape[1] * 64, device="cuda")
+    kv.observe(q.to(types[0]).cuda(), pool.cuda(), table.cuda(), ints([n]),
+               mass, starts=ints([0, rows]))
+    given = mass.double().sum(-1).cpu() / (rows * 4)
+    assert ((given - 1).abs() <= 2.0 ** -23).all(), given - 1
