@@ -914,6 +914,8 @@ struct ObserveArgs {
 // row i, so that one pass over the keys serves the kv head's queries.
 struct Seq {
     int b, t0, m, len;   // its first packed row, its rows, its places
+    int before;          // places before its first row's own, negative if that
+                         // has none; row i sees the first before + i + 1, of len
 };
 
 __device__ __forceinline__ Seq sequence_at(const ObserveArgs& a, int b) {
@@ -921,8 +923,18 @@ __device__ __forceinline__ Seq sequence_at(const ObserveArgs& a, int b) {
     s.b = b;
     s.t0 = max(0, min(a.starts[b], a.rows));
     s.m = max(0, min(a.starts[b + 1], a.rows) - s.t0);
-    s.len = kv_clamp_len(a.lens[b], a.reach);
+    // a length past the last place is that of a longer sequence, whose later
+    // tokens were not stored: its rows' places are counted from there (as far
+    // as it matters: where each row sees all places)
+    const int len = max(a.lens[b], 0);
+    s.len = min(len, a.reach);
+    s.before = min(len, a.reach + s.m) - s.m;
     return s;
+}
+
+// How many places row i of the sequence sees.
+__device__ __forceinline__ int sees(const Seq& s, int i) {
+    return min(s.before + i + 1, s.len);
 }
 
 // Rows are staged in LDS with 16 bytes more than they have: an odd number of
@@ -980,7 +992,8 @@ __device__ __forceinline__ RowBlock row_block(const ObserveArgs& a, int rows,
             // scalars, as all that follows from them
             const int at = __builtin_ctzll(over);
             auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-            s = {base + at, of(own.t0), of(own.m), of(own.len)};
+            s = {base + at, of(own.t0), of(own.m), of(own.len),
+                 of(own.before)};
             return {at_x - before - of(upto) + of(all), of(all)};
         }
         before += __builtin_amdgcn_readlane(upto, 63);
@@ -1038,9 +1051,8 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
     const int R = s.m * G;
     const int r0 = id * ROWS + wave * 16 * RW;
     // places that the workgroup's last row, and the wave's first, see
-    const int most = s.len - s.m
-        + a.group.of(min(id * ROWS + ROWS, R) - 1) + 1;
-    const int least = s.len - s.m + a.group.of(r0) + 1;
+    const int most = sees(s, a.group.of(min(id * ROWS + ROWS, R) - 1));
+    const int least = sees(s, a.group.of(r0));
     const int begin = blockIdx.z * a.part, end = min(begin + a.part, most);
 
     u32x4 q[RW][NQ][D / 32];
@@ -1053,7 +1065,7 @@ __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
         load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
                              + (int64_t)(head * G + h) * a.q.head_stride,
                          there, g, q[w]);
-        seen[w] = there ? s.len - s.m + i + 1 : 0;
+        seen[w] = there ? sees(s, i) : 0;
     }
     #pragma unroll
     for (int w = 0; w < RW; w++)
@@ -1209,8 +1221,8 @@ __global__ __launch_bounds__(256) void k_kv_observe_few(ObserveArgs a) {
     const int id = late_block<ROWS>(a, s);
     if (id < 0) return;
     const int R = s.m * G, r0 = id * ROWS;
-    const int most = s.len - s.m + a.group.of(min(r0 + ROWS, R) - 1) + 1;
-    const int least = s.len - s.m + a.group.of(r0) + 1;
+    const int most = sees(s, a.group.of(min(r0 + ROWS, R) - 1));
+    const int least = sees(s, a.group.of(r0));
     const int begin = blockIdx.z * a.part, end = min(begin + a.part, most);
 
     u32x4 q[RW][NQ][D / 32];
@@ -1222,7 +1234,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_few(ObserveArgs a) {
         load_q<C, NQ, D>(a.q.data, (int64_t)(s.t0 + i) * a.q.row_stride
                              + (int64_t)(head * G + h) * a.q.head_stride,
                          r < R, g, q[w]);
-        seen[w] = r < R ? s.len - s.m + i + 1 : 0;
+        seen[w] = r < R ? sees(s, i) : 0;
         m[w] = -INFINITY;
         l[w] = 0.f;
     }
@@ -1352,7 +1364,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int first = block * 16 * PW * WAVES, p0 = first + wave * 16 * PW;
     const int R = s.m * G;
     // rows from the first that sees the block's first place on
-    const int from = max(0, first - (s.len - s.m)) * G;
+    const int from = max(0, first - s.before) * G;
     const int begin = max(chunk * a.chunk, from / QT * QT);
     const int end = min(chunk * a.chunk + a.chunk, R);
     if (first >= s.len || begin >= end) return;
@@ -1422,7 +1434,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
         if (tid < QT) {
             const int r = r0 + tid;
             next_norm = r < R ? from_norm[r] : f32x2{INFINITY, 0.f};
-            next_seen = r < R ? s.len - s.m + a.group.of(r) + 1 : 0;
+            next_seen = r < R ? sees(s, a.group.of(r)) : 0;
         }
     };
     auto stage = [&](int buf) {
@@ -1500,7 +1512,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
             const int seen = s_seen[buf][t * 16 + n];
             // the first of 16 rows sees the least; rows past the last see none
             if (r + 16 <= R &&
-                p0 + 16 * PW <= s.len - s.m + a.group.of(r) + 1)
+                p0 + 16 * PW <= sees(s, a.group.of(r)))
                 rows16(q, norm, seen, False{});
             else
                 rows16(q, norm, seen, True{});
@@ -1542,7 +1554,7 @@ __global__ __launch_bounds__(256) void k_kv_observe_add(ObserveArgs a) {
                      a.chunks);
     #pragma unroll
     for (int x = 1; x < 64; x <<= 1) before += __shfl_xor(before, x, 64);
-    const int from = max(0, p / a.block * a.block - (s.len - s.m)) * G;
+    const int from = max(0, p / a.block * a.block - s.before) * G;
     if (p >= s.len || from >= R) return;
     const int64_t step = (int64_t)a.kv_heads * a.ld;
     const float* part = a.partial + before * step + (int64_t)head * a.ld + p;

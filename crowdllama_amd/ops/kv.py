@@ -390,8 +390,10 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
     q: `[rows, heads, head_dim]`, rotated; rows `starts[b]` to `starts[b + 1]`
     are the queries of sequence b's last tokens (without `starts`, row b is
     that of sequence b's last), whose keys are in the cache: `lens[b]` counts
-    them. Each sees the places up to its own. What `attend` adds for one token,
-    this adds for a prompt, without making its outputs. Returns mass.
+    them. Each sees the places up to its own; where `lens[b]` goes past the last
+    place, the tokens past it have none, and the others see what they would in
+    a longer cache. What `attend` adds for one token, this adds for a prompt,
+    without making its outputs. Returns mass.
     """
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]

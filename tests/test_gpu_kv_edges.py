@@ -181,3 +181,35 @@ def test_observe_rows_add_up_to_one(types, rows, n, far):
                mass, starts=ints([0, rows]))
     given = mass.double().sum(-1).cpu() / (rows * 4)
     assert ((given - 1).abs() <= 2.0 ** -23).all(), given - 1
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("past", [0, 1, 5, 29, 30, 31, 1000, 2 ** 31 - 200])
+def test_observe_past_the_last_place(types, past):
+    """Tokens past the last place were not stored; the rows before them see
+    what they would see in a longer cache."""
+    from crowdllama_amd.ops import kv
+    cap, rows = 128, [30, 30, 4]
+    lens = [cap + past, 70, min(cap + 3, cap + past)]
+    _, pool, table = make(75, [cap, 70, cap], 4, 2, 64, 16, types,
+                          strange=False)
+    table = table[:, :cap // 16].contiguous()
+    q = torch.randn(64, 4, 64, generator=torch.Generator().manual_seed(2))
+    q = q.to(types[0])
+    starts = [0, 30, 60, 64]
+    mass = torch.zeros(3, 2, cap, device="cuda")
+    kv.observe(q.cuda(), pool.cuda(), table.cuda(), ints(lens), mass,
+               starts=ints(starts))
+    want = torch.zeros(3, 2, cap, dtype=torch.float64)
+    for b, n in enumerate(lens):
+        k, _, there = oracle.keys_values(pool, table, b, min(n, cap))
+        seen = torch.arange(min(n, cap))[None] <= \
+            (n - rows[b] + torch.arange(rows[b]))[:, None]
+        for h in range(2):
+            x = q[starts[b]:starts[b + 1], 2 * h:2 * h + 2].double()
+            w, _ = oracle.weights(x.transpose(0, 1), k[h], there, 64 ** -.5,
+                                  seen)
+            want[b, h, :min(n, cap)] = w.sum((0, 1))
+    # 68 x 4 half steps of scores below 16, 30 rows: below 2^-10
+    assert torch.allclose(mass.double().cpu(), want, rtol=2.0 ** -10,
+                          atol=1e-6)
