@@ -268,12 +268,13 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     const bool mine = b >= 0 && b < a.slots;
     const int64_t place = mine ? (int64_t)a.lens[b] + i : -1;
     const int position = mine ? a.next_pos[b] + i : 0;
-    if (a.inv_freq && tid < D / 2) {
+    // rows behind the last sequence keep their queries as they are
+    const bool turned = a.inv_freq && mine;
+    if (turned && tid < D / 2) {
         const double turn = (double)position * (double)a.inv_freq[tid];
         const double whole = rint(turn * 0.15915494309189535);
         const float rest = (float)fma(whole, -6.283185307179586, turn);
-        // rows behind the last sequence keep their queries as they are
-        sincosf(mine ? rest : 0.f, &sn[tid], &cs[tid]);
+        sincosf(rest, &sn[tid], &cs[tid]);
     }
     __syncthreads();
 
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
         const int h = kvh < 0 ? head : is_v ? kvh - a.kv_heads : kvh;
         float x[8];
         load8<T>(src.data, t * src.row_stride + h * src.head_stride + d, x);
-        if (a.inv_freq && !is_v) {
+        if (turned && !is_v) {
             #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float c = cs[d / 2 + j], s = sn[d / 2 + j];

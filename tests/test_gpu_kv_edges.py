@@ -213,3 +213,28 @@ def test_observe_past_the_last_place(types, past):
     # 68 x 4 half steps of scores below 16, 30 rows: below 2^-10
     assert torch.allclose(mass.double().cpu(), want, rtol=2.0 ** -10,
                           atol=1e-6)
+
+
+@pytest.mark.parametrize("types", TYPES, ids=IDS)
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_leaves_rows_behind_the_last_sequence(types, in_place):
+    """As they are, infinities, NaN and signs of zeros among them."""
+    from crowdllama_amd.ops import kv
+    lens = [3, 8]
+    _, pool, table = make(76, lens, 4, 2, 64, 16, types, 4, strange=False)
+    x = torch.randn(9, 8, 64, generator=torch.Generator().manual_seed(1))
+    x = x.to(types[0])
+    x[5, :, ::2], x[5, :, 1::4] = math.inf, -1.
+    x[6] = math.nan
+    x[7, :, ::3], x[7, :, 1::3] = -0., -2.
+    x[8, :, 1::2] = -math.inf
+    dx, dp = x.cuda(), pool.cuda()
+    inv = torch.rand(32, device="cuda")
+    got = kv.append(dx[:, 4:6], dx[:, 6:], dp, table.cuda(), ints(lens),
+                    ints([1, 2]), q=dx[:, :4], inv_freq=inv,
+                    starts=ints([0, 2, 5]),
+                    q_out=dx[:, :4] if in_place else None)
+    bits = torch.int32 if types[0] is torch.float32 else torch.int16
+    assert torch.equal(got[5:].cpu().contiguous().view(bits),
+                       x[5:, :4].contiguous().view(bits))
+    assert not got[:5].isnan().any()
