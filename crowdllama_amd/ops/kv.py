@@ -27,12 +27,14 @@ there: no call waits for the device, and all may be captured into a graph
 (which then goes by the values at replay). Lengths are cut to what the table
 and the mass reach; page numbers outside the pool are not followed: such places
 have no weight, and nothing is stored there. Work goes to the current stream
-of the tensors' device. None of the operators has a gradient.
+of the tensors' device. None of the operators has a gradient, and none can be
+traced (fake or functional tensors, `make_fx`).
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _NONE = (0, 0, 0)
@@ -91,11 +93,33 @@ def _dense(t, name: str, n: int):
     return want
 
 
-def _no_grad(*tensors):
+_depth = torch._C._len_torch_dispatch_stack
+_TRACERS = [getattr(torch._C._TorchDispatchModeKey, x)
+            for x in ("FAKE", "PROXY", "FUNCTIONAL")]
+
+
+def _plain(*tensors):
+    """The call is neither differentiated nor traced."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 _fail("no operator of the cache has a gradient")
+    if forward_ad._current_level >= 0:       # there may be tangents
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                _fail("no operator of the cache has a gradient")
+    if _depth() and any(torch._C._get_dispatch_mode(x) is not None
+                        for x in _TRACERS):
+        _fail("the operators work on memory and cannot be traced")
+
+
+def _memory(t, name: str) -> int:
+    """The address of a tensor that has values."""
+    at = t.data_ptr()
+    if not at and t.numel():
+        _fail(f"{name} has no memory (a fake or functional tensor): the "
+              "operators work on memory and cannot be traced")
+    return at
 
 
 def _pages(pool, table, layers: bool):
@@ -112,14 +136,15 @@ def _pages(pool, table, layers: bool):
                 and not (layers and (st[1] < st[2] * heads or st[1] % 8
                                      or st[0] < st[1] * ps[1]))
                 and st[0] >= 2 * per * heads and not (st[0] % 8 or at % 16)
-                and p and heads and page and dim
+                and p and heads and page and dim and at
                 and table.dtype is torch.int32 and len(ts) == 2
                 and ts[0] and ts[1] and table.stride()[1] == 1
-                and table.device == dev):
+                and table.device == dev and (pages := table.data_ptr())):
             return dev, ts[1] * page, (
-                at, st[0], p, table.data_ptr(), table.stride()[0], ts[1],
-                page, ts[0], heads, dim, kind, dev.index)
-    except (AttributeError, KeyError, ValueError, IndexError, TypeError):
+                at, st[0], p, pages, table.stride()[0], ts[1], page, ts[0],
+                heads, dim, kind, dev.index)
+    except (AttributeError, KeyError, ValueError, IndexError, TypeError,
+            RuntimeError):
         pass
     return _pages_slowly(pool, table, layers)
 
@@ -146,7 +171,7 @@ def _pages_slowly(pool, table, layers: bool):
             stride[0] >= stride[1] * shape[1]
             or stride[1] >= stride[0] * p):
         _fail("pool's layers and pages must not overlap")
-    if pool.numel() == 0 or pool.data_ptr() % 16:
+    if pool.numel() == 0 or _memory(pool, "pool") % 16:
         _fail("pool must not be empty and must be 16-byte aligned")
     _on(table, "table", torch.int32, 2, dev)
     _dense(table, "table", 1)
@@ -154,23 +179,25 @@ def _pages_slowly(pool, table, layers: bool):
     if not slots or not reach:
         _fail("table must not be empty")
     return dev, reach, (
-        pool.data_ptr(), stride[0], p, table.data_ptr(), table.stride(0),
-        table.shape[1], page, slots, heads, dim, _TYPES[pool.dtype],
-        dev.index)
+        pool.data_ptr(), stride[0], p, _memory(table, "table"),
+        table.stride(0), table.shape[1], page, slots, heads, dim,
+        _TYPES[pool.dtype], dev.index)
 
 
 def _vector(t, name: str, n: int, dev):
     try:
         if (t.dtype is torch.int32 and t.shape == (n,) and t.stride() == (1,)
                 and t.device == dev):
-            return t.data_ptr()
+            at = t.data_ptr()
+            if at:
+                return at
     except (AttributeError, TypeError):
         pass
     _on(t, name, torch.int32, 1, dev)
     if t.shape[0] != n:
         _fail(f"{name} must have {n} values, not {t.shape[0]}")
     _dense(t, name, 1)
-    return t.data_ptr()
+    return _memory(t, name)
 
 
 def _heads(t, name: str, rows, heads, dim: int, dtype, dev):
@@ -178,12 +205,12 @@ def _heads(t, name: str, rows, heads, dim: int, dtype, dev):
         n, h, d = t.shape
         s0, s1, s2 = t.stride()
         at = t.data_ptr()
-        if (d == dim and s2 == 1 and t.dtype is dtype and t.device == dev
+        if (at and d == dim and s2 == 1 and t.dtype is dtype and t.device == dev
                 and (rows is None or n == rows)
                 and (heads is None or h == heads)
                 and not (at % 16 or s0 % 8 or s1 % 8)):
             return at, s0, s1
-    except (AttributeError, TypeError, ValueError):
+    except (AttributeError, TypeError, ValueError, RuntimeError):
         pass
     _on(t, name, dtype, 3, dev)
     shape = t.shape
@@ -195,10 +222,11 @@ def _heads(t, name: str, rows, heads, dim: int, dtype, dev):
     _dense(t, name, 1)
     s0, s1, _ = t.stride()
     unit = 4 if dtype is torch.float32 else 8
-    if t.data_ptr() % 16 or (shape[0] > 1 and s0 % unit) or (
+    at = _memory(t, name)
+    if at % 16 or (shape[0] > 1 and s0 % unit) or (
             shape[1] > 1 and s1 % unit):
         _fail(f"{name}'s rows must be 16-byte aligned")
-    return t.data_ptr(), s0, s1
+    return at, s0, s1
 
 
 def _apart(t, name: str):
@@ -228,7 +256,9 @@ def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
         if (t.shape[:-1] == lead and 0 < t.shape[-1] <= reach
                 and t.dtype is dtype and t.is_contiguous()
                 and t.device == dev):
-            return (t.data_ptr(), *t.stride()[:-1])
+            at = t.data_ptr()
+            if at:
+                return (at, *t.stride()[:-1])
     except (AttributeError, TypeError):
         pass
     _on(t, name, dtype, len(lead) + 1, dev)
@@ -239,7 +269,7 @@ def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
               f"reaches), not {t.shape[-1]}")
     _dense(t, name, 1)
     _apart(t, name)
-    return (t.data_ptr(), *t.stride()[:-1])
+    return (_memory(t, name), *t.stride()[:-1])
 
 
 def _queries(q, dtype_of_pool):
@@ -332,7 +362,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         _dense(inv_freq, "inv_freq", 1)
         if inv_freq.shape[0] != dim // 2:
             _fail(f"inv_freq must have {dim // 2} values")
-        fr = inv_freq.data_ptr()
+        fr = _memory(inv_freq, "inv_freq")
     ms = ps = _NONE
     if mass is not None:
         ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
@@ -342,7 +372,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         reach = min(reach, pos.shape[-1])
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
-    _no_grad(k, v, q, pool, mass)
+    _plain(k, v, q, pool, mass, inv_freq)
     _get(dev).kv_append(kv, kh, vh, qh, qo, q_heads, _TYPES[k.dtype], rows,
                         st, le, np, fr, ms, ps, reach, _stream(dev))
     return q_out
@@ -375,7 +405,7 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
         oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
         _apart(out, "out")
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
-    _no_grad(q, pool, mass)
+    _plain(q, pool, mass)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
                                              mass is not None), table)
@@ -410,7 +440,7 @@ def observe(q, pool, table, lens, mass, *, starts=None, scale=None):
         starts = torch.arange(slots + 1, dtype=torch.int32, device=dev)
     st = _vector(starts, "starts", slots + 1, dev)
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
-    _no_grad(q, pool, mass)
+    _plain(q, pool, mass)
     core = _get(dev)
     ws = _workspace(core.kv_observe_workspace(kv, q_heads, rows, reach,
                                               _TYPES[q.dtype]), table)
@@ -458,7 +488,7 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
         _fail("layers x sequences x kv heads must be below 2^22")
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
-    _no_grad(pool, mass)
+    _plain(pool, mass)
     spans = [_ends(mass), _ends(pos), _ends(lens)]
     if out is None:
         mass_out, pos_out, lens_out = mass, pos, lens
