@@ -33,6 +33,7 @@ traced (fake or functional tensors, `make_fx`).
 
 from __future__ import annotations
 
+import numpy
 import torch
 from torch.autograd import forward_ad
 
@@ -251,6 +252,44 @@ def _ends(t):
         1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
+def _pieces(t):
+    """The first and last address of each contiguous piece of a tensor."""
+    size, shape, stride = t.element_size(), list(t.shape), list(t.stride())
+    long_ = 1
+    while shape and (shape[-1] == 1 or stride[-1] == long_):
+        long_ *= shape.pop()
+        stride.pop()
+    at = numpy.array([t.data_ptr()])
+    for n, step in zip(shape, stride):
+        if step:
+            at = (at[:, None] + numpy.arange(n) * (step * size)).ravel()
+    return at, at + (long_ * size - 1)
+
+
+def _over(t, name: str, inputs):
+    """An output that a caller gives must not overlap what the call reads:
+    other workgroups read that while one writes."""
+    if not t.numel():
+        return
+    first, last = _ends(t)
+    for of, x, at in inputs:
+        if not at or at >= last:
+            continue
+        lo, hi = _ends(x)
+        if hi <= first or not x.numel() or (of == "q" and lo == first and all(
+                m == n for m, n, size in zip(x.stride(), t.stride(), t.shape)
+                if size > 1)):
+            continue
+        # piece by piece: what lies between an input's rows is free
+        a, b = _pieces(t)
+        order = numpy.argsort(a)
+        a, b = a[order], b[order]
+        lo, hi = _pieces(x)
+        at = numpy.searchsorted(a, hi, side="right")    # pieces that begin by hi
+        if ((at > 0) & (b[at - 1] >= lo)).any():
+            _fail(f"{name} overlaps {of}")
+
+
 def _places(t, name: str, dtype, lead: tuple, reach: int, dev):
     try:
         if (t.shape[:-1] == lead and 0 < t.shape[-1] <= reach
@@ -326,7 +365,8 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
 
     inv_freq: float32 `[head_dim / 2]`, the radians per position of each
     adjacent pair; without it nothing is rotated. q `[rows, heads, head_dim]`
-    is rotated as k is, and returned (in `q_out`, which may be q itself).
+    is rotated as k is, and returned (in `q_out`, which may be q itself, but
+    must not overlap it, or another input, otherwise).
     mass, pos: the new places' mass becomes 0 and their pos the position.
 
     `lens` and `next_pos` are only read (all layers share them). Rows past the
@@ -340,7 +380,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
     kh = _heads(k, "k", None, heads, dim, k.dtype, dev)
     vh = _heads(v, "v", rows, heads, dim, k.dtype, dev)
     qh = qo = _NONE
-    q_heads = 0
+    q_heads, over = 0, None
     if q is not None:
         qh = _heads(q, "q", rows, None, dim, k.dtype, dev)
         q_heads = q.shape[1]
@@ -349,6 +389,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
             qo = (q_out.data_ptr(), q_heads * dim, dim)
         else:
             qo = _heads(q_out, "q_out", rows, q_heads, dim, k.dtype, dev)
+            over = q_out
             _apart(q_out, "q_out")
     elif q_out is not None:
         _fail("q_out without q")
@@ -372,6 +413,13 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         reach = min(reach, pos.shape[-1])
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
+    if over is not None:
+        _over(over, "q_out", (
+            ("q", q, qh[0]), ("k", k, kh[0]), ("v", v, vh[0]),
+            ("pool", pool, kv[0]), ("mass", mass, ms[0]), ("pos", pos, ps[0]),
+            ("table", table, kv[3]), ("lens", lens, le),
+            ("next_pos", next_pos, np), ("starts", starts, st),
+            ("inv_freq", inv_freq, fr)))
     _plain(k, v, q, pool, mass, inv_freq)
     _get(dev).kv_append(kv, kh, vh, qh, qo, q_heads, _TYPES[k.dtype], rows,
                         st, le, np, fr, ms, ps, reach, _stream(dev))
@@ -385,8 +433,9 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     q: `[slots, heads, head_dim]`, of the pool's type or float32 over a
     bfloat16 pool; query heads g * i ... g * i + g - 1 share kv head i.
     mass: each place's weight is added, summed over the query heads that share
-    the kv head. scale: of the scores, positive, head_dim ** -0.5 by default. A sequence
-    without places gives zeros.
+    the kv head. scale: of the scores, positive, head_dim ** -0.5 by default.
+    out: may be q itself, but must not overlap it, or another input, otherwise.
+    A sequence without places gives zeros.
     """
     dev, reach, kv = _pages(pool, table, False)
     slots, heads, dim = kv[7], kv[8], kv[9]
@@ -398,13 +447,18 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     if mass is not None:
         ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
         reach = mass.shape[-1]
-    if out is None:
+    given = out is not None
+    if not given:
         out = q.new_empty((slots, q_heads, dim))
         oh = (out.data_ptr(), q_heads * dim, dim)
     else:
         oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
         _apart(out, "out")
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
+    if given:
+        _over(out, "out", (
+            ("q", q, qh[0]), ("pool", pool, kv[0]), ("mass", mass, ms[0]),
+            ("table", table, kv[3]), ("lens", lens, le)))
     _plain(q, pool, mass)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,

@@ -180,3 +180,93 @@ def test_outputs_of_a_written_tensor_are_checked_too(core):
         with pytest.raises(ValueError, match="no memory"):
             call()
     assert not core.calls
+
+
+def rows_of(base, at, n, heads=4, stride=None):
+    """[n, heads, 64] from element `at` of a flat tensor on."""
+    return base.as_strided((n, heads, 64), (stride or heads * 64, 64, 1), at)
+
+
+def test_outputs_over_inputs_are_refused(core):
+    """All but exactly the queries: other workgroups still read what one
+    writes."""
+    t = tensors()
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    t["q"] = rows_of(base, 256, 2)
+    for at, stride in ((0, None), (256 + 64, None), (256 + 256, None),
+                       (256, 512), (256 + 448, 64 * 5), (256 - 192, None)):
+        for call in (append, attend):
+            name = "q_out" if call is append else "out"
+            with pytest.raises(ValueError, match=name + " overlaps q"):
+                call(t, **{name: rows_of(base, at, 2, stride=stride)})
+    swapped = t["q"].as_strided((2, 4, 64), (64, 128, 1))
+    with pytest.raises(ValueError, match="out overlaps q"):
+        attend(t, out=swapped)
+    for name in ("k", "v"):
+        both = tensors()
+        both[name] = rows_of(base, 0, 2, heads=2)
+        for at in (0, 64, 192):
+            with pytest.raises(ValueError, match=f"q_out overlaps {name}"):
+                append(both, q_out=rows_of(base, at, 2))
+    assert not core.calls
+    for out in (t["q"], rows_of(base, 256, 2), rows_of(base, 768, 2),
+                rows_of(base, 1024, 2, stride=1024)):
+        assert append(t, q_out=out) is out and attend(t, out=out) is out
+    assert len(core.calls) == 8
+
+
+def test_outputs_over_the_cache_are_refused(core):
+    t = tensors()
+    pool = t["pool"].reshape(-1)
+    out = rows_of(pool, pool.numel() - 600, 2)
+    for call, name in ((append, "q_out"), (attend, "out")):
+        with pytest.raises(ValueError, match=name + " overlaps pool"):
+            call(t, **{name: out})
+        whole = torch.zeros(4096, dtype=torch.bfloat16)
+        for part, dtype in (("mass", torch.float32), ("table", torch.int32),
+                            ("lens", torch.int32)):
+            u = dict(t)
+            n = t[part].numel() * 2
+            u[part] = whole[64:64 + n].view(dtype).view(t[part].shape)
+            with pytest.raises(ValueError, match=f"{name} overlaps {part}"):
+                call(u, **{name: rows_of(whole, 0, 2)})
+    assert not core.calls
+
+
+def test_outputs_between_inputs_are_taken(core):
+    """Rows of one fused product, and other strides that meet nowhere."""
+    wide = torch.zeros(2, 8 * 64 + 64, dtype=torch.bfloat16)
+    t = tensors()
+    t["q"] = wide[:, :256].view(2, 4, 64)
+    t["k"] = wide[:, 256:384].view(2, 2, 64)
+    t["v"] = wide[:, 384:512].view(2, 2, 64)
+    append(t, q_out=t["q"])
+    base = torch.zeros(4096, dtype=torch.bfloat16)
+    t["q"] = base.as_strided((2, 4, 64), (1024, 128, 1))
+    between = base.as_strided((2, 4, 64), (1024, 128, 1), 64)
+    append(t, q_out=between)
+    attend(t, out=between)
+    attend(t, out=base.as_strided((2, 4, 64), (1024, 64, 1), 512))
+    assert len(core.calls) == 4
+    with pytest.raises(ValueError, match="out overlaps q"):
+        attend(t, out=base.as_strided((2, 4, 64), (1024, 64, 1), 440))
+
+
+def test_more_than_one_sequence_may_read_one_row(core):
+    """Inputs may overlap themselves and each other."""
+    t = tensors()
+    t["q"] = t["q"][:1].expand(2, 4, 64)
+    t["k"] = t["v"] = t["k"][:1].expand(2, 2, 64)
+    append(t)
+    attend(t, out=torch.zeros(2, 4, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="overlap itself"):
+        append(t, q_out=t["q"])
+
+
+def test_one_row_has_no_stride(core):
+    t = tensors()
+    t["q"] = torch.zeros(1, 512, dtype=torch.bfloat16)[:, :256].view(1, 4, 64)
+    for x in ("table", "lens", "mass"):
+        t[x] = t[x][:1]
+    out = t["q"].as_strided((1, 4, 64), (256, 64, 1))
+    assert attend(t, out=out) is out
