@@ -154,7 +154,7 @@ void check_pages(const KvPages& kv, int q_heads, int reach) {
 }
 
 void check_scale(float scale) {
-    if (!(scale > 0.f && scale < INFINITY))
+    if (!(scale > 0.f && scale * LOG2E < INFINITY))
         throw std::runtime_error("scale must be positive and finite");
 }
 

@@ -330,8 +330,10 @@ def _scale(scale, dim: int) -> float:
     if scale is None:
         return dim ** -0.5
     scale = float(scale)
-    if not 0 < scale < 3e38:
-        _fail(f"scale must be positive and finite, not {scale}")
+    # the kernels multiply by it and log2(e) in float32, without subnormals
+    if not 2.0 ** -126 <= scale <= 2.0 ** 127:
+        _fail(f"scale must be positive and finite in float32 (2^-126 to "
+              f"2^127), not {scale}")
     return scale
 
 

@@ -270,3 +270,16 @@ def test_one_row_has_no_stride(core):
         t[x] = t[x][:1]
     out = t["q"].as_strided((1, 4, 64), (256, 64, 1))
     assert attend(t, out=out) is out
+
+
+@pytest.mark.parametrize("op", [attend, observe])
+def test_scales_that_float32_does_not_hold(core, op):
+    """As it is, and times log2(e)."""
+    t = tensors()
+    for scale in (1e-40, 1e-320, 2.4e38, 2.9e38, 1e300):
+        with pytest.raises(ValueError, match="scale must be positive"):
+            op(t, scale=scale)
+    assert not core.calls
+    for scale in (2.0 ** -126, 1, 2.0 ** 127):
+        op(t, scale=scale)
+        assert core.calls[-1][1][-3] == scale
