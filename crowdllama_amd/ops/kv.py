@@ -26,7 +26,7 @@ differ from head to head.
 there: no call waits for the device, and all may be captured into a graph
 (which then goes by the values at replay). Lengths are cut to what the table
 and the mass reach; page numbers outside the pool are not followed: such places
-have no weight, and nothing is stored there. Work goes to the current stream
+have no weight, and no keys and values are stored there. Work goes to the current stream
 of the tensors' device. None of the operators has a gradient, and none can be
 traced (fake or functional tensors, `make_fx`).
 """
@@ -515,15 +515,18 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
     pool: `[pages, layers, kv_heads, 2, page, head_dim]`; mass, pos:
     `[layers, slots, kv_heads, places]`. Places with a pos of at least
     `next_pos[b] - recent` stay before all others, the others by mass; among
-    equals the lower place stays, and a NaN counts as less than any number.
-    Survivors below place `keep` stay where they are; the free places there
-    take the others, both in order. What lies at and above `keep` afterwards is
-    left as it was.
+    equals the lower place stays, and a NaN counts as less than any number. The
+    late ones are equals: of more than `keep` of them those in the lower places
+    stay. Survivors below place `keep` stay where they are; the free places
+    there take the others, both in order. What lies at and above `keep`
+    afterwards is left as it was.
 
     Keys and values move within the pool, so a page must not serve two places
-    of the table. mass, pos and lens are changed in
-    place, or, with `out=(mass, pos, lens)`, written there whole while these
-    stay as they were.
+    of the table, and the pages of a sequence that is to be evicted from must
+    be there: mass and pos order and move its places whether they have a page
+    or not, keys and values move where both places have one. mass, pos and lens
+    are changed in place, or, with `out=(mass, pos, lens)`, written there whole
+    while these stay as they were.
     """
     dev, reach, kv = _pages(pool, table, True)
     slots, heads, layers = kv[7], kv[8], pool.shape[1]
