@@ -47,7 +47,7 @@ struct KvHeads {
 
 // Pages are only followed where the table and the pool have them: -1 for a
 // place past the table's end and for a page number outside the pool. Such
-// places have no weight and nothing is stored there.
+// places have no weight, and no keys and values are stored there.
 __host__ __device__ inline int32_t kv_page_of(const int32_t* row,
                                               int64_t index,
                                               int32_t max_pages,
@@ -111,7 +111,8 @@ void launch_kv_observe(const KvPages& kv, const KvHeads& q, int q_heads,
 
 // Keep `keep` places of each sequence that has more than `limit`, in all
 // layers. mass, pos and lens are written to the *_out tensors, which may be
-// the same ones.
+// the same ones. Places are ordered and moved whether they have a page or not;
+// keys and values move where both places have one.
 struct KvLayers {              // [layers][slots][kv heads][places]
     void* data = nullptr;
     int64_t layer_stride = 0, slot_stride = 0, head_stride = 0;
