@@ -29,12 +29,14 @@ class WireError(Exception):
 async def end_tasks(tasks: list[asyncio.Task]) -> None:
     """Cancel background tasks and wait for their end. One cancellation is not
     enough: asyncio.wait_for drops it (up to Python 3.11) if what it waits for
-    is done at the same time, and the task's loop goes on."""
-    left = set(tasks)
+    is done at the same time, and the task's loop goes on. A task has two
+    seconds to clean up before it is cancelled again; one that calls this
+    itself is left to end by itself."""
+    left = set(tasks) - {asyncio.current_task()}
     while left:
         for t in left:
             t.cancel()
-        done, left = await asyncio.wait(left, timeout=0.5)
+        done, left = await asyncio.wait(left, timeout=2)
         for t in done:
             if not t.cancelled():
                 t.exception()       # seen: an error here ends nothing else
