@@ -61,6 +61,7 @@ async def _run_start(args) -> None:
     cfg = _mk_config(args)
     cfg.worker_mode = args.worker_mode
     cfg.gateway_port = args.port
+    cfg.max_new_tokens = args.max_new_tokens
     log = new_app_logger("crowdllama", cfg.verbose)
     log.info("%s", version_string())
 
@@ -115,7 +116,7 @@ async def _run_start(args) -> None:
                 return pb.response_message(req.model,
                                            f"Error: model {req.model} not loaded",
                                            done_reason="error")
-            result = await eng.generate(req.prompt)
+            result = await eng.generate(req.prompt, cfg.max_new_tokens)
             return pb.response_message(req.model, result.text, peer.peer_id)
         ipc = IPCServer(cfg, cfg.ipc_socket, ipc_handler)
         await ipc.start()
@@ -213,6 +214,9 @@ def main(argv: list[str] | None = None) -> int:
     st.add_argument("--kv-recent", type=int, default=0,
                     help="of the --kv-keep places, how many are reserved "
                          "for the newest tokens")
+    st.add_argument("--max-new-tokens", type=int,
+                    default=Config.max_new_tokens,
+                    help="tokens for a request at most (worker mode)")
 
     dh = sub.add_parser("dht", help="start a bootstrap/rendezvous node")
     _add_common(dh)
@@ -234,6 +238,10 @@ def main(argv: list[str] | None = None) -> int:
         print(version_string())
         return 0
     if args.cmd == "start":
+        if args.max_new_tokens < 1:
+            st.error("--max-new-tokens must be at least 1")
+        if args.kv_recent and not args.kv_keep:
+            st.error("--kv-recent goes with --kv-keep")
         asyncio.run(_run_start(args))
         return 0
     if args.cmd == "dht":

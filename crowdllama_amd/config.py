@@ -59,6 +59,8 @@ class Config:
     test_mode: bool = False
     ipc_socket: str | None = None
     max_seq: int = 4096
+    # tokens that a worker generates for a request at most
+    max_new_tokens: int = 256
     # every peer runs an embedded rendezvous server (reference: libp2p
     # DHT ModeServer on every peer)
     peer_dht: bool = True

@@ -284,7 +284,8 @@ class Peer:
                 # a final done=True frame (extension over the reference,
                 # which reserves `stream` but never streams — SURVEY.md §2.2)
                 total_tokens = 0
-                async for chunk in engine.generate_stream(req.prompt):
+                async for chunk in engine.generate_stream(
+                        req.prompt, self.cfg.max_new_tokens):
                     total_tokens = chunk.tokens_generated
                     final = bool(chunk.done_reason)
                     resp = pb.response_message(
@@ -297,7 +298,8 @@ class Peer:
                 self.rate.add(total_tokens)
                 self.requests_served += 1
                 return
-            result = await engine.generate(req.prompt)
+            result = await engine.generate(req.prompt,
+                                           self.cfg.max_new_tokens)
             self.rate.add(result.tokens_generated)
             self.requests_served += 1
             resp = pb.response_message(
