@@ -10,6 +10,7 @@ MockEngine replacing the integration tests' MockOllamaServer
 from __future__ import annotations
 
 import asyncio
+import codecs
 import threading
 import time
 from dataclasses import dataclass
@@ -118,6 +119,18 @@ class MockEngine(EngineBase):
 
     def vram_gb(self) -> float:
         return 24.0
+
+
+class TextStream:
+    """A request's text as its tokens come: each is decoded once, and a
+    character that is not whole yet waits for the next ones."""
+
+    def __init__(self, tok):
+        self._tok = tok
+        self._chars = codecs.getincrementaldecoder("utf-8")("replace")
+
+    def add(self, ids: list[int], last: bool = False) -> str:
+        return self._chars.decode(self._tok.decode_bytes(ids), last)
 
 
 class RollingRate:

@@ -22,8 +22,8 @@ from dataclasses import dataclass, field
 
 from ..quant.gguf import GGUFReader
 from ..tokenizer import NativeTokenizer, Tokenizer
-from .api import EngineBase, GenerateResult, RollingRate, token_budget
-from .api import EVICTING_GEN
+from .api import EngineBase, GenerateResult, RollingRate, TextStream
+from .api import EVICTING_GEN, token_budget
 
 DECODE_STRIDE = 8  # graph replays between slot bookkeeping passes
 
@@ -38,7 +38,6 @@ class _Req:
     # `loop.call_soon_threadsafe` from the batcher thread
     chunks: object = None
     loop: object = None
-    sent_text: str = ""
 
     def push(self, item) -> None:
         if self.chunks is not None and self.loop is not None:
@@ -48,7 +47,9 @@ class _Req:
 class _Slot:
     def __init__(self):
         self.req: _Req | None = None
-        self.collected = 0
+        self.collected = 0                    # tokens that are in `parts`
+        self.text: TextStream | None = None
+        self.parts: list[str] = []
 
 
 class BatchingHipEngine(EngineBase):
@@ -112,6 +113,7 @@ class BatchingHipEngine(EngineBase):
             self.eng.prefill_slot(i, req.ids)
             slot.req = req
             slot.collected = 0
+            slot.text, slot.parts = TextStream(self.tok), []
             self._active += 1
 
     def _harvest(self) -> None:
@@ -122,40 +124,37 @@ class BatchingHipEngine(EngineBase):
                 # request completes: the decode step no longer advances them,
                 # so no per-stride reset is needed
                 continue
-            toks = list(self.eng.gen_tokens(i))
+            # the new ones only: a long request must not cost more a stride
+            toks = list(self.eng.gen_tokens(i, slot.collected))
             done = False
             if self.tok.eos_id in toks:
                 toks = toks[: toks.index(self.tok.eos_id)]
                 done = True
-            if len(toks) >= req.max_new:
-                toks = toks[: req.max_new]
+            if slot.collected + len(toks) >= req.max_new:
+                toks = toks[: req.max_new - slot.collected]
                 done = True
-            slot.collected = len(toks)
+            slot.collected += len(toks)
+            delta = slot.text.add(toks, done)
+            slot.parts.append(delta)
+            count = slot.collected
             if done:
-                text = self.tok.decode(toks)
-                self._rate.add(len(toks))
-                reason = "stop" if len(toks) < req.max_new else "length"
+                self._rate.add(count)
+                reason = "stop" if count < req.max_new else "length"
                 req.push(GenerateResult(
-                    text=text[len(req.sent_text):],
-                    tokens_generated=len(toks),
+                    text=delta, tokens_generated=count,
                     duration_ns=time.monotonic_ns() - req.t0,
                     done_reason=reason))
                 req.future.set_result(GenerateResult(
-                    text=text, tokens_generated=len(toks),
+                    text="".join(slot.parts), tokens_generated=count,
                     duration_ns=time.monotonic_ns() - req.t0,
                     done_reason=reason))
                 slot.req = None
                 self._active -= 1
                 self.eng.set_slot_active(i, False)
                 self.eng.reset_slot(i)
-            elif req.chunks is not None:
-                text = self.tok.decode(toks)
-                delta = text[len(req.sent_text):]
-                if delta:
-                    req.sent_text = text
-                    req.push(GenerateResult(text=delta,
-                                            tokens_generated=len(toks),
-                                            done_reason=""))
+            elif delta:
+                req.push(GenerateResult(text=delta, tokens_generated=count,
+                                        done_reason=""))
 
     def _loop(self) -> None:
         while not self._stop:

@@ -10,8 +10,8 @@ from concurrent.futures import ThreadPoolExecutor
 
 from ..quant.gguf import GGUFReader
 from ..tokenizer import NativeTokenizer, Tokenizer
-from .api import EngineBase, GenerateResult, RollingRate, token_budget
-from .api import EVICTING_GEN
+from .api import EngineBase, GenerateResult, RollingRate, TextStream
+from .api import EVICTING_GEN, token_budget
 
 
 class HipEngine(EngineBase):
@@ -140,34 +140,31 @@ class HipEngine(EngineBase):
             self.eng.reset()
             self.eng.prefill(np.asarray([ids], dtype=np.int32))
             n_new = max(1, max_new_tokens)
-            sent = ""
+            text, count = TextStream(self.tok), 0
             done_reason = "length"
             while True:
-                toks = list(self.eng.gen_tokens(0))
+                toks = list(self.eng.gen_tokens(0, count))
                 finished = False
                 if self.tok.eos_id in toks:
                     toks = toks[: toks.index(self.tok.eos_id)]
                     done_reason = "stop"
                     finished = True
-                if len(toks) >= n_new:
-                    toks = toks[:n_new]
+                if count + len(toks) >= n_new:
+                    toks = toks[:n_new - count]
                     finished = True
-                text = self.tok.decode(toks)
-                delta = text[len(sent):]
+                count += len(toks)
+                delta = text.add(toks, finished)
                 if finished:
-                    self._rate.add(len(toks))
+                    self._rate.add(count)
                     emit(GenerateResult(
-                        text=delta, tokens_generated=len(toks),
+                        text=delta, tokens_generated=count,
                         duration_ns=time.monotonic_ns() - t0,
                         done_reason=done_reason))
                     return
                 if delta:
-                    sent = text
-                    emit(GenerateResult(text=delta,
-                                        tokens_generated=len(toks),
+                    emit(GenerateResult(text=delta, tokens_generated=count,
                                         done_reason=""))
-                self.eng.decode(min(self.STREAM_STRIDE,
-                                    n_new - len(toks)))
+                self.eng.decode(min(self.STREAM_STRIDE, n_new - count))
 
     async def generate_stream(self, prompt: str, max_new_tokens: int = 256,
                               temperature: float = 0.0):

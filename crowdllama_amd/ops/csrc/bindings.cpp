@@ -133,7 +133,8 @@ PYBIND11_MODULE(_core, m) {
                  py::gil_scoped_release rel;
                  e.prefill_slot(slot, ids);
              })
-        .def("gen_tokens", &Engine::gen_tokens)
+        .def("gen_tokens", &Engine::gen_tokens, py::arg("slot"),
+             py::arg("first") = 0)
         .def("logits",
              [](Engine& e, int slot) {
                  auto v = e.logits(slot);

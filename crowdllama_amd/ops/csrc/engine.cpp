@@ -1140,14 +1140,17 @@ void Engine::decode(int n_steps) {
     hipEventDestroy(e1);
 }
 
-std::vector<int32_t> Engine::gen_tokens(int slot) {
+std::vector<int32_t> Engine::gen_tokens(int slot, int first) {
+    if (slot < 0 || slot >= cfg_.batch || first < 0)
+        throw std::runtime_error("gen_tokens: no such slot or token");
     int32_t count = 0;
     HIP_CHECK(hipMemcpy(&count, gen_count_ + slot, 4, hipMemcpyDeviceToHost));
     count = std::min(count, cfg_.gen_cap);
-    std::vector<int32_t> out(count);
-    if (count)
-        HIP_CHECK(hipMemcpy(out.data(), gen_tokens_ + (size_t)slot * cfg_.gen_cap,
-                            count * 4, hipMemcpyDeviceToHost));
+    std::vector<int32_t> out(std::max(count - first, 0));
+    if (!out.empty())
+        HIP_CHECK(hipMemcpy(out.data(),
+                            gen_tokens_ + (size_t)slot * cfg_.gen_cap + first,
+                            out.size() * 4, hipMemcpyDeviceToHost));
     return out;
 }
 

@@ -98,7 +98,8 @@ public:
     // Run n decode steps back-to-back (graph replays; one sync at the end).
     void decode(int n_steps);
     // Fetch generated tokens for a slot (gen_count entries).
-    std::vector<int32_t> gen_tokens(int slot);
+    // A slot's generated tokens, from its first-th on.
+    std::vector<int32_t> gen_tokens(int slot, int first = 0);
     // Copy a slot's current logits to host (for host-side sampling).
     std::vector<float> logits(int slot);
     // Override a slot's current input token (host-side sampling path).

@@ -110,6 +110,11 @@ class Tokenizer:
     # ------------------------------------------------------------- decode
 
     def decode(self, ids: list[int]) -> str:
+        return self.decode_bytes(ids).decode("utf-8", errors="replace")
+
+    def decode_bytes(self, ids: list[int]) -> bytes:
+        """A token's bytes need not be whole characters; those of a text are
+        its tokens' in turn."""
         out = bytearray()
         b2u = _bytes_to_unicode() if self.merge_ranks else None
         u2b = {v: k for k, v in b2u.items()} if b2u else None
@@ -130,7 +135,7 @@ class Tokenizer:
                         out.extend(ch.encode("utf-8"))
             else:
                 out.extend(tok.replace("▁", " ").encode("utf-8"))
-        return out.decode("utf-8", errors="replace")
+        return bytes(out)
 
     def __len__(self) -> int:
         return len(self.tokens)
@@ -159,7 +164,10 @@ class NativeTokenizer:
         return list(self._t.encode(text, add_bos))
 
     def decode(self, ids: list[int]) -> str:
-        return self._t.decode(list(ids)).decode("utf-8", errors="replace")
+        return self.decode_bytes(ids).decode("utf-8", errors="replace")
+
+    def decode_bytes(self, ids: list[int]) -> bytes:
+        return self._t.decode(list(ids))
 
     def __len__(self) -> int:
         return len(self._t)
