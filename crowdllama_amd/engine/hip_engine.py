@@ -60,6 +60,8 @@ class HipEngine(EngineBase):
 
     # ------------------------------------------------------------ generate
 
+    STRIDE = 32   # decode steps between looks at the tokens
+
     def _budget(self, prompt: str, max_new_tokens: int):
         """Clamp max_new to the sequence/ring budget (matching
         BatchingHipEngine); reject only when the PROMPT itself does not fit
@@ -99,9 +101,13 @@ class HipEngine(EngineBase):
                     out.append(tok_id)
                     self.eng.set_cur_token(0, tok_id)
             else:
-                if n_new > 1:
-                    self.eng.decode(n_new - 1)
+                # in strides: a request may end long before its limit
                 out = list(self.eng.gen_tokens(0))
+                while len(out) < n_new:
+                    if self.tok.eos_id in out[-self.STRIDE:]:
+                        break
+                    self.eng.decode(min(self.STRIDE, n_new - len(out)))
+                    out += self.eng.gen_tokens(0, len(out))
             if self.tok.eos_id in out:
                 out = out[: out.index(self.tok.eos_id)]
                 reason = "stop"

@@ -141,3 +141,18 @@ def test_harvest():
             assert not any(c.done_reason for c in req.chunks[:-1])
     assert not any(e.eng.active)
     assert e.eng.handed <= sum(len(tokens(t)) + 8 for t in texts)
+
+
+@pytest.mark.parametrize("limit", [5000, 70, 33, 32, 2, 1])
+@pytest.mark.parametrize("text", [TEXT * 30, TEXT, "x" * 31, ""])
+def test_greedy(limit, text):
+    """A request that ends early does not hold the engine to its limit."""
+    e = hip([tokens(text)])
+    r = e._generate_sync("hello", limit)
+    want = tokens(text)[:limit]
+    ended = EOS in want
+    assert r.text == e.tok.decode(want)
+    assert r.tokens_generated == len(want) - ended
+    assert r.done_reason == ("stop" if ended else "length")
+    assert len(want) - 1 <= e.eng.steps < len(want) + e.STRIDE
+    assert e.eng.steps <= limit - 1
