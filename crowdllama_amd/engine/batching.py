@@ -92,6 +92,10 @@ class BatchingHipEngine(EngineBase):
         # behind a saturated engine (gateway failover retries elsewhere)
         self._queue: "queue.Queue[_Req]" = queue.Queue(maxsize=8 * batch)
         self._slots = [_Slot() for _ in range(batch)]
+        # a slot without a request is parked: with kv_keep it would fill its
+        # cache, attend to all of it and evict, for nothing
+        for i in range(batch):
+            self.eng.set_slot_active(i, False)
         self._wake = threading.Event()
         self._stop = False
         self._active = 0
@@ -115,6 +119,10 @@ class BatchingHipEngine(EngineBase):
             slot.collected = 0
             slot.text, slot.parts = TextStream(self.tok), []
             self._active += 1
+
+    def _park(self, i: int) -> None:
+        self.eng.set_slot_active(i, False)
+        self.eng.reset_slot(i)
 
     def _harvest(self) -> None:
         for i, slot in enumerate(self._slots):
@@ -150,8 +158,7 @@ class BatchingHipEngine(EngineBase):
                     done_reason=reason))
                 slot.req = None
                 self._active -= 1
-                self.eng.set_slot_active(i, False)
-                self.eng.reset_slot(i)
+                self._park(i)
             elif delta:
                 req.push(GenerateResult(text=delta, tokens_generated=count,
                                         done_reason=""))
@@ -169,7 +176,7 @@ class BatchingHipEngine(EngineBase):
             except Exception as e:  # noqa: BLE001
                 # fatal engine error: fail every waiting request instead of
                 # leaving their futures hanging, then keep serving new ones
-                for slot in self._slots:
+                for i, slot in enumerate(self._slots):
                     req, slot.req = slot.req, None
                     if req is None:
                         continue
@@ -178,6 +185,10 @@ class BatchingHipEngine(EngineBase):
                     if not req.future.done():
                         req.future.set_exception(RuntimeError(
                             f"batch engine error: {e}"))
+                    try:
+                        self._park(i)
+                    except Exception:  # noqa: BLE001  the engine is gone
+                        pass
 
     # --------------------------------------------------------------- api
 

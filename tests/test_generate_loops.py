@@ -156,3 +156,58 @@ def test_greedy(limit, text):
     assert r.done_reason == ("stop" if ended else "length")
     assert len(want) - 1 <= e.eng.steps < len(want) + e.STRIDE
     assert e.eng.steps <= limit - 1
+
+
+@pytest.mark.parametrize("gone", [False, True])
+def test_a_failed_step_parks_the_slots(gone):
+    """Every request hears of it, and no slot goes on without one."""
+    e = batching([tokens(TEXT), tokens(TEXT)])
+    e._stop, e._admit = False, lambda: None
+
+    def decode(n):
+        e._stop = True
+        raise RuntimeError("step")
+    e.eng.decode = decode
+    if gone:
+        def park(slot, on):
+            raise RuntimeError("gone")
+        e.eng.set_slot_active = park
+    reqs = [_Req(ids=[1], max_new=9) for _ in e._slots]
+    for i, (slot, req) in enumerate(zip(e._slots, reqs)):
+        e.eng.prefill_slot(i, req.ids)
+        slot.req = req
+    e._loop()
+    for req in reqs:
+        with pytest.raises(RuntimeError, match="step"):
+            req.future.result(timeout=0)
+    assert e._active == 0 and e.eng.active == [gone, gone]
+
+
+@pytest.mark.gpu
+def test_idle_slots_stay_empty(tmp_path):
+    """One request of four slots' engine, twice its cache: the others neither
+    fill theirs nor evict, before and after."""
+    import asyncio
+    from crowdllama_amd.models import write_synthetic_gguf
+    path = write_synthetic_gguf(str(tmp_path / "t.gguf"), "testllama",
+                                scheme="f32", mode="exact", seed=11)
+    eng = BatchingHipEngine("m", path, batch=4, max_seq=64, kv_keep=40,
+                            kv_recent=8)
+
+    def empty():
+        # a slot is parked right after its request is told
+        for _ in range(100):
+            if eng.eng.kv_lens() == eng.eng.n_past() == [0] * 4:
+                return True
+            time.sleep(0.01)
+        return False
+    try:
+        asyncio.run(eng.generate("hello", 150))
+        assert empty()
+        async def go():
+            await asyncio.gather(eng.generate("hello", 150),
+                                 eng.generate("there", 30))
+        asyncio.run(go())
+        assert empty()
+    finally:
+        asyncio.run(eng.close())
