@@ -61,12 +61,14 @@ def build(verbose: bool = True, force: bool = False) -> str:
     for src in SOURCES:
         obj = os.path.join(OPS_DIR, "build", src.rsplit(".", 1)[0] + ".o")
         objs.append(obj)
-        cmd = [hipcc, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC",
+        # (hipcc takes a .cpp for HIP too, and testutil.cpp has a kernel)
+        cmd = [hipcc, *HIP_FLAGS, f"--offload-arch={ARCH}", "-O3",
+               "-std=c++17", "-fPIC",
                *(["-DCLA_PERF_PROBE_NOATOMIC"] if os.environ.get("CLA_PROBE") else []),
                "-I", CSRC, "-I", py_inc, "-I", pybind11.get_include(),
                "-c", os.path.join(CSRC, src), "-o", obj]
         if src.endswith(".hip"):
-            cmd[1:1] = ["-x", "hip", *HIP_FLAGS, *FILE_FLAGS.get(src, [])]
+            cmd[1:1] = ["-x", "hip", *FILE_FLAGS.get(src, [])]
         if verbose:
             print("[ops.build]", " ".join(cmd), file=sys.stderr)
         procs.append(subprocess.Popen(cmd, stdout=subprocess.PIPE,
