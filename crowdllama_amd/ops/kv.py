@@ -185,16 +185,16 @@ def _pages_slowly(pool, table, layers: bool):
         _TYPES[pool.dtype], dev.index)
 
 
-def _vector(t, name: str, n: int, dev):
+def _vector(t, name: str, n: int, dev, dtype=torch.int32):
     try:
-        if (t.dtype is torch.int32 and t.shape == (n,) and t.stride() == (1,)
+        if (t.dtype is dtype and t.shape == (n,) and t.stride() == (1,)
                 and t.device == dev):
             at = t.data_ptr()
             if at:
                 return at
     except (AttributeError, TypeError):
         pass
-    _on(t, name, torch.int32, 1, dev)
+    _on(t, name, dtype, 1, dev)
     if t.shape[0] != n:
         _fail(f"{name} must have {n} values, not {t.shape[0]}")
     _dense(t, name, 1)
@@ -399,13 +399,8 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
         _fail(f"without starts there must be one row for each of {slots} "
               f"sequences, not {rows}")
     st = 0 if starts is None else _vector(starts, "starts", slots + 1, dev)
-    fr = 0
-    if inv_freq is not None:
-        _on(inv_freq, "inv_freq", torch.float32, 1, dev)
-        _dense(inv_freq, "inv_freq", 1)
-        if inv_freq.shape[0] != dim // 2:
-            _fail(f"inv_freq must have {dim // 2} values")
-        fr = _memory(inv_freq, "inv_freq")
+    fr = 0 if inv_freq is None else _vector(inv_freq, "inv_freq", dim // 2,
+                                            dev, torch.float32)
     ms = ps = _NONE
     if mass is not None:
         ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
