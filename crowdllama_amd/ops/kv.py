@@ -417,7 +417,7 @@ def append(k, v, pool, table, lens, next_pos, *, q=None, inv_freq=None,
             ("table", table, kv[3]), ("lens", lens, le),
             ("next_pos", next_pos, np), ("starts", starts, st),
             ("inv_freq", inv_freq, fr)))
-    _plain(k, v, q, pool, mass, inv_freq)
+    _plain(k, v, q, pool, mass, inv_freq, over)
     _get(dev).kv_append(kv, kh, vh, qh, qo, q_heads, _TYPES[k.dtype], rows,
                         st, le, np, fr, ms, ps, reach, _stream(dev))
     return q_out
@@ -444,19 +444,19 @@ def attend(q, pool, table, lens, *, mass=None, scale=None, out=None):
     if mass is not None:
         ms = _places(mass, "mass", torch.float32, (slots, heads), reach, dev)
         reach = mass.shape[-1]
-    given = out is not None
-    if not given:
+    given = out
+    if given is None:
         out = q.new_empty((slots, q_heads, dim))
         oh = (out.data_ptr(), q_heads * dim, dim)
     else:
         oh = _heads(out, "out", slots, q_heads, dim, q.dtype, dev)
         _apart(out, "out")
     le, scale = _vector(lens, "lens", slots, dev), _scale(scale, dim)
-    if given:
+    if given is not None:
         _over(out, "out", (
             ("q", q, qh[0]), ("pool", pool, kv[0]), ("mass", mass, ms[0]),
             ("table", table, kv[3]), ("lens", lens, le)))
-    _plain(q, pool, mass)
+    _plain(q, pool, mass, given)
     core = _get(dev)
     ws = _workspace(core.kv_attend_workspace(kv, q_heads, reach,
                                              mass is not None), table)
@@ -542,7 +542,6 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
         _fail("layers x sequences x kv heads must be below 2^22")
     le = _vector(lens, "lens", slots, dev)
     np = _vector(next_pos, "next_pos", slots, dev)
-    _plain(pool, mass)
     spans = [_ends(mass), _ends(pos), _ends(lens)]
     if out is None:
         mass_out, pos_out, lens_out = mass, pos, lens
@@ -560,6 +559,7 @@ def evict(pool, table, lens, next_pos, mass, pos, *, keep, recent=0,
             spans.append(_ends(pos_out))
         if lo != le:
             spans.append(_ends(lens_out))
+    _plain(pool, mass, mass_out)
     if np != le or lo == le:       # both are only read, else
         spans.append(_ends(next_pos))
     spans.sort()

@@ -283,3 +283,18 @@ def test_scales_that_float32_does_not_hold(core, op):
     for scale in (2.0 ** -126, 1, 2.0 ** 127):
         op(t, scale=scale)
         assert core.calls[-1][1][-3] == scale
+
+
+def test_outputs_with_a_gradient_are_refused(core):
+    """They would be written behind autograd's back."""
+    t = tensors()
+    grad = lambda x: (x + 0).requires_grad_()  # noqa: E731
+    for call in (lambda: append(t, q_out=grad(t["q"])),
+                 lambda: attend(t, out=grad(t["q"])),
+                 lambda: evict(t, out=(grad(t["masses"]), t["places"],
+                                       t["lens"]))):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    assert len(core.calls) == 3
