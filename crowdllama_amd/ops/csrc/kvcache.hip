@@ -254,8 +254,8 @@ __device__ __forceinline__ void store8(void* p, int64_t at, const float* x) {
 // by side), 8 elements a thread and pass; the row's angles are shared by all
 // heads through LDS. position * inv_freq is taken and reduced in 64 bits: in
 // 32 it would be off by 2^-24 of the angle, 0.06 rad at position 10^6.
-// Bound by memory: 8632 rows of 32 + 16 heads of 128 (177 MB) take 30 us, 5.9
-// TB/s; few rows by latency (3.6 us).
+// Bound by memory: 7203 rows of 32 + 16 heads of 128 (177 MB) take 37.6 us, 4.7
+// TB/s, nearly a large copy's rate; few rows by latency (3.4 us).
 template <KVT T, KVT C, int D>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     __shared__ float cs[D / 2], sn[D / 2];
@@ -346,11 +346,11 @@ constexpr int UNIT = TILE * WAVES;
 
 // How many workgroups the whole of the batch's places are split into, about:
 // two a CU, which stream as fast as more and leave less to join (one sequence
-// of 131071 places: 124 us, 128 with 2048). With as many rows (sequences x kv
-// heads) as CUs most rows would stay whole, and the CUs that get long ones
-// finish late: finer parts even that out (16 x 32 rows of up to 8191 places:
-// 175 us, 212 with 512; 64 x 4 of up to 4096: 40 us, 43 with 512; but 16 x 8
-// of up to 4096: 32 us, 28 with 512).
+// of 131071 places: 125 us, 133 with 2048; 16 x 8 rows of up to 4096: 33 us, 35
+// with 2048). With as many rows (sequences x kv heads) as CUs most rows would
+// stay whole, and the CUs that get long ones finish late: finer parts even that
+// out (16 x 32 rows of up to 8191 places: 172 us, 208 with 512; 64 x 4 of up to
+// 4096: 50 us, 55 with 512).
 inline int attend_target(const KvPages& kv) {
     return (int64_t)kv.slots * kv.kv_heads >= 256 ? 2048 : 512;
 }
@@ -628,11 +628,11 @@ __device__ __forceinline__ void give(const Softmax<D>& x, int n, int g,
 // a time in turn.
 //
 // Bound by the reads of K and V: one sequence of 131071 places of 8 kv heads of
-// 128 (537 MB) takes 95 us without a mass, 5.6 TB/s, as fast as a stream that
-// is only read. Its scores go out as they are where a mass is wanted, since the
-// weights are known only once all parts are; those 17 MB cost another 15 us.
-// The products take a third of that (three pieces), so loading a tile ahead
-// gains nothing (119 us for 112).
+// 128 (537 MB) takes 102 us without a mass, with its join, 5.3 TB/s; a stream
+// that is only read reaches 5.5. Its scores go out as they are where a mass is
+// wanted, since the weights are known only once all parts are; those 17 MB, out
+// and back, cost another 23 us. The products take a third of that (three
+// pieces), so loading a tile ahead gains nothing (119 us for 112).
 template <class C, int NQ, int NP, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
     __shared__ float s_m[WAVES][16], s_l[WAVES][16];
@@ -706,8 +706,8 @@ __global__ __launch_bounds__(256) void k_kv_attend(AttendArgs a) {
 
 // Short rows, grid (kv heads, slots): eight waves take all of a row's places,
 // and its mass in the same launch, from scores in LDS. Bound by what one CU can
-// have under way, about 2.4 us for each 256 places of heads of 128; the next
-// tile's loads ahead of a tile's products gain nothing.
+// have under way (601 places of heads of 128: 11.7 us); the next tile's loads
+// ahead of a tile's products gain nothing.
 constexpr int ROW_WAVES = 8, ROW_PLACES = 1024;
 
 template <class C, int NQ, int NP, int D, bool MASS>
@@ -775,8 +775,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void k_kv_attend_row(
 
 // Join the parts: the same workgroups once more. Each makes its share of the
 // head's outputs (the parts' sums, in their order) and, from the scores, the
-// weights of its own places. Latency and the scores' 17 MB: 10.8 us for the
-// sequence above, 5 us for one of 601 places.
+// weights of its own places. Latency and the scores' 17 MB: 10.7 us for the
+// sequence above.
 template <class C, bool F32OUT, int D, bool MASS>
 __global__ __launch_bounds__(256) void k_kv_join(AttendArgs a) {
     __shared__ float s_m[16], s_r[16];
@@ -885,9 +885,9 @@ Div div_by(int d) {
 
 // Groups of 16 places that a wave of the second pass holds, where there is
 // work for many. Three leave room for a third wave a SIMD with heads of 128 and
-// one piece (8192 rows of 32 heads: 345 us, 422 with four); more pieces have
-// more to do for each row that is read (3 x 500 rows over 16000 places: 307 us,
-// 355 with three).
+// one piece (8192 rows of 32 heads, both passes: 633 us, 653 with four); more
+// pieces have more to do for each row that is read (3 x 500 rows over 16000
+// places: 466 us, 482 with three).
 constexpr int obs_groups(bool one_piece, int dim) {
     return one_piece && dim == 128 ? 3 : 4;
 }
@@ -1031,11 +1031,11 @@ __device__ __forceinline__ void store_sum(const ObserveArgs& a, const Seq& s,
 //
 // A score costs a multiplication, an exponential and an addition: 16 + 32 + 16
 // cycles of the SIMD for 4 x 64 of them, beside 64 of matrix products, which
-// run at the same time in part. 355 us for 8192 rows of 32 heads (275 GFLOP).
+// run at the same time in part. 312 us for 8192 rows of 32 heads (275 GFLOP).
 //
-// Three waves a SIMD for one piece (375 us for 8192 rows of 32 heads, 442 with
-// two), two for three (249 us for 3 x 500 rows over 16000 places, 290 with
-// three waves, which spill).
+// One piece leaves room for three waves a SIMD; with three pieces they would
+// spill (both passes for 3 x 500 rows over 16000 places: 466 us with two waves,
+// 502 with three).
 template <class C, int NQ, int D, int RW>
 __global__ __launch_bounds__(256, NQ > 1 ? 2 : 3) void k_kv_observe_sums(
     ObserveArgs a) {
@@ -1353,9 +1353,10 @@ __global__ __launch_bounds__(256) void k_kv_observe_mass(ObserveArgs a) {
     const int G = a.group.d;
     // chunks differ in their work (late ones are seen by more places, short
     // sequences have less): turned by one from block to block and from head to
-    // head, so that no XCD (every eighth workgroup) gets the long ones (4 x 282
-    // float32 rows: 48 us, 61 turned by block alone, 62 by an arbitrary amount a
-    // block; 7 x 251 rows of 32 kv heads 168, 178 and 170, 275 not turned)
+    // head, so that no XCD (every eighth workgroup) gets the long ones (both
+    // passes for 7 x 251 rows of 32 kv heads: 270 us, 279 turned by block alone,
+    // 370 not turned; 4 x 282 float32 rows of 8: 89, 104 and 85; 3 x 500 over
+    // 16000 places: 466, 461 and 469)
     const int block = blockIdx.x / a.chunks;
     const int at = (blockIdx.x + block + head) % a.chunks;
     Seq s{};
@@ -1614,12 +1615,13 @@ __device__ __forceinline__ WaveSums wave_sums(uint32_t x, uint32_t* red,
 // wave counts its free places and those that come into them, and numbers them
 // on from the counts of the waves before it.
 //
-// NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of 8192: 22 us, 24
-// with KPT 32, 38 with 0), 32 up to 32768 (128 of 20000: 43 us, 87 with 0).
-// NT 256, KPT 8 up to 2048 places (2304 rows of 318: 17 us, 68 with 1024
-// threads; 192 of 2048: 13.5 us either way). Bound by the counting: keys of one
+// With the moves, NT 1024: KPT 8 serves rows of up to 8192 places (256 rows of
+// 8192: 131 us, 133 with KPT 32, 145 with 0), 32 up to 32768 (128 of 20000: 170
+// us, 215 with 0). NT 256, KPT 8 up to 2048 places (2304 rows of 318: 26 us, 66
+// with 1024 threads; 8 of 512: 11.3, 13.5; 192 of 2048: 23 either way). The 256
+// rows of 8192 are selected in 22.6 us, bound by the counting: keys of one
 // exponent meet in few digits (the first one's lanes are added at once). Two
-// bits a round, by ballots over three candidates, takes 28 us for 256 x 8192.
+// bits a round, by ballots over three candidates, took 28.
 template <int NT, int KPT>
 __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
     constexpr int NW = NT / 64;
@@ -1804,7 +1806,7 @@ __global__ __launch_bounds__(NT) void k_kv_evict_select(EvictArgs a) {
 // Pass 2, grid (rows, blocks of moves): the movers' keys and values, 16
 // lanes a row. Sources are at or above keep and destinations below it, so
 // no order is needed. 2048 places of 256 rows (537 MB read and written) take
-// 100 us, the rate of a large copy.
+// 108 us, the rate of a large copy.
 __global__ __launch_bounds__(256) void k_kv_evict_move(EvictArgs a, int dim) {
     const int row = blockIdx.x;
     const int h = row % a.kv_heads, b = row / a.kv_heads % a.slots,
@@ -1920,10 +1922,10 @@ int64_t attend_wgs(const KvPages& kv, int reach) {
                     rows * std::max(1, (reach + UNIT - 1) / UNIT));
 }
 // Whether a row's places, which `reach` bounds, are one workgroup's: one launch
-// and no join then take less time than more workgroups save. 8 rows of 300
-// places 9 us, 13.5 in parts; 64 of 700, 13 and 13; 8 of 1000, 16 and 12.5; 128
-// of 1000, 18 and 19.5; 256 of 1000, 18 and 25; 1024 of 300, 21 and 26; but
-// 2048 of 200, 45 and 37 (its LDS leaves a CU one workgroup).
+// and no join then take less time than more workgroups save. 8 rows of up to 300
+// places 8.8 us, 12.1 in parts; 64 of 700, 14 and 14; 8 of 1000, 15.4 and 12.1;
+// 128 of 1000, 17 and 19.5; 256 of 1000, 19 and 28; 1024 of 300, 36 and 38; but
+// 2048 of 200, 61 and 52 (its LDS leaves a CU one workgroup).
 bool attend_rows(const KvPages& kv, int reach) {
     const int64_t rows = (int64_t)kv.slots * kv.kv_heads;
     return rows <= 1024 && reach <= (rows < 128 ? 768 : ROW_PLACES);
@@ -2004,12 +2006,12 @@ struct ObserveCut {
 };
 
 // Rows of a workgroup of the first pass in its form for few rows; 0: the other
-// form. For few rows a sequence on average (4 rows of 8 sequences of up to 3867
-// places, 32 kv heads: 27 us, 69 in the other form; 16 x 4 rows over 131071
-// places, 8 kv heads: 56 us, 79), and where the other form would not have 256
-// workgroups (4 x 100 x 4 rows, 500 places, 8 kv heads: 13 us, 19 in the other
-// form; 500 rows, 2000 places, 16 heads of 64: 13 us, 16; with more of them it
-// loses, 512 x 4 rows over 8000 places: 98 us, 50).
+// form. For few rows a sequence on average (both passes for up to 4 rows of 8
+// sequences of up to 3867 places, 32 kv heads: 86 us, 120 in the other form; 16
+// x 4 tokens of 32 / 8 heads over up to 131071 places: 1147 us, 1472), and where
+// the other form would not have 256 workgroups (4 x 100 tokens over 500 places:
+// 26 us, 32 in the other form; 500 rows, 2000 places, 16 heads of 64: 28 us, 33;
+// with more of them it loses, 512 tokens over 8000 places: 142 us, 97).
 int64_t observe_few(const KvPages& kv, int q_heads, int rows, int reach,
                     KVT type) {
     const int64_t R = (int64_t)rows * (q_heads / kv.kv_heads);
@@ -2039,10 +2041,10 @@ ObserveCut observe_cut(const KvPages& kv, int q_heads, int rows, int reach,
     c.part = up(up(places, c.parts), 64) * 64;
     c.parts = up(places, c.part);
     // Two groups of 16 places a wave where that many workgroups' worth of
-    // tiles of 64 rows would leave most of the chip idle (300 x 4 float32 rows
-    // of 8 kv heads: 9 us, 14 with four; 500 rows of 2000 places, 16 heads of
-    // 64: 9.5 us, 12 with four; 900 x 4 float32 rows, 1824 tiles: 35 us, 30
-    // with four).
+    // tiles of 64 rows would leave most of the chip idle (both passes for 300
+    // float32 tokens of 32 / 8 heads: 26 us, 30 with four; 500 rows of 2000
+    // places, 16 heads of 64: 28 us, 30.5 with four; 900 float32 tokens of 32 /
+    // 8 heads, 1824 tiles: 65 us, 60 with four).
     int64_t blocks;
     for (int groups : {obs_groups(type != KVT::F32, kv.dim), 2}) {
         c.block = 16 * WAVES * groups;
