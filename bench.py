@@ -5,8 +5,8 @@ Driver contract: `python bench.py --gpus N --steps K --warmup W`; for N>1
 launched via torch.distributed.run with one rank per GPU. One "step" = one
 decode iteration of the engine's whole batch (B tokens per step per GPU).
 Rank 0 prints ONE JSON line with the aggregate whole-job tokens/sec
-(BASELINE.json metric: "aggregate tokens/sec + p50 latency, llama3:8b Q4_K
-across 1/2/4/8 workers"); weights are random-init GGUF (no network for real
+(the metric: aggregate tokens/sec + p50 latency, llama3:8b Q4_K across
+1/2/4/8 workers); weights are random-init GGUF (no network for real
 checkpoints), prompts synthetic.
 """
 
@@ -33,22 +33,20 @@ def main() -> None:
     ap.add_argument("--model", default="llama3-8b")
     ap.add_argument("--scheme", default="q4_k_m")
     ap.add_argument("--mode", default="dp", choices=["dp", "tp", "serve"],
-                    help="dp: one replica worker per GPU (default; the "
-                         "driver's scaling bench). tp: ONE worker spanning "
+                    help="dp: one replica worker per GPU (default). tp: ONE worker spanning "
                          "all ranks via RCCL tensor parallelism "
-                         "(BASELINE config 4; e.g. --mode tp --model "
+                         "(e.g. --mode tp --model "
                          "llama3-70b --scheme bf16). serve: the FULL "
                          "serving path — DHT + worker (continuous "
                          "batching) + gateway /api/chat, concurrent HTTP "
-                         "clients, true request p50/p95 (BASELINE config "
-                         "2's metric)")
+                         "clients, true request p50/p95")
     ap.add_argument("--concurrency", type=int, default=32,
                     help="serve mode: concurrent in-flight HTTP requests")
     ap.add_argument("--models", default="",
                     help="serve mode: comma-separated models for a mixed "
                          "fleet (one worker per model on this GPU; "
-                         "requests round-robin across models — BASELINE "
-                         "config 5's model-aware routing)")
+                         "requests round-robin across models: model-aware "
+                         "routing)")
     ap.add_argument("--max-new", type=int, default=64,
                     help="serve mode: max_new_tokens per request")
     ap.add_argument("--batch", type=int, default=16,
@@ -179,7 +177,7 @@ def main() -> None:
             "p50_latency_ms": ms_per_step,  # per-token latency at this batch
             "higher_is_better": True,
             "scaling": "weak",
-            "vs_baseline": None,  # reference publishes no numbers (BASELINE.md)
+            "vs_baseline": None,  # reference publishes no numbers
             # act_q8: per-32-block int8 activations for quantized-weight
             # GEMMs — the same activation-quantization scheme llama.cpp's
             # MMQ path (the reference's compute backend) uses for these
@@ -204,11 +202,9 @@ def main() -> None:
 
 
 def serve_bench(args) -> None:
-    """BASELINE config 2 measured as specified: N concurrent /api/chat
+    """The serving path: N concurrent /api/chat
     requests through DHT + worker + gateway on loopback; reports aggregate
-    generated tokens/sec AND true request-level p50/p95 (the round-1 bench
-    drove the engine directly and reported ms_per_step as 'p50' — VERDICT
-    'What's weak' item 2)."""
+    generated tokens/sec AND true request-level p50/p95."""
     import asyncio
     import statistics
 
@@ -247,7 +243,7 @@ def serve_bench(args) -> None:
         dht_port = await dht.start("127.0.0.1", 0)
         boot = [f"127.0.0.1:{dht_port}"]
         # one worker per model, all on this GPU (288 GB HBM holds a mixed
-        # fleet; BASELINE config 5 runs 2 models with model-aware routing).
+        # fleet, e.g. 2 models with model-aware routing).
         # Per-request token budget rides the engine default max_new (the
         # PB GenerateRequest is reference-schema: model/prompt/stream).
         workers = []

@@ -1,6 +1,5 @@
 """CLI entry points (reference parity: cmd/crowdllama + cmd/dht — but a
-first-party CLI rather than the reference's re-skinned Ollama cobra tree,
-SURVEY.md §7.4).
+first-party CLI rather than the reference's re-skinned Ollama cobra tree).
 
     python -m crowdllama_amd.cli start [--worker-mode] [--models ...]
     python -m crowdllama_amd.cli dht [--port 9000]

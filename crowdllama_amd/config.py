@@ -2,7 +2,7 @@
 
 Three layers: defaults <- env (CROWDLLAMA_*) <- CLI flags. Unlike the
 reference, test-mode interval shrinking is a config field (`test_mode`)
-rather than env-sniffing scattered through library code (SURVEY.md §7.4).
+rather than env-sniffing scattered through library code.
 """
 
 from __future__ import annotations

@@ -53,8 +53,7 @@ class EngineBase:
                               temperature: float = 0.0):
         """Async iterator of GenerateResult chunks; `text` is the DELTA since
         the previous chunk, and exactly the last chunk has done_reason set
-        (capability extension over the reference — SURVEY.md §2.2 notes the
-        reference carries `stream` but never streams, gateway.go:243-293).
+        (capability extension over the reference: the reference carries `stream` but never streams, gateway.go:243-293).
         Default: one final chunk from the non-streaming path."""
         yield await self.generate(prompt, max_new_tokens, temperature)
 

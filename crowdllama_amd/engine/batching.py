@@ -65,8 +65,8 @@ class BatchingHipEngine(EngineBase):
         cfg.batch = batch
         cfg.max_seq = max_seq
         # size the generated-token ring from max_seq so a request's max_new
-        # can never exceed it (a request with
-        # max_new > gen_cap saturated the ring and decoded forever)
+        # can never exceed it (with max_new > gen_cap it would saturate the
+        # ring and decode forever)
         cfg.gen_cap = max_seq * EVICTING_GEN if kv_keep else max_seq
         # past max_seq by eviction, as HipEngine
         cfg.kv_keep, cfg.kv_recent = kv_keep, kv_recent

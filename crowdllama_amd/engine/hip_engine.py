@@ -65,7 +65,7 @@ class HipEngine(EngineBase):
     def _budget(self, prompt: str, max_new_tokens: int):
         """Clamp max_new to the sequence/ring budget (matching
         BatchingHipEngine); reject only when the PROMPT itself does not fit
-        — never truncate it silently (round-1 advisor finding)."""
+        — never truncate it silently."""
         ids = self.tok.encode(prompt)
         max_new = token_budget(max_new_tokens, len(ids), self.max_seq,
                                self.gen_cap, self.kv_keep)

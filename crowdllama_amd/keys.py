@@ -6,8 +6,7 @@ ed25519 seed (0600, dir 0700); the peer id is derived from the ed25519
 PUBLIC key (mesh/crypto.py peer_id_from_pub), so any peer shown the key
 can verify it hashes to the claimed id — and the mesh handshake
 (mesh/wire.py secure_open/secure_accept) proves possession of the private
-half. Round 1 used an unsigned digest pseudo-identity; this is the real
-keypair VERDICT item 3 asked for.
+half.
 """
 
 from __future__ import annotations

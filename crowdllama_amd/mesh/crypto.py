@@ -14,7 +14,7 @@ build environment has no `cryptography`/`nacl` wheels):
 - A SIGMA-style authenticated handshake binding the ephemeral exchange to
   both ed25519 identities; peer_id = hash of the ed25519 public key, so a
   dialer that knows a peer_id cryptographically verifies it is talking to
-  that peer (the round-1 mesh accepted any claimed peer_id).
+  that peer.
 - An encrypt-then-MAC secure channel over the existing 4-byte length
   framing: per-direction keys from BLAKE2b-HKDF, BLAKE2b keystream in
   counter mode, BLAKE2b-128 MAC, strictly increasing per-frame counters

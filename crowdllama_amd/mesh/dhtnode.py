@@ -3,7 +3,7 @@ Kademlia DHT server (pkg/dht/dht.go:25-437).
 
 The reference uses libp2p Kademlia purely as a rendezvous: workers
 `Provide` a namespace CID every second and consumers `FindProvidersAsync`
-it (SURVEY.md §3.4). This node implements those semantics directly over the
+it. This node implements those semantics directly over the
 mesh wire protocol: provider records with TTL expiry, peer-address lookup,
 connection stats logging, and eager eviction on disconnect
 (dht.go:370-383).
@@ -38,7 +38,7 @@ class DHTServer:
         # real cryptographic identity from the keyfile (the legacy second
         # argument is kept for compatibility but the advertised id is
         # always derived from the key — ids are now verifiable hashes of
-        # ed25519 public keys, VERDICT item 3). An embedded per-peer
+        # ed25519 public keys). An embedded per-peer
         # server passes the peer's own identity instead.
         self.identity = identity or load_identity("dht", cfg.key_path)
         self.peer_id = self.identity.peer_id

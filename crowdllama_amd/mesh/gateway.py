@@ -84,8 +84,7 @@ class Gateway:
 
     async def _discovery_loop(self) -> None:
         # gateway-side provider pull (reference gateway.go:351-423); unlike
-        # the reference this shares the peer's single PeerManager code path
-        # (deduplicate gateway-vs-peermanager discovery).
+        # the reference this shares the peer's single PeerManager code path.
         while True:
             try:
                 for res in await self.peer.discovery.discover_peers():

@@ -1,7 +1,7 @@
 """Protobuf wire schema for the inference protocol.
 
-Equivalent of the reference's external crowdllama-pb package (SURVEY.md
-§2.2: BaseMessage oneof{GenerateRequest, GenerateResponse}). Hand-rolled
+Equivalent of the reference's external crowdllama-pb package
+(BaseMessage oneof{GenerateRequest, GenerateResponse}). Hand-rolled
 proto3 wire-format codec (no protoc in the image); the bytes are valid
 protobuf, decodable by any proto library given the schema:
 
@@ -197,7 +197,7 @@ class GenerateResponse:
 
 @dataclass
 class BaseMessage:
-    """oneof envelope (reference BaseMessage, SURVEY.md §2.2)."""
+    """oneof envelope (reference BaseMessage)."""
     generate_request: GenerateRequest | None = None
     generate_response: GenerateResponse | None = None
 
@@ -230,7 +230,7 @@ def response_message(model: str, response: str, worker_id: str = "",
                      total_duration_ns: int = 0,
                      done: bool = True, eval_count: int = 0) -> BaseMessage:
     # done=False frames are streamed chunks (capability extension over the
-    # reference, which carries `stream` but never streams — SURVEY.md §2.2)
+    # reference, which carries `stream` but never streams)
     return BaseMessage(generate_response=GenerateResponse(
         model=model, created_at=Timestamp.now(), response=response, done=done,
         done_reason=done_reason if done else "", worker_id=worker_id,

@@ -282,7 +282,7 @@ class Peer:
             if req.stream:
                 # streamed chunks: one done=False frame per text delta, then
                 # a final done=True frame (extension over the reference,
-                # which reserves `stream` but never streams — SURVEY.md §2.2)
+                # which reserves `stream` but never streams)
                 total_tokens = 0
                 async for chunk in engine.generate_stream(
                         req.prompt, self.cfg.max_new_tokens):

@@ -1,6 +1,6 @@
 """Peer membership + scheduling (reference parity: pkg/peermanager/manager.go).
 
-Semantics carried over exactly (SURVEY.md §7.2 step 2): thread-safe registry
+Semantics carried over exactly: thread-safe registry
 with recently-removed tombstones, four background loops (discovery, metadata
 touch, health check, cleanup), health = reachability + metadata RTT with
 per-peer linear backoff `failed_attempts * backoff_base`, stale eviction

@@ -2,7 +2,7 @@
 
 Unlike the reference — which hardcodes "RTX 4090"/150 tok/s/24 GB
 (peer.go:319-343) — workers here fill these from real HIP device props and a
-measured rolling throughput (SURVEY.md §7.3 "throughput metadata honesty").
+measured rolling throughput.
 """
 
 from __future__ import annotations
@@ -31,7 +31,7 @@ class Resource:
     # consumers add it as a rendezvous target, so losing the bootstrap
     # node leaves N live servers, not one gossip fallback
     dht_addr: str = ""
-    # record authentication (VERDICT item 3): pubkey is the advertising
+    # record authentication: pubkey is the advertising
     # peer's ed25519 public key (hex); sig signs the canonical payload.
     # Receivers verify sig AND that peer_id == hash(pubkey), so a record
     # cannot be forged for another peer's id. (The reference relies on

@@ -92,8 +92,7 @@ async def accept_protocol(reader: asyncio.StreamReader,
 # agreement bound to ed25519 identities, then every frame sealed
 # (encrypt-then-MAC, per-direction keys, strict counters). The reference
 # gets the equivalent from libp2p's noise/TLS security transports
-# (reference internal/discovery/discovery.go:48-84); round 1 spoke
-# plaintext TCP and trusted any claimed peer_id.
+# (reference internal/discovery/discovery.go:48-84).
 
 import os as _os
 

@@ -1,7 +1,7 @@
 """Model-family presets (llama architecture family).
 
 The reference advertises/serves these model names (hardcoded list at
-reference pkg/peer/peer.go:322 and the BASELINE.json configs); here they map
+reference pkg/peer/peer.go:322) and a few common ones; here they map
 to real architecture hyperparameters used for synthetic random-init
 checkpoints and engine graph construction.
 """
@@ -47,7 +47,7 @@ def _reg(cfg: ModelConfig) -> ModelConfig:
     return cfg
 
 
-# BASELINE.json config models
+# models of the benchmarks
 _reg(ModelConfig("tinyllama", vocab_size=32000, hidden_size=2048, n_layers=22,
                  n_heads=32, n_kv_heads=4, ffn_hidden=5632,
                  rope_theta=10000.0, max_seq_len=2048))

@@ -1,7 +1,6 @@
 """Synthetic random-init GGUF checkpoint generation.
 
-There is no network access for real checkpoints ("synthetic
-prompts / random-init GGUF weights"), so benches and tests generate
+There is no network access for real checkpoints, so benches and tests generate
 random-init GGUF files of the real architectures.
 
 Two modes:

@@ -2,8 +2,7 @@
 
 Invoked by setup.py, __graft_entry__.build(), and lazily on first import
 attempt. hipcc cross-compiles on CPU-only boxes; the resulting .so travels
-with the repo snapshot to GPU boxes (it is git-ignored but NOT
-gpurun-ignored).
+with a copy of the tree to GPU machines (it is git-ignored).
 """
 
 from __future__ import annotations

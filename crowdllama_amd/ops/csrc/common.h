@@ -179,8 +179,8 @@ __host__ __device__ inline int64_t i8g_rawb(DT t) {
 // GEMM-tiled weight copy: [ceil(N/128)][K/64][128 rows][RAWB] — each
 // (n-block, k-window) tile is contiguous (= the kernel's LDS image), so
 // the weight DMA reads whole cachelines. The row-major qs layout reads
-// only 32 B per 128 B line at BK=64 windows (4x HBM over-fetch — the
-// round-2 ~1.5 TB/s wall on both GEMM kernels). Rows past N are zeros.
+// only 32 B per 128 B line at BK=64 windows (4x HBM over-fetch — a
+// ~1.5 TB/s wall on both GEMM kernels). Rows past N are zeros.
 __host__ __device__ inline int64_t dqs2_bytes(DT t, int64_t n, int64_t k) {
     if (t != DT::DQ4K && t != DT::DQ8 && t != DT::DQ6K) return 0;
     const int64_t nb = (n + I8G_BN - 1) / I8G_BN;

@@ -516,7 +516,7 @@ void Engine::alloc_state() {
     const int NH = meta_.heads_l, NKV = meta_.kv_heads_l, D = meta_.head_dim;
     const int F = meta_.ffn_l;
     // KV split count: 256/(B*NKV) with a floor of 2 up to B=32 — S=2 at
-    // B=16 measured best with the round-2 i8 GEMM step (4548 vs 4396
+    // B=16 measured best with the i8 GEMM step (4548 vs 4396
     // tok/s at S=4), B=32 regressed at S=1 (5549 vs 6260 at S=2), and
     // B=64 has enough workgroups without splits
     attn_splits_ = std::max(1, std::min(32, 256 / std::max(1, B * NKV)));
@@ -783,8 +783,8 @@ static void gemv_pick(bool act_q8, const WTensor& w, int pre,
 
 void Engine::reset_slot(int slot) {
     // async on the engine stream: ordered behind any in-flight decode work,
-    // no host serialization (per-stride sync memcpys here
-    // serialized the batcher thread against the stream).
+    // no host serialization (per-stride sync memcpys here would serialize
+    // the batcher thread against the stream).
     kv_host_.at(slot) = 0;
     HIP_CHECK(hipMemsetAsync(n_past_ + slot, 0, 4, stream_));
     HIP_CHECK(hipMemsetAsync(gen_count_ + slot, 0, 4, stream_));
@@ -924,7 +924,7 @@ void Engine::step(hipStream_t s) {
     if (!gemv_path && (meta_.layers & 1)) xfinal = x2_;
     // TP: each rank computes its compact [B][vocab_l] slice, ONE all-gather
     // of B*vocab_l moves every slice, then a scatter kernel restores the
-    // [B][V] layout (B separate per-row collectives).
+    // [B][V] layout (instead of B separate per-row collectives).
     float* lg = tp ? logits_tp_ : logits_;
     const int ldl = tp ? meta_.vocab_l : meta_.vocab;
     if (gemv_path) {
@@ -966,8 +966,8 @@ void Engine::ensure_graph() {
     if (graph_exec_ || !cfg_.use_graph) return;
     // warm-up eager step is NOT run here; capture directly (all state is
     // device-resident, shapes static). Capture of in-graph RCCL collectives
-    // (tp>1) is the finicky case SURVEY §7.3 flags: on any capture failure
-    // fall back to eager stepping instead of dying.
+    // (tp>1) is the finicky case: on any capture failure fall back
+    // to eager stepping instead of dying.
     hipGraph_t graph = nullptr;
     try {
         // Relaxed: other engines in the process (mixed-fleet serving

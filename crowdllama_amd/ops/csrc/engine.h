@@ -26,13 +26,13 @@ struct EngineConfig {
     bool use_graph = true;
     int prefill_chunk = 1024;  // prompt tokens per prefill GEMM pass
     // tensor parallelism over RCCL/xGMI (capability extension; the
-    // reference has no collectives at all — SURVEY.md §2.3)
+    // reference has no collectives at all)
     int tp_rank = 0;
     int tp_size = 1;
     // int8-quantized activations (per-32 symmetric; semantics replicated
     // by ref_numpy(act_q8=True)) for quantized-weight GEMMs — the
     // v_mfma_i32 batched-decode path (gemm_i8.hip). Default ON: measured
-    // +33% at B=16 over the bf16-staging GEMM (round 2). Exact-f32
+    // +33% at B=16 over the bf16-staging GEMM. Exact-f32
     // comparisons (tests) set this false.
     bool act_q8 = true;
     // int8-activation GEMV (v_dot4) for the B=1 decode path. Off: measured

@@ -641,8 +641,8 @@ static int splitk_target(int M) {
 // Single source of truth for the split-K factor: launch_gemm_ex and
 // gemm_uses_splitk (which tells the caller whether C must be pre-zeroed
 // for the atomicAdd accumulation) MUST agree exactly — a mismatch for any
-// M range means accumulating into stale scratch (
-// M=33..128 prompts silently corrupted activations).
+// M range means accumulating into stale scratch and silently
+// corrupted activations.
 int gemm_splitk_factor(int N, int K, int M) {
     // split-K applies to the decode/short-prefill range; beyond it there
     // are enough (bm x n) tiles to fill the chip without it

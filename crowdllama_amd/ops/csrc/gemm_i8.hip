@@ -24,7 +24,7 @@
 //   read serves both K=32 halves (lo/hi nibble planes of the same bytes).
 //
 // Replaces (functionally) llama.cpp's MMQ path for batched decode — the
-// compute the reference delegates to Ollama (SURVEY.md §2.3); designed for
+// compute the reference delegates to Ollama; designed for
 // CDNA4 wave64/XCD/LDS-DMA geometry, not ported.
 #include "common.h"
 
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256) void k_gemm_i8(
     // ---- W source: the GEMM-tiled qs2 copy (common.h) — each (n-block,
     // k-window) tile is contiguous and identical to the LDS image, so a
     // wave's DMA covers whole cachelines (the row-major layout read only
-    // 32 of every 128 B here: the round-2 bandwidth wall).
+    // 32 of every 128 B here).
     const int64_t ktiles = K / BK;
     const uint8_t* wtile0 = qs2 + (int64_t)bn * ktiles * (BN * RAWB);
     // cooperative (XSHARED) source/dest; private: slice by wn, copy by wid
@@ -539,8 +539,7 @@ bool gemm_i8_supported(DT dtype, int M, int K) {
     // (template above) but measured SLOWER than both the BM=32-with-
     // re-read i8 path (B=64: 4458 vs 8338 tok/s) and the bf16 prefill
     // kernel for 1024-row chunks (prefill 1541 vs 1382 ms at 16x1024) —
-    // its 20 KB/buffer LDS footprint halves occupancy. Kept unselected;
-    // see docs/PERF_NOTES.md round-2 notes.
+    // its 20 KB/buffer LDS footprint halves occupancy. Kept unselected.
     return (dtype == DT::DQ4K || dtype == DT::DQ8 || dtype == DT::DQ6K) &&
            M <= 128 && K % BK == 0 && K % 256 == 0;
 }

@@ -1,6 +1,6 @@
 // Minimal C++ GGUF v3 reader: mmap the file, parse metadata + tensor table.
 // (MI355X-native replacement for the GGUF loading the reference delegates to
-// Ollama/llama.cpp — SURVEY.md §2.3 row "GGUF loader".)
+// Ollama/llama.cpp.)
 #pragma once
 
 #include <cstdint>

@@ -1,7 +1,7 @@
 // HIP/CDNA4 (gfx950) kernels for the crowdllama-amd decode engine.
 //
 // MI355X-native replacements for the GGML compute the reference delegates to
-// Ollama/llama.cpp (SURVEY.md §2.3): fused dequant-GEMV (Q4_K/Q6_K/Q8_0),
+// Ollama/llama.cpp: fused dequant-GEMV (Q4_K/Q6_K/Q8_0),
 // RMSNorm + SwiGLU fused into GEMV activation staging, RoPE + paged-KV
 // append, split-KV online-softmax decode attention, embedding gather,
 // on-device greedy sampling.
@@ -457,9 +457,9 @@ __global__ __launch_bounds__(256) void k_gemv_q8(
             inv = rsqrtf((red[0] + red[1] + red[2] + red[3]) / (float)K + eps);
         }
         // lane-parallel block quantization: 8 lanes per 32-block, one
-        // float4 each, amax/sum via 8-lane shuffles. The round-1 per-thread
-        // version serialized ~120 dependent ops per block on at most half
-        // the threads (PERF_NOTES lever 2).
+        // float4 each, amax/sum via 8-lane shuffles. A thread
+        // per block would serialize ~120 dependent ops on at most half the
+        // threads.
         const int jl = tid & 7;   // lane within the block's 8-lane group
         for (int blk = tid >> 3; blk < NB32; blk += 32) {
             float4 v;
@@ -611,8 +611,8 @@ __global__ __launch_bounds__(256) void k_gemv_q8(
 //    (~33 vs 23 us: x re-staging there is L2-served and the stripe
 //    launches don't amortize), so it was removed; K > 4096 uses
 //    k_gemv_rl (K = 14336) or the legacy kernel.
-// Reference parity: same mat-vec the reference delegates to llama.cpp
-// (SURVEY.md §2.3); numerics = plain f32 dot of dequantized weights.
+// Reference parity: same mat-vec the reference delegates to llama.cpp;
+// numerics = plain f32 dot of dequantized weights.
 
 template <DT W, int P, int SEGF, int BB = 1>
 __global__ __launch_bounds__(256) void k_gemv_r(
@@ -1655,7 +1655,7 @@ __global__ __launch_bounds__(64) void k_argmax_final(
 // TP logits epilogue: undo the rank-major ncclAllGather layout in one
 // launch. src is [TP][B][Vl] (each rank's compact [B][Vl] slice gathered in
 // rank order), dst is [B][TP*Vl] global logits. One collective of B*Vl per
-// step instead of the round-1 per-batch-row loop (B collectives of Vl).
+// step instead of a loop over batch rows (B collectives of Vl).
 __global__ __launch_bounds__(256) void k_scatter_logits(
     const float* __restrict__ src, float* __restrict__ dst, int B, int Vl) {
     const int r = blockIdx.x, b = blockIdx.y;

@@ -251,8 +251,7 @@ double bench_gemv_g(int dtype, int N, int K, int B, int iters) {
 namespace cla {
 
 // 1-rank RCCL communicator + hipGraph-captured ncclAllReduce/ncclAllGather:
-// validates the graph-capture-of-collectives machinery (SURVEY §7.3 risk)
-// inside a 1-GPU lease. (TP>=2 on one device is impossible: RCCL rejects
+// validates the graph-capture-of-collectives machinery on one GPU. (TP>=2 on one device is impossible: RCCL rejects
 // duplicate devices per communicator — see tests/test_gpu_tp.py.)
 // Returns the buffer after 2 graph replays of (allreduce; allgather-self):
 // with 1 rank both are identity-ish copies, so out == in numerically.

@@ -1,5 +1,5 @@
 // Native tokenizer (reference parity: the C++ BPE/SPM tokenizer inside
-// llama.cpp that Ollama uses — SURVEY.md §2.3 row "Tokenizer").
+// llama.cpp that Ollama uses).
 // Byte-level BPE with merge ranks + <0xNN> byte-fallback vocabularies.
 #include <cstdint>
 #include <map>

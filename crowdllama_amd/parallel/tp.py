@@ -1,7 +1,6 @@
 """Tensor-parallel sharding plan for the llama family over RCCL/xGMI.
 
-Capability extension over the reference (which has no collectives at all —
-SURVEY.md §2.3: "Collectives / NCCL call sites: none exist"): one worker
+Capability extension over the reference (which has no collectives at all): one worker
 spanning N GPUs with row/column-sharded projections and RCCL all-reduce
 after attn-out and ffn-down, sized for 8x MI355X with 7 point-to-point xGMI
 links per GPU.

@@ -1,8 +1,7 @@
 """GGUF v3 container reader/writer (pure Python, numpy-backed).
 
-The north star keeps the reference ecosystem's GGUF checkpoint format (the
-reference's models are Ollama-managed GGUF files on the worker's disk —
-SURVEY.md §5.4). This module provides:
+Checkpoints are in the reference ecosystem's GGUF format (the reference's
+models are Ollama-managed GGUF files on the worker's disk). This module provides:
 
 - GGUFWriter: used by models/synth.py to emit random-init checkpoints for
   benches and tests.

@@ -1,8 +1,7 @@
 """CPU reference codecs for the GGUF quantization formats the engine serves.
 
 The byte layouts are the public GGML/GGUF on-disk formats (so checkpoints
-interoperate with the wider GGUF ecosystem, per the north-star requirement of
-keeping the GGUF checkpoint format). The quantizer here is a simple
+interoperate with the wider GGUF ecosystem). The quantizer here is a simple
 absmax/minmax fit — any valid encoding dequantizes correctly everywhere; we
 do not replicate llama.cpp's iterative scale search.
 

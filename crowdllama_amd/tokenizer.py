@@ -1,6 +1,5 @@
 """Tokenizer fed from the GGUF vocab section (reference parity: the C++
-tokenizer inside llama.cpp that Ollama uses — SURVEY.md §2.3 row
-"Tokenizer").
+tokenizer inside llama.cpp that Ollama uses).
 
 Two implementations with identical behavior:
 - Tokenizer: pure-Python reference (CPU tests, fallback),

@@ -1,10 +1,10 @@
-"""Bench the model/scheme matrix on one GPU (BASELINE configs)."""
+"""Bench the model/scheme matrix on one GPU."""
 import json
 import subprocess
 import sys
 
 CASES = [
-    ("tinyllama", "q8_0", 1, 128),     # BASELINE config 1 model (on GPU)
+    ("tinyllama", "q8_0", 1, 128),     # the smallest model (on GPU)
     ("llama3-8b", "q4_k_m", 1, 256),   # headline
     ("mistral-7b", "q4_k_m", 1, 256),
     ("llama3-8b", "q8_0", 1, 128),
